@@ -9,34 +9,47 @@ SRCS  := $(CSRC)/pclseg_kernels.h $(CSRC)/pclseg_graph.h $(CSRC)/pclseg_api.hip 
 # figure when the binary that ran was built from something else.  The shipped build has no switches, so its hash is the
 # hash of the sources alone; every stamps / tuning / variant build hashes differently and is never mistaken for it.
 sha = $(shell (cat $(SRCS); printf '%s' '$(strip $(1))') | sha256sum | cut -c1-16)
-HIPFLAGS := -O3 -std=c++17 --offload-arch=$(ARCH) -fPIC -shared -Wall -Wno-unused-function
+# the row operators (include/pclseg.h, second half) are a translation unit of their own: the forward pass's device kernels
+# stay the instruction streams that tests/golden/verified_kernels_r03.json names.  Packed float32 instructions are off in it
+# (the host pass does not know the feature and says so).
+OPS_SRCS := $(CSRC)/pclseg_ops.hip $(CSRC)/pclseg_rows.h $(CSRC)/pclseg_score.h $(CSRC)/pclseg_i8.h $(CSRC)/pclseg_status.h include/pclseg.h
+OPS_OBJ := build/pclseg_ops.o
+OPS_FLAGS := -Xclang -target-feature -Xclang -packed-fp32-ops
+HIPFLAGS := -O3 -std=c++17 --offload-arch=$(ARCH) -fPIC -Wall -Wno-unused-function
 # $(call hipbuild,<output>,<-D switches>)
-hipbuild = $(HIPCC) $(HIPFLAGS) $(2) -DPCLSEG_SRC_SHA=\"$(call sha,$(2))\" -o $(1) $(CSRC)/pclseg_api.hip
+define hipbuild
+$(HIPCC) $(HIPFLAGS) $(2) -DPCLSEG_SRC_SHA=\"$(call sha,$(2))\" -c -o build/$(notdir $(1:.so=.o)) $(CSRC)/pclseg_api.hip
+$(HIPCC) --offload-arch=$(ARCH) -shared -o $(1) build/$(notdir $(1:.so=.o)) $(OPS_OBJ)
+endef
 
 all: $(LIB)
 
-$(LIB): $(SRCS)
+$(OPS_OBJ): $(OPS_SRCS)
+	@mkdir -p build
+	$(HIPCC) $(HIPFLAGS) $(OPS_FLAGS) -c -o $@ $(CSRC)/pclseg_ops.hip
+
+$(LIB): $(SRCS) $(CSRC)/pclseg_status.h $(OPS_OBJ)
 	$(call hipbuild,$@,$(EXTRA))
 
 # the candidate kernel variants of pclseg_kernels.h (never run on an MI355X; NOT in the shipped library): the
 # hardware A/B of scripts/gpu_all.sh (step 4) loads this one through PCLSEG_DEBUG=1 PCLSEG_LIB=build/libpclseg_cand.so
-candidates: $(SRCS)
+candidates: $(SRCS) $(OPS_OBJ)
 	@mkdir -p build
 	$(call hipbuild,build/libpclseg_cand.so,-DPCLSEG_CAND $(EXTRA))
 
 # debug build with in-kernel phase timestamps (PCLSEG_STAMP=<layer>; loaded with PCLSEG_DEBUG=1 PCLSEG_LIB=build/libpclseg_stamps.so)
-stamps: $(SRCS)
+stamps: $(SRCS) $(OPS_OBJ)
 	@mkdir -p build
 	$(call hipbuild,build/libpclseg_stamps.so,-DPCLSEG_WITH_STAMPS $(EXTRA))
 
 # A/B build: the experiment switches of DESIGN.md §9/§10 (PCLSEG_GEOM, PCLSEG_DN8, ...) are read from the
 # environment; the shipped library carries only their defaults
-tuning: $(SRCS)
+tuning: $(SRCS) $(OPS_OBJ)
 	@mkdir -p build
 	$(call hipbuild,build/libpclseg_tuning.so,-DPCLSEG_TUNING $(EXTRA))
 
 # any other A/B build: make variant NAME=foo EXTRA="-DPCLSEG_..."  ->  build/libpclseg_foo.so
-variant: $(SRCS)
+variant: $(SRCS) $(OPS_OBJ)
 	@mkdir -p build
 	$(call hipbuild,build/libpclseg_$(NAME).so,$(EXTRA))
 

@@ -333,6 +333,73 @@ int pclseg_op_project_ex(const pclseg_proj_desc* desc, const float* points, int 
                          const int32_t* label_lut, int lut_size, float* image, int32_t* proj_idx,
                          uint64_t* scratch, void* hip_stream);
 
+/* ---- row operators: the 8-bit linear layer and the log probabilities of labels (csrc/pclseg_ops.hip).  Device pointers on
+ * the current device, handle-less, asynchronous on `hip_stream` (NULL = default stream); nothing is allocated, kept or
+ * synchronised, so every call can be captured into a graph.  Rows have unit element stride and any row stride; element
+ * alignment is enough.  A count of rows of 0 is no work and succeeds. */
+typedef enum pclseg_dtype { PCLSEG_F32 = 0, PCLSEG_BF16 = 1, PCLSEG_F16 = 2 } pclseg_dtype;
+
+#define PCLSEG_TOP_MAX 64      /* alternatives a row can be asked for */
+#define PCLSEG_I8_K_MAX 131071 /* 128 * 128 * k stays below 2^31 */
+
+/* Bytes a row of k codes takes: k rounded up to 64, and to 128 above 64.  0 for k outside [1, PCLSEG_I8_K_MAX]. */
+int64_t pclseg_i8_row_bytes(int64_t k);
+
+/* Symmetric quantisation, one scale per row: scale = max|x| / 127 (float32), q = round(x / scale), ties to even.
+ *   x      [rows, cols] dtype, row stride x_stride elements
+ *   q      int8 [rows, pclseg_i8_row_bytes(cols)], 8-byte aligned, written whole: zeros behind cols
+ *   scale  float32 [rows]: 0 for a row of zeros, NaN (codes 0) for a row that holds an infinity or a NaN */
+int pclseg_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_stride, int8_t* q,
+                            float* scale, void* hip_stream);
+
+/* y[i,j] = act(a_scale[i] b_scale[j] sum_k a[i,k] b[j,k] + bias[j]) + residual[i,j]: op_conv2d's epilogue on an int8 product
+ * with exact int32 sums.
+ *   a      int8 [m, pclseg_i8_row_bytes(k)], b likewise [n, ...], 16-byte aligned; the bytes behind k are 0 in both
+ *   act    0 none / 1 relu / 2 leaky(0.1) / 3 sigmoid
+ *   y, residual [m, n] dtype, row strides in elements; residual and bias (float32 [n]) may be NULL.  y may be residual. */
+int pclseg_op_matmul_i8(const int8_t* a, const float* a_scale, const int8_t* b, const float* b_scale, int64_t m,
+                        int64_t n, int64_t k, const float* bias, int act, const void* residual, int64_t residual_stride,
+                        void* y, int64_t y_stride, int dtype, void* hip_stream);
+
+/* The layer on float rows: op_quantize_rows of x into the workspace, then op_matmul_i8.
+ *   x      [m, k] dtype; weight codes and scales as for b above
+ *   workspace  pclseg_op_linear_i8_workspace bytes, 16-byte aligned; two calls in flight need two */
+int pclseg_op_linear_i8_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes);
+int pclseg_op_linear_i8(const void* x, int dtype, int64_t x_stride, const int8_t* weight, const float* weight_scale,
+                        int64_t m, int64_t n, int64_t k, const float* bias, int act, const void* residual,
+                        int64_t residual_stride, void* y, int64_t y_stride, int y_dtype, void* workspace,
+                        size_t workspace_bytes, void* hip_stream);
+
+/* Log probability of one label per row, entropy and the top_k most probable classes (the float side of op_head's softmax
+ * and argmax).  Classes that `allowed` excludes do not take part, whatever their logit holds; a logit of -inf is an excluded
+ * class.
+ *   logits   [rows, classes] dtype, row stride in elements
+ *   labels   int32 (label_bytes 4) or int64 (8) [rows], or NULL; a label outside [0, classes) is not counted: logprob 0
+ *   allowed  uint8, 0 = excluded: one row of `classes` for all (allowed_stride 0) or one per row; NULL: all allowed
+ *   logprob, entropy, lse  float32 [rows], each may be NULL.  An excluded label has -inf.
+ *   top_ids int32, top_logprobs float32 [rows, top_k]: largest first, the lowest index first among equals (op_head's argmax
+ *            rule); -1 and -inf where fewer classes are allowed.  0 <= top_k <= PCLSEG_TOP_MAX
+ * A row without an allowed class: lse -inf, entropy 0, no alternatives.  A row with an allowed NaN or +inf: NaN, ids -1.
+ *   workspace  pclseg_op_label_logprobs_workspace bytes (0 for most sizes), 16-byte aligned */
+int pclseg_op_label_logprobs_workspace(int64_t rows, int64_t classes, int top_k, size_t* bytes);
+int pclseg_op_label_logprobs(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t stride,
+                             const void* labels, int label_bytes, const uint8_t* allowed, int64_t allowed_stride, int top_k,
+                             float* logprob, float* entropy, float* lse, int32_t* top_ids, float* top_logprobs,
+                             void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/* Gradient of any loss in logprob, entropy and top_logprobs with respect to the logits, from the lse (and entropy) that
+ * op_label_logprobs wrote for the same logits and mask:
+ *   grad[j] = d_logprob [j = label] + sum_i d_top[i] [j = top_ids[i]] - p_j (d_logprob + sum_i d_top[i])
+ *             - d_entropy p_j (ln p_j + entropy),       p_j = exp(logit_j - lse)
+ * 0 for excluded classes, rows without an allowed class and the logprob of uncounted labels.  d_logprob (with labels),
+ * d_entropy (with entropy) and d_top (with top_ids, top_k) may be NULL; one at least is given.
+ *   grad   [rows, classes] dtype of the logits, row stride in elements; does not overlap the logits */
+int pclseg_op_label_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t stride,
+                                  const void* labels, int label_bytes, const uint8_t* allowed, int64_t allowed_stride,
+                                  const float* lse, const float* entropy, const float* d_logprob, const float* d_entropy,
+                                  const int32_t* top_ids, const float* d_top, int top_k, void* grad, int64_t grad_stride,
+                                  void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,7 @@
 #define PCLSEG_SLOTS 2
 #endif
 #include "pclseg_kernels.h"
+#include "pclseg_status.h"
 
 using namespace pclseg;
 
@@ -1531,6 +1532,10 @@ struct HandleGuard {
 };
 
 }  // namespace
+
+// the row operators' entry points (pclseg_ops.hip) report through the same two functions
+int pclseg::op_fail(int code, const std::string& msg) { return fail(nullptr, code, msg); }
+int pclseg::op_exception() noexcept { return on_exception(nullptr); }
 
 // =============================================================================== C ABI
 extern "C" {

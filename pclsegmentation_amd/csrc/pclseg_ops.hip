@@ -1,0 +1,282 @@
+// pclseg_ops.hip — C entry points of the row operators (include/pclseg.h): argument checks, choice of a kernel, launch.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdio.h>
+
+#include <algorithm>
+#include <string>
+
+#include "../../include/pclseg.h"
+#include "pclseg_i8.h"
+#include "pclseg_score.h"
+#include "pclseg_status.h"
+
+using namespace pclseg;
+
+namespace {
+
+#define OP_CATCH catch (...) { return pclseg::op_exception(); }
+
+int bad(const char* op, const char* what) { return op_fail(PCLSEG_ERR_BAD_ARG, std::string(op) + ": " + what); }
+int bad_shape(const char* op, const char* what) { return op_fail(PCLSEG_ERR_BAD_SHAPE, std::string(op) + ": " + what); }
+int launched(const char* op) {
+  const hipError_t e = hipGetLastError();
+  if (e == hipSuccess) return PCLSEG_OK;
+  return op_fail(e == hipErrorOutOfMemory ? PCLSEG_ERR_OOM : PCLSEG_ERR_HIP, std::string(op) + ": " + hipGetErrorString(e));
+}
+bool dtype_ok(int d) { return d == PCLSEG_F32 || d == PCLSEG_BF16 || d == PCLSEG_F16; }
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+size_t dtype_size(int d) { return d == PCLSEG_F32 ? 4 : 2; }
+constexpr int64_t kMaxBlocks = 0x7fffffff;
+
+// calls f with a value of the element type
+template <typename F> void with_type(int dtype, F f) {
+  if (dtype == PCLSEG_F32) f(float{});
+  else if (dtype == PCLSEG_BF16) f(__bf16{});
+  else f(_Float16{});
+}
+
+// ---------------------------------------------------------------------------------------------- quantisation, product
+int64_t row_bytes(int64_t k) {
+  if (k < 1 || k > PCLSEG_I8_K_MAX) return 0;
+  return k <= 64 ? 64 : (k + 127) / 128 * 128;
+}
+
+template <typename T, int G> void launch_quant(const QuantArgs& a, hipStream_t s) {
+  const int64_t blocks = (a.rows + 256 / G - 1) / (256 / G);
+  if (a.cols > 32 * G) quantize_rows_kernel<T, G, true><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(a);
+  else quantize_rows_kernel<T, G, false><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(a);
+}
+
+int quantize(const char* op, const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, int8_t* q, float* scale,
+             hipStream_t s) {
+  QuantArgs a{x, rows, stride, (int)cols, q, row_bytes(cols), scale};
+  with_type(dtype, [&](auto t) {
+    typedef decltype(t) T;
+    if (cols <= 256) launch_quant<T, 8>(a, s);
+    else if (cols <= 2048) launch_quant<T, 64>(a, s);
+    else launch_quant<T, 256>(a, s);
+  });
+  return launched(op);
+}
+
+template <typename T, int BM, int BN, int BK, int WM, int WN>
+void launch_tiles(const I8Args& p, hipStream_t s) {
+  const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
+  i8_tiles<T, BM, BN, BK, WM, WN><<<dim3((unsigned)(tm * tn)), dim3(WM * WN * 64), 0, s>>>(p, (unsigned)tn);
+}
+
+int matmul(const char* op, const I8Args& p, int dtype, hipStream_t s) {
+  auto tiles = [&](int bm, int bn) { return ((p.m + bm - 1) / bm) * ((p.n + (int64_t)bn - 1) / bn); };
+  if (p.m > 64 && tiles(64, 64) > kMaxBlocks) return bad_shape(op, "more output tiles than a launch has blocks");
+  with_type(dtype, [&](auto t) {
+    typedef decltype(t) T;
+    const dim3 few((unsigned)((p.n + 15) / 16));
+    if (p.m <= 16) i8_few_rows<T, 1, 8><<<few, dim3(512), 0, s>>>(p);
+    else if (p.m <= 32) i8_few_rows<T, 2, 8><<<few, dim3(512), 0, s>>>(p);
+    else if (p.m <= 64) i8_few_rows<T, 4, 8><<<few, dim3(512), 0, s>>>(p);
+    else if (p.kp == 64) launch_tiles<T, 128, 128, 64, 2, 2>(p, s);
+    else if (tiles(256, 256) >= 192) launch_tiles<T, 256, 256, 128, 2, 4>(p, s);
+    else if (tiles(128, 128) >= 192) launch_tiles<T, 128, 128, 128, 2, 2>(p, s);
+    else launch_tiles<T, 64, 64, 128, 2, 2>(p, s);
+  });
+  return launched(op);
+}
+
+int check_product(const char* op, int64_t m, int64_t n, int64_t k, const int8_t* b, const float* b_scale, int act,
+                  const void* residual, int64_t residual_stride, const void* y, int64_t y_stride, int dtype) {
+  if (!dtype_ok(dtype)) return bad(op, "unknown dtype");
+  if (act < 0 || act > 3) return bad(op, "unknown activation");
+  if (m < 0 || n < 1 || n > 0x7fffffff - 256) return bad_shape(op, "m must not be negative, n must be in [1, 2^31 - 257]");
+  if (!row_bytes(k)) return bad_shape(op, "k must be in [1, 131071]");
+  if (!b || !b_scale || (m && !y)) return bad(op, "NULL buffer");
+  if (!aligned(b, 16)) return bad(op, "codes must be 16-byte aligned");
+  if (y_stride < n || (residual && residual_stride < n)) return bad_shape(op, "row stride smaller than n");
+  if (!aligned(y, dtype_size(dtype)) || !aligned(residual, dtype_size(dtype))) return bad(op, "misaligned y or residual");
+  return PCLSEG_OK;
+}
+
+// ---------------------------------------------------------------------------------------------- log probabilities
+constexpr int kThreadRow = 32, kGroupRow = 2048, kPiece = 2048, kWaves = 4;
+
+// pieces a long row is cut into so that few rows still fill the chip: a block streams kWaves pieces of 2048 elements at a
+// time, and 512 blocks hide the memory's latency
+int score_segs(int64_t rows, int64_t classes) {
+  if (classes <= kGroupRow) return 1;
+  const int64_t most = (classes + (int64_t)kPiece * kWaves - 1) / ((int64_t)kPiece * kWaves);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(most, 64), 512 / rows));
+}
+size_t score_workspace(int64_t rows, int64_t classes, int top_k) {
+  const int segs = rows > 0 ? score_segs(rows, classes) : 1;
+  return segs == 1 ? 0 : (size_t)rows * segs * (sizeof(ScorePart) + (top_k ? 64 * sizeof(Key) : 0));
+}
+
+template <typename T> void launch_score(const ScoreArgs& a, hipStream_t s) {
+  const int v = a.classes;
+  if (v <= kThreadRow) {
+    const dim3 g((unsigned)((a.rows + 255) / 256)), b(256);
+    if (v <= 8) logprob_thread_rows<T, 8><<<g, b, 0, s>>>(a);
+    else if (v <= 16) logprob_thread_rows<T, 16><<<g, b, 0, s>>>(a);
+    else if (v <= 24) logprob_thread_rows<T, 24><<<g, b, 0, s>>>(a);
+    else logprob_thread_rows<T, 32><<<g, b, 0, s>>>(a);
+  } else if (v <= kGroupRow) {
+    auto grid = [&](int g) { return dim3((unsigned)((a.rows + 256 / g - 1) / (256 / g))); };
+    if (v <= 8 * 32) logprob_group_rows<T, 8><<<grid(8), dim3(256), 0, s>>>(a);
+    else if (v <= 16 * 32) logprob_group_rows<T, 16><<<grid(16), dim3(256), 0, s>>>(a);
+    else if (v <= 32 * 32) logprob_group_rows<T, 32><<<grid(32), dim3(256), 0, s>>>(a);
+    else logprob_group_rows<T, 64><<<grid(64), dim3(256), 0, s>>>(a);
+  } else {
+    const dim3 g((unsigned)(a.rows * a.segs)), b(kWaves * 64);
+    if (a.top_k) logprob_wave_rows<T, kWaves, true><<<g, b, 0, s>>>(a);
+    else logprob_wave_rows<T, kWaves, false><<<g, b, 0, s>>>(a);
+    if (a.segs > 1) {
+      if (a.top_k) logprob_join<T, true><<<dim3((unsigned)a.rows), dim3(256), 0, s>>>(a);
+      else logprob_join<T, false><<<dim3((unsigned)a.rows), dim3(256), 0, s>>>(a);
+    }
+  }
+}
+
+int check_rows(const char* op, const void* logits, int dtype, int64_t rows, int64_t classes, int64_t stride,
+               const void* labels, int label_bytes, const uint8_t* allowed, int64_t allowed_stride, int top_k) {
+  if (!dtype_ok(dtype)) return bad(op, "unknown dtype");
+  if (rows < 0 || classes < 1 || classes > 0x7fffffff - 4096)
+    return bad_shape(op, "rows must not be negative, classes must be in [1, 2^31 - 4097]");
+  if (stride < classes) return bad_shape(op, "row stride smaller than classes");
+  if (top_k < 0 || top_k > PCLSEG_TOP_MAX) return bad(op, "top_k must be in [0, 64]");
+  if (rows && !logits) return bad(op, "logits is NULL");
+  if (!aligned(logits, dtype_size(dtype))) return bad(op, "misaligned logits");
+  if (labels && label_bytes != 4 && label_bytes != 8) return bad(op, "labels are int32 or int64");
+  if (labels && !aligned(labels, (size_t)label_bytes)) return bad(op, "misaligned labels");
+  if (allowed && allowed_stride != 0 && allowed_stride < classes) return bad_shape(op, "mask stride smaller than classes");
+  return PCLSEG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t pclseg_i8_row_bytes(int64_t k) { return row_bytes(k); }
+
+int pclseg_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_stride, int8_t* q,
+                            float* scale, void* hip_stream) try {
+  const char* op = "op_quantize_rows";
+  if (!dtype_ok(dtype)) return bad(op, "unknown dtype");
+  if (rows < 0 || rows > kMaxBlocks || !row_bytes(cols)) return bad_shape(op, "rows must be in [0, 2^31), cols in [1, 131071]");
+  if (x_stride < cols) return bad_shape(op, "row stride smaller than cols");
+  if (rows == 0) return PCLSEG_OK;
+  if (!x || !q || !scale) return bad(op, "NULL buffer");
+  if (!aligned(x, dtype_size(dtype)) || !aligned(q, 8)) return bad(op, "misaligned x or codes");
+  return quantize(op, x, dtype, rows, cols, x_stride, q, scale, (hipStream_t)hip_stream);
+} OP_CATCH
+
+int pclseg_op_matmul_i8(const int8_t* a, const float* a_scale, const int8_t* b, const float* b_scale, int64_t m,
+                        int64_t n, int64_t k, const float* bias, int act, const void* residual, int64_t residual_stride,
+                        void* y, int64_t y_stride, int dtype, void* hip_stream) try {
+  const char* op = "op_matmul_i8";
+  const int rc = check_product(op, m, n, k, b, b_scale, act, residual, residual_stride, y, y_stride, dtype);
+  if (rc) return rc;
+  if (m == 0) return PCLSEG_OK;
+  if (!a || !a_scale) return bad(op, "NULL buffer");
+  if (!aligned(a, 16)) return bad(op, "codes must be 16-byte aligned");
+  I8Args p{a, b, a_scale, b_scale, row_bytes(k), row_bytes(k), m, (int)n, (int)row_bytes(k), bias, act, residual,
+           residual_stride, y, y_stride};
+  return matmul(op, p, dtype, (hipStream_t)hip_stream);
+} OP_CATCH
+
+int pclseg_op_linear_i8_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes) try {
+  const char* op = "op_linear_i8_workspace";
+  if (!bytes) return bad(op, "bytes is NULL");
+  if (m < 0 || m > kMaxBlocks || n < 1 || !row_bytes(k)) return bad_shape(op, "m must be in [0, 2^31), n positive, k in [1, 131071]");
+  *bytes = (size_t)m * ((size_t)row_bytes(k) + sizeof(float));
+  return PCLSEG_OK;
+} OP_CATCH
+
+int pclseg_op_linear_i8(const void* x, int dtype, int64_t x_stride, const int8_t* weight, const float* weight_scale,
+                        int64_t m, int64_t n, int64_t k, const float* bias, int act, const void* residual,
+                        int64_t residual_stride, void* y, int64_t y_stride, int y_dtype, void* workspace,
+                        size_t workspace_bytes, void* hip_stream) try {
+  const char* op = "op_linear_i8";
+  const int rc = check_product(op, m, n, k, weight, weight_scale, act, residual, residual_stride, y, y_stride, y_dtype);
+  if (rc) return rc;
+  if (!dtype_ok(dtype)) return bad(op, "unknown dtype");
+  if (m > kMaxBlocks || x_stride < k) return bad_shape(op, "m must be below 2^31, the row stride at least k");
+  if (m == 0) return PCLSEG_OK;
+  if (!x || !workspace) return bad(op, "NULL buffer");
+  if (!aligned(x, dtype_size(dtype)) || !aligned(workspace, 16)) return bad(op, "misaligned x or workspace");
+  const int64_t ld = row_bytes(k);
+  if (workspace_bytes < (size_t)m * ((size_t)ld + sizeof(float))) return bad(op, "workspace too small");
+  int8_t* q = static_cast<int8_t*>(workspace);
+  float* scale = reinterpret_cast<float*>(q + m * ld);
+  const int rq = quantize(op, x, dtype, m, k, x_stride, q, scale, (hipStream_t)hip_stream);
+  if (rq) return rq;
+  I8Args p{q, weight, scale, weight_scale, ld, ld, m, (int)n, (int)ld, bias, act, residual, residual_stride, y, y_stride};
+  return matmul(op, p, y_dtype, (hipStream_t)hip_stream);
+} OP_CATCH
+
+int pclseg_op_label_logprobs_workspace(int64_t rows, int64_t classes, int top_k, size_t* bytes) try {
+  const char* op = "op_label_logprobs_workspace";
+  if (!bytes) return bad(op, "bytes is NULL");
+  const int rc = check_rows(op, bytes, PCLSEG_BF16, rows, classes, classes, nullptr, 0, nullptr, 0, top_k);
+  if (rc) return rc;
+  *bytes = score_workspace(rows, classes, top_k);
+  return PCLSEG_OK;
+} OP_CATCH
+
+int pclseg_op_label_logprobs(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t stride,
+                             const void* labels, int label_bytes, const uint8_t* allowed, int64_t allowed_stride, int top_k,
+                             float* logprob, float* entropy, float* lse, int32_t* top_ids, float* top_logprobs,
+                             void* workspace, size_t workspace_bytes, void* hip_stream) try {
+  const char* op = "op_label_logprobs";
+  const int rc = check_rows(op, logits, dtype, rows, classes, stride, labels, label_bytes, allowed, allowed_stride, top_k);
+  if (rc) return rc;
+  if (logprob && !labels) return bad(op, "logprob needs labels");
+  if (rows == 0) return PCLSEG_OK;
+  if (top_k && (!top_ids || !top_logprobs)) return bad(op, "top_k without top_ids and top_logprobs");
+  const size_t need = score_workspace(rows, classes, top_k);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return bad(op, "workspace too small or misaligned");
+  ScoreArgs a{logits, rows, stride, (int)classes, labels, label_bytes == 8, allowed, allowed_stride, top_k,
+              logprob, entropy, lse, top_ids, top_logprobs, workspace, score_segs(rows, classes)};
+  if (rows > kMaxBlocks || rows * a.segs > kMaxBlocks) return bad_shape(op, "more rows than a launch has blocks");
+  with_type(dtype, [&](auto t) { launch_score<decltype(t)>(a, (hipStream_t)hip_stream); });
+  return launched(op);
+} OP_CATCH
+
+int pclseg_op_label_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t stride,
+                                  const void* labels, int label_bytes, const uint8_t* allowed, int64_t allowed_stride,
+                                  const float* lse, const float* entropy, const float* d_logprob, const float* d_entropy,
+                                  const int32_t* top_ids, const float* d_top, int top_k, void* grad, int64_t grad_stride,
+                                  void* hip_stream) try {
+  const char* op = "op_label_logprobs_grad";
+  const int rc = check_rows(op, logits, dtype, rows, classes, stride, labels, label_bytes, allowed, allowed_stride, top_k);
+  if (rc) return rc;
+  if (!d_logprob && !d_entropy && !d_top) return bad(op, "no gradient arrives");
+  if (d_logprob && !labels) return bad(op, "d_logprob needs labels");
+  if (d_entropy && !entropy) return bad(op, "d_entropy needs entropy");
+  if (d_top && (!top_ids || top_k < 1)) return bad(op, "d_top needs top_ids and top_k");
+  if (grad_stride < classes) return bad_shape(op, "gradient stride smaller than classes");
+  if (rows == 0) return PCLSEG_OK;
+  if (!lse || !grad) return bad(op, "NULL buffer");
+  if (!aligned(grad, dtype_size(dtype))) return bad(op, "misaligned grad");
+  const uintptr_t sz = dtype_size(dtype), x0 = (uintptr_t)logits, g0 = (uintptr_t)grad;
+  const uintptr_t x1 = x0 + ((uintptr_t)(rows - 1) * stride + classes) * sz;
+  const uintptr_t g1 = g0 + ((uintptr_t)(rows - 1) * grad_stride + classes) * sz;
+  if (g0 < x1 && x0 < g1) return bad(op, "grad overlaps the logits");
+  GradArgs a{logits, rows, stride, (int)classes, labels, label_bytes == 8, allowed, allowed_stride, lse, entropy,
+             d_logprob, d_entropy, top_ids, d_top, d_top ? top_k : 0, grad, grad_stride, 1, (int)classes, 1};
+  // a block writes about 8192 elements: that many columns of a long row, or whole short rows
+  constexpr int kSpan = 8192;
+  if (classes > kSpan) {
+    a.span = kSpan;
+    a.pieces = (int)((classes + kSpan - 1) / kSpan);
+  } else {
+    a.rows_per_block = (int)std::min<int64_t>(256, std::max<int64_t>(1, kSpan / classes));
+  }
+  const int64_t blocks = a.pieces > 1 ? rows * a.pieces : (rows + a.rows_per_block - 1) / a.rows_per_block;
+  if (rows > kMaxBlocks * 256 || blocks > kMaxBlocks) return bad_shape(op, "more rows than a launch has blocks");
+  with_type(dtype, [&](auto t) {
+    logprob_grad<decltype(t)><<<dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream>>>(a);
+  });
+  return launched(op);
+} OP_CATCH
+
+}  // extern "C"

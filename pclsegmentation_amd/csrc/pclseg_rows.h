@@ -1,0 +1,86 @@
+// pclseg_rows.h — what the row operators (pclseg_score.h, pclseg_i8.h) share: element types, 16-byte accesses at any
+// element alignment, lane exchanges.  gfx950, 64-lane waves.
+#ifndef PCLSEG_ROWS_H_
+#define PCLSEG_ROWS_H_
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace pclseg {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+// the hardware takes a global access of any size at any 2-byte (16-bit types) or 4-byte (float) address: rows of an odd
+// length need no other path, a 16-byte access that crosses a 128-byte line only costs a second tag look-up
+struct __attribute__((packed, aligned(2))) Pack16a2 { u32x4 v; };
+struct __attribute__((packed, aligned(4))) Pack16a4 { u32x4 v; };
+struct __attribute__((packed, aligned(1))) Pack8a1 { uint64_t v; };
+struct __attribute__((packed, aligned(1))) Pack4a1 { uint32_t v; };
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+  typedef Pack16a4 Pack;
+  static constexpr int VEC = 4;
+  static __device__ __forceinline__ float get(const u32x4& v, int e) { return __uint_as_float(v[e]); }
+  static __device__ __forceinline__ float load(const float* p) { return *p; }
+  static __device__ __forceinline__ float from(float f) { return f; }
+};
+template <> struct Elem<__bf16> {
+  typedef Pack16a2 Pack;
+  static constexpr int VEC = 8;
+  static __device__ __forceinline__ float get(const u32x4& v, int e) {
+    return __uint_as_float((e & 1) ? (v[e >> 1] & 0xffff0000u) : (v[e >> 1] << 16));
+  }
+  static __device__ __forceinline__ float load(const __bf16* p) { return (float)*p; }
+  static __device__ __forceinline__ __bf16 from(float f) { return (__bf16)f; }   // nearest, ties to even
+};
+template <> struct Elem<_Float16> {
+  typedef Pack16a2 Pack;
+  static constexpr int VEC = 8;
+  static __device__ __forceinline__ float get(const u32x4& v, int e) {
+    const uint32_t w = v[e >> 1];
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)((e & 1) ? (w >> 16) : (w & 0xffffu)));
+  }
+  static __device__ __forceinline__ float load(const _Float16* p) { return (float)*p; }
+  static __device__ __forceinline__ _Float16 from(float f) { return (_Float16)f; }
+};
+
+// 16 bytes at element p (any element alignment)
+template <typename T> __device__ __forceinline__ u32x4 load16(const T* p) {
+  return reinterpret_cast<const typename Elem<T>::Pack*>(p)->v;
+}
+template <typename T> __device__ __forceinline__ void store16(T* p, const u32x4& v) {
+  reinterpret_cast<typename Elem<T>::Pack*>(p)->v = v;
+}
+template <typename T> __device__ __forceinline__ u32x4 pack16(const float* f) {
+  u32x4 v;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(f[e]);
+  } else {
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    typedef float F2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(F2{f[2 * e], f[2 * e + 1]}, T2));
+  }
+  return v;
+}
+
+__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+
+// LDS traffic inside one wave is in order in the hardware; this keeps the compiler from reordering it
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Blocks are dealt round robin over the 8 XCDs: give each XCD one contiguous range of tiles, so neighbours share an L2.
+// A bijection of [0, total) for every total.
+__device__ __forceinline__ unsigned xcd_contiguous(unsigned block, unsigned total) {
+  const unsigned q = total >> 3, r = total & 7, x = block & 7, i = block >> 3;
+  return x * q + (x < r ? x : r) + i;
+}
+
+}  // namespace pclseg
+
+#endif  // PCLSEG_ROWS_H_

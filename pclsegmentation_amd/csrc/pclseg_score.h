@@ -1,0 +1,595 @@
+// pclseg_score.h — log probabilities of given labels, entropy and top alternatives of rows of logits, and their gradient.
+//
+// For a row x[0..V) with the classes A = {j : allowed[j], x[j] > -inf}:
+//   M = max x,  S = sum e^(x-M),  T = sum e^(x-M) (x-M)          (sums over A)
+//   lse = M + ln S,   logprob = (x[label] - M) - ln S,   entropy = ln S - T / S
+// (M, S, T) of two disjoint parts join with M = max(M1, M2), d = Mi - M <= 0:  S += Si e^d, T += e^d (Ti + d Si), so a row
+// is read once and can be cut anywhere.  All of it is float32: the terms of S and T have one sign and at most a few roundings
+// per element, 2^-24 each, and the differences x - M are taken before the exponential, so large logits lose nothing.
+// The exponential is v_exp_f32 on (x-M) log2 e: both roundings are relative to an exponent of at most a few tens.
+// Terms with x - M < -200 are 0 in float32; the clamp of the second factor at -200 keeps 0 * inf out of T.
+//
+// Three kernels, by the length of a row (what a row costs besides its elements is what differs):
+//   logprob_thread_rows   V <= 32    a thread owns a row: no exchange between lanes at all
+//   logprob_group_rows    V <= 2048  8, 16, 32 or 64 lanes own a row, held in registers; the top list by rounds of argmax
+//   logprob_wave_rows     longer     the waves of a block (or of several blocks) stream a row in pieces of 2048 elements
+#ifndef PCLSEG_SCORE_H_
+#define PCLSEG_SCORE_H_
+
+#include "pclseg_rows.h"
+
+namespace pclseg {
+
+struct ScoreArgs {
+  const void* x;             // logits, rows of `classes` elements, `stride` elements apart
+  int64_t rows, stride;
+  int classes;
+  const void* labels;        // int32 or int64 (label64), NULL: none
+  int label64;
+  const uint8_t* allowed;    // NULL: all classes
+  int64_t allowed_stride;    // 0: one mask for all rows
+  int top_k;
+  float *logprob, *entropy, *lse;   // each may be NULL
+  int32_t* top_ids;
+  float* top_logprobs;
+  void* part;                // workspace of a split row
+  int segs;                  // pieces a row is cut into
+};
+
+constexpr float kLowest = -3.402823466e38f;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct Stat { float m, s, t; };   // maximum, sum of e^(x-m), sum of e^(x-m)(x-m)
+
+__device__ __forceinline__ float fast_exp(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
+
+__device__ __forceinline__ Stat stat_shift(const Stat& a, float m) {   // the same sums relative to m >= a.m
+  const float d = fmaxf(a.m - m, -200.f), f = fast_exp(d);
+  return Stat{m, a.s * f, f * fmaf(d, a.s, a.t)};
+}
+__device__ __forceinline__ Stat stat_join(const Stat& a, const Stat& b) {
+  const float m = fmaxf(a.m, b.m);
+  const Stat p = stat_shift(a, m), q = stat_shift(b, m);
+  return Stat{m, p.s + q.s, p.t + q.t};
+}
+__device__ __forceinline__ void stat_add(Stat& a, float x) {   // a.m >= x unless x is -inf, +inf or NaN
+  const float z = x - a.m, e = fast_exp(z);
+  a.s += e;
+  a.t = fmaf(e, fmaxf(z, -200.f), a.t);
+}
+
+// a row's results.  s == 0: nothing is allowed (or every allowed logit is -inf); s NaN: an allowed logit is NaN or +inf, the
+// row has no distribution and every float result is NaN.
+struct RowOut { float m, logs, lse, entropy; bool empty, bad; };
+__device__ __forceinline__ RowOut row_out(const Stat& a) {
+  RowOut o;
+  o.empty = a.s == 0.f;
+  o.bad = !(a.s < __builtin_inff());
+  o.m = a.m;
+  o.logs = logf(a.s);
+  o.lse = o.empty ? neg_inf() : (o.bad ? __builtin_nanf("") : a.m + o.logs);
+  o.entropy = o.empty ? 0.f : (o.bad ? __builtin_nanf("") : o.logs - a.t / a.s);
+  return o;
+}
+__device__ __forceinline__ float row_logprob(const RowOut& o, float x) {
+  if (o.bad) return __builtin_nanf("");
+  return x == neg_inf() ? neg_inf() : (x - o.m) - o.logs;
+}
+
+__device__ __forceinline__ int64_t label_of(const ScoreArgs& a, int64_t row) {
+  if (!a.labels) return -1;
+  return a.label64 ? static_cast<const int64_t*>(a.labels)[row] : static_cast<const int32_t*>(a.labels)[row];
+}
+
+// logprob, entropy and lse of a row: called by one lane
+template <typename T> __device__ __forceinline__ void write_row(const ScoreArgs& a, int64_t row, const RowOut& o) {
+  if (a.entropy) a.entropy[row] = o.entropy;
+  if (a.lse) a.lse[row] = o.lse;
+  if (a.logprob) {
+    const int64_t lab = label_of(a, row);
+    float lp = 0.f;
+    if (lab >= 0 && lab < a.classes) {
+      float x = Elem<T>::load(static_cast<const T*>(a.x) + row * a.stride + lab);
+      if (a.allowed && !a.allowed[row * a.allowed_stride + lab]) x = neg_inf();
+      lp = row_logprob(o, x);
+    }
+    a.logprob[row] = lp;
+  }
+}
+
+// elements [c, c + VEC) of a row of `classes`, -inf behind its end and where the mask is 0
+template <typename T>
+__device__ __forceinline__ void load_masked(const T* row, const uint8_t* mask, int c, int classes, float* f) {
+  constexpr int VEC = Elem<T>::VEC;
+  if (c + VEC <= classes) {
+    const u32x4 v = load16(row + c);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = Elem<T>::get(v, e);
+    if (mask) {
+      if constexpr (VEC == 8) {
+        const uint64_t mk = reinterpret_cast<const Pack8a1*>(mask + c)->v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = ((mk >> (8 * e)) & 0xff) ? f[e] : neg_inf();
+      } else {
+        const uint32_t mk = reinterpret_cast<const Pack4a1*>(mask + c)->v;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = ((mk >> (8 * e)) & 0xff) ? f[e] : neg_inf();
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      f[e] = neg_inf();
+      if (c + e < classes && (!mask || mask[c + e])) f[e] = Elem<T>::load(row + c + e);
+    }
+  }
+}
+
+// ---- V <= 32: a thread owns a row
+// CAP = the row's registers.  A row of 20 floats is 80 bytes: the 16-byte loads of a wave touch 40 lines, five times over,
+// all of them in the L1 after the first.
+template <typename T, int CAP>
+__global__ __launch_bounds__(256) void logprob_thread_rows(ScoreArgs a) {
+  constexpr int VEC = Elem<T>::VEC;
+  const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (row >= a.rows) return;
+  const T* src = static_cast<const T*>(a.x) + row * a.stride;
+  const uint8_t* mask = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+  float x[CAP];
+#pragma unroll
+  for (int v = 0; v < CAP / VEC; ++v) {
+    if (v * VEC < a.classes) {
+      load_masked(src, mask, v * VEC, a.classes, x + v * VEC);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[v * VEC + e] = neg_inf();
+    }
+  }
+  Stat st{kLowest, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < CAP; ++j) st.m = fmaxf(st.m, x[j]);
+#pragma unroll
+  for (int j = 0; j < CAP; ++j) stat_add(st, x[j]);
+  const RowOut o = row_out(st);
+  write_row<T>(a, row, o);
+  for (int k = 0; k < a.top_k; ++k) {
+    float best = neg_inf();
+    int id = -1;
+#pragma unroll
+    for (int j = 0; j < CAP; ++j) {     // ascending and strict: the lowest index among equals
+      const bool g = x[j] > best;
+      best = g ? x[j] : best;
+      id = g ? j : id;
+    }
+#pragma unroll
+    for (int j = 0; j < CAP; ++j) x[j] = j == id ? neg_inf() : x[j];
+    a.top_ids[row * a.top_k + k] = o.bad ? -1 : id;
+    a.top_logprobs[row * a.top_k + k] = row_logprob(o, best);
+  }
+}
+
+// ---- V <= 2048: G lanes own a row
+template <int G> __device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+  for (int d = 1; d < G; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
+  return v;
+}
+template <int G> __device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int d = 1; d < G; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+
+template <typename T, int G>
+__global__ __launch_bounds__(256) void logprob_group_rows(ScoreArgs a) {
+  constexpr int VEC = Elem<T>::VEC, NV = 32 / VEC;
+  const int g = threadIdx.x & (G - 1);
+  const int64_t row0 = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  const bool live = row0 < a.rows;
+  const int64_t row = live ? row0 : a.rows - 1;      // lanes behind the last row repeat it and write nothing
+  const T* src = static_cast<const T*>(a.x) + row * a.stride;
+  const uint8_t* mask = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+  const int nv = (a.classes + G * VEC - 1) / (G * VEC);   // uniform
+  float x[NV][VEC];
+  float bv = neg_inf();      // this lane's largest element that is left, and its index
+  int bi = 0x7fffffff;
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    if (v < nv) load_masked(src, mask, (v * G + g) * VEC, a.classes, x[v]);
+  }
+  Stat st{kLowest, 0.f, 0.f};
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    if (v < nv) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const bool b = x[v][e] > bv;
+        bv = b ? x[v][e] : bv;
+        bi = b ? (v * G + g) * VEC + e : bi;
+      }
+    }
+  }
+  st.m = group_max<G>(fmaxf(bv, kLowest));
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    if (v < nv) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) stat_add(st, x[v][e]);
+    }
+  }
+  st.s = group_sum<G>(st.s);
+  st.t = group_sum<G>(st.t);
+  const RowOut o = row_out(st);
+  if (g == 0 && live) write_row<T>(a, row, o);
+  for (int k = 0; k < a.top_k; ++k) {
+    float best = bv;
+    int id = bi;
+#pragma unroll
+    for (int d = 1; d < G; d <<= 1) {
+      const float ov = __shfl_xor(best, d);
+      const int oi = __shfl_xor(id, d);
+      const bool b = ov > best || (ov == best && oi < id);
+      best = b ? ov : best;
+      id = b ? oi : id;
+    }
+    const bool none = best == neg_inf();
+    if (g == 0 && live) {
+      a.top_ids[row * a.top_k + k] = none || o.bad ? -1 : id;
+      a.top_logprobs[row * a.top_k + k] = row_logprob(o, best);
+    }
+    if (bi == id) {      // the winner's lane looks for its next one: after (best, id) in the order value down, index up
+      bv = neg_inf();
+      bi = 0x7fffffff;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        if (v < nv) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const int i = (v * G + g) * VEC + e;
+            const bool b = (x[v][e] < best || (x[v][e] == best && i > id)) && x[v][e] > bv;
+            bv = b ? x[v][e] : bv;
+            bi = b ? i : bi;
+          }
+        }
+      }
+    }
+  }
+}
+
+// ---- longer rows: waves stream pieces of 2048 elements
+// The top list of a wave is one 64-bit key per lane, sorted downwards: the float mapped to an unsigned of the same order
+// above the complement of the index, so one comparison decides value first and lowest index among equals; 0 is no entry.
+typedef unsigned long long Key;
+__device__ __forceinline__ Key make_key(float x, int idx) {
+  const uint32_t u = __float_as_uint(x + 0.0f);       // -0 and +0 are equal: one key
+  const uint32_t o = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return ((Key)o << 32) | (uint32_t)~(uint32_t)idx;
+}
+__device__ __forceinline__ float key_value(Key k) {
+  const uint32_t o = (uint32_t)(k >> 32);
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+__device__ __forceinline__ int key_index(Key k) { return (int)~(uint32_t)k; }
+__device__ __forceinline__ Key shfl_key(Key k, int src) {
+  return ((Key)(uint32_t)__shfl((int)(k >> 32), src) << 32) | (uint32_t)__shfl((int)(uint32_t)k, src);
+}
+__device__ __forceinline__ Key shfl_xor_key(Key k, int d) {
+  return ((Key)(uint32_t)__shfl_xor((int)(k >> 32), d) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)k, d);
+}
+// 64 keys of a wave that rise and then fall (or any rotation): sorted downwards
+__device__ __forceinline__ Key bitonic_clean(Key k, int lane) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    const Key o = shfl_xor_key(k, d);
+    const bool want_max = !(lane & d);
+    k = ((o > k) == want_max) ? o : k;
+  }
+  return k;
+}
+__device__ __forceinline__ Key bitonic_sort(Key k, int lane) {
+#pragma unroll
+  for (int w = 2; w <= 64; w <<= 1) {
+#pragma unroll
+    for (int d = w >> 1; d > 0; d >>= 1) {
+      const Key o = shfl_xor_key(k, d);
+      const bool want_max = (!(lane & d)) == (!(lane & w));
+      k = ((o > k) == want_max) ? o : k;
+    }
+  }
+  return k;
+}
+// the 64 largest of two lists sorted downwards: the second is given reversed
+__device__ __forceinline__ Key merge_lists(Key a, Key b_reversed, int lane) {
+  return bitonic_clean(a > b_reversed ? a : b_reversed, lane);
+}
+__device__ __forceinline__ float bitonic_sort_f(float v, int lane) {
+#pragma unroll
+  for (int w = 2; w <= 64; w <<= 1) {
+#pragma unroll
+    for (int d = w >> 1; d > 0; d >>= 1) {
+      const float o = __shfl_xor(v, d);
+      v = ((!(lane & d)) == (!(lane & w))) ? fmaxf(v, o) : fminf(v, o);
+    }
+  }
+  return v;
+}
+
+__device__ __forceinline__ Stat wave_join(Stat st) {
+  const float m = group_max<64>(st.m);
+  st = stat_shift(st, m);
+  st.s = group_sum<64>(st.s);
+  st.t = group_sum<64>(st.t);
+  return st;
+}
+
+// a piece's statistics and list in the workspace: [row * segs + seg]
+struct ScorePart { float m, s, t, pad; };
+
+template <typename T, int NW, bool TOP>
+__global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
+  constexpr int VEC = Elem<T>::VEC, NV = 32 / VEC, PIECE = 64 * 32;
+  __shared__ Key cand[TOP ? NW : 1][128];
+  __shared__ Key lists[TOP ? NW : 1][64];
+  __shared__ Stat stats[NW];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x / (unsigned)a.segs;
+  const int seg = (int)(blockIdx.x % (unsigned)a.segs);
+  const T* src = static_cast<const T*>(a.x) + row * a.stride;
+  const uint8_t* mask = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+  const int pieces = (int)(((int64_t)a.classes + PIECE - 1) / PIECE);
+  const int p0 = (int)((int64_t)pieces * seg / a.segs), p1 = (int)((int64_t)pieces * (seg + 1) / a.segs);
+
+  Stat st{kLowest, 0.f, 0.f};
+  Key list = 0;
+  float thr = neg_inf();      // a candidate is at least thr and behind no listed entry: key > thr_key
+  Key thr_key = 0;
+  int n = 0;                  // candidates waiting in cand[wave]
+
+  auto flush = [&](int count) {   // the first 64 (count of them valid) into the list
+    wave_lds_fence();
+    Key k = lane < count ? cand[wave][lane] : 0;
+    const Key rest = cand[wave][64 + lane];
+    k = bitonic_sort(k, lane);
+    list = merge_lists(list, shfl_key(k, 63 - lane), lane);
+    wave_lds_fence();
+    cand[wave][lane] = rest;
+    const Key kth = shfl_key(list, a.top_k - 1);
+    if (kth) {
+      thr_key = kth;
+      thr = key_value(kth);
+    }
+  };
+
+  for (int p = p0 + wave; p < p1; p += NW) {
+    float x[NV][VEC], vm[NV];
+    const int base = p * PIECE;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) load_masked(src, mask, base + (v * 64 + lane) * VEC, a.classes, x[v]);
+    float cm = kLowest;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      vm[v] = x[v][0];
+#pragma unroll
+      for (int e = 1; e < VEC; ++e) vm[v] = fmaxf(vm[v], x[v][e]);
+      cm = fmaxf(cm, vm[v]);
+    }
+    st = stat_shift(st, fmaxf(st.m, cm));
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) stat_add(st, x[v][e]);
+    if constexpr (TOP) {
+      // at least top_k elements of this piece are not below the top_k-th largest of the lanes' maxima: a bound that keeps
+      // the first piece from offering all of its elements, and a rising row from offering all of every piece
+      float lane_max = neg_inf();
+#pragma unroll
+      for (int v = 0; v < NV; ++v) lane_max = fmaxf(lane_max, vm[v]);
+      const Key over = __ballot(lane_max >= thr);
+      if (__popcll(over) > a.top_k || thr == neg_inf()) {
+        const float bound = __shfl(bitonic_sort_f(lane_max, lane), a.top_k - 1);
+        if (bound > thr) {
+          thr = bound;
+          thr_key = 0;
+        }
+      }
+      if (__ballot(lane_max >= thr)) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          if (__ballot(vm[v] >= thr)) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const int idx = base + (v * 64 + lane) * VEC + e;
+              const Key key = make_key(x[v][e], idx);
+              const bool take = x[v][e] >= thr && x[v][e] > neg_inf() && key > thr_key;
+              const Key who = __ballot(take);
+              if (who) {
+                if (take) cand[wave][n + __popcll(who & ((1ull << lane) - 1))] = key;
+                n += (int)__popcll(who);
+                if (n >= 64) {
+                  flush(64);
+                  n -= 64;
+                }
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+  if (TOP && n) flush(n);
+  st = wave_join(st);
+  if (lane == 0) stats[wave] = st;
+  if constexpr (TOP) lists[wave][lane] = list;
+  __syncthreads();
+  if constexpr (TOP) {
+#pragma unroll
+    for (int h = NW / 2; h > 0; h >>= 1) {
+      if (wave < h) {
+        list = merge_lists(list, lists[wave + h][63 - lane], lane);
+        lists[wave][lane] = list;
+      }
+      __syncthreads();
+    }
+  }
+  if (wave) return;
+  st = stats[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) st = stat_join(st, stats[w]);
+  if (a.segs > 1) {
+    ScorePart* part = static_cast<ScorePart*>(a.part);
+    const int64_t slot = row * a.segs + seg;
+    if (lane == 0) part[slot] = ScorePart{st.m, st.s, st.t, 0.f};
+    if constexpr (TOP) reinterpret_cast<Key*>(part + a.rows * a.segs)[slot * 64 + lane] = list;
+    return;
+  }
+  const RowOut o = row_out(st);
+  if (lane == 0) write_row<T>(a, row, o);
+  if (TOP && lane < a.top_k) {
+    a.top_ids[row * a.top_k + lane] = list == 0 || o.bad ? -1 : key_index(list);
+    a.top_logprobs[row * a.top_k + lane] = row_logprob(o, list == 0 ? neg_inf() : key_value(list));
+  }
+}
+
+// joins the pieces of a row: one block a row, four waves
+template <typename T, bool TOP>
+__global__ __launch_bounds__(256) void logprob_join(ScoreArgs a) {
+  __shared__ Key lists[TOP ? 4 : 1][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x;
+  const ScorePart* part = static_cast<const ScorePart*>(a.part) + row * a.segs;
+  Key list = 0;
+  if constexpr (TOP) {
+    const Key* keys = reinterpret_cast<const Key*>(static_cast<const ScorePart*>(a.part) + a.rows * a.segs) + row * a.segs * 64;
+    for (int s = wave; s < a.segs; s += 4) list = merge_lists(list, keys[s * 64 + 63 - lane], lane);
+    lists[wave][lane] = list;
+    __syncthreads();
+    if (wave < 2) lists[wave][lane] = list = merge_lists(list, lists[wave + 2][63 - lane], lane);
+    __syncthreads();
+    if (wave == 0) list = merge_lists(list, lists[1][63 - lane], lane);
+  }
+  if (wave) return;
+  Stat st{kLowest, 0.f, 0.f};
+  for (int s = lane; s < a.segs; s += 64) st = stat_join(st, Stat{part[s].m, part[s].s, part[s].t});
+  st = wave_join(st);
+  const RowOut o = row_out(st);
+  if (lane == 0) write_row<T>(a, row, o);
+  if (TOP && lane < a.top_k) {
+    a.top_ids[row * a.top_k + lane] = list == 0 || o.bad ? -1 : key_index(list);
+    a.top_logprobs[row * a.top_k + lane] = row_logprob(o, list == 0 ? neg_inf() : key_value(list));
+  }
+}
+
+// ---- gradient
+// With p_j = e^(x_j - lse) (0 where not allowed), H the row's entropy, gl / ge / gt the gradients that arrive:
+//   d loss / d x_j = gl [j = label] + sum_i gt_i [j = id_i] - p_j (gl + sum_i gt_i) - ge p_j (x_j - lse + H)
+// One read of the logits and one write of the gradient; a block owns whole rows (or a piece of one), writes the dense part
+// and then, behind a barrier, rewrites the few elements that the label and the alternatives name.
+struct GradArgs {
+  const void* x;
+  int64_t rows, stride;
+  int classes;
+  const void* labels;
+  int label64;
+  const uint8_t* allowed;
+  int64_t allowed_stride;
+  const float *lse, *entropy, *d_logprob, *d_entropy;   // entropy / d_entropy / d_logprob may be NULL
+  const int32_t* top_ids;
+  const float* d_top;
+  int top_k;
+  void* grad;
+  int64_t grad_stride;
+  int rows_per_block, span, pieces;     // a block: rows_per_block rows, or `span` columns of one row
+};
+
+struct GradRow { float lse, w, ge, h; };   // w = gl + sum gt; h = entropy - lse; lse NaN-safe: empty rows have w = ge = 0
+
+__device__ __forceinline__ float grad_dense(const GradRow& r, float x) {
+  if (x == neg_inf()) return 0.f;
+  const float z = x - r.lse, p = fast_exp(z);
+  // an underflowed p takes the entropy term with it (0 * -inf otherwise)
+  return -p * fmaf(r.ge, fmaxf(z, -200.f) + r.h, r.w);
+}
+
+template <typename T>
+__device__ __forceinline__ GradRow grad_row(const GradArgs& a, int64_t row, int64_t& label) {
+  GradRow r;
+  const float lse = a.lse[row];
+  label = -1;
+  r.w = 0.f;
+  if (a.d_logprob) {
+    label = a.label64 ? static_cast<const int64_t*>(a.labels)[row] : static_cast<const int32_t*>(a.labels)[row];
+    if (label < 0 || label >= a.classes) label = -1;
+    if (label >= 0) r.w = a.d_logprob[row];
+  }
+  for (int k = 0; k < a.top_k; ++k) {
+    const int id = a.top_ids[row * a.top_k + k];
+    if (id >= 0 && id < a.classes) r.w += a.d_top[row * a.top_k + k];
+  }
+  r.ge = a.d_entropy ? a.d_entropy[row] : 0.f;
+  r.h = a.d_entropy ? a.entropy[row] : 0.f;
+  r.lse = lse;
+  if (lse == neg_inf()) {      // nothing is allowed: the row's gradient is 0
+    r.lse = 0.f;
+    r.w = r.ge = r.h = 0.f;
+    label = -2;
+  }
+  return r;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
+  constexpr int VEC = Elem<T>::VEC;
+  constexpr int MAXR = 256;
+  __shared__ GradRow prm[MAXR];
+  __shared__ int lab[MAXR];
+  const int64_t row0 = a.pieces > 1 ? (int64_t)(blockIdx.x / (unsigned)a.pieces) : (int64_t)blockIdx.x * a.rows_per_block;
+  const int c0 = a.pieces > 1 ? (int)(blockIdx.x % (unsigned)a.pieces) * a.span : 0;
+  const int c1 = a.pieces > 1 ? (a.classes - c0 < a.span ? a.classes : c0 + a.span) : a.classes;
+  const int nr = a.pieces > 1 ? 1 : (int)(a.rows - row0 < a.rows_per_block ? a.rows - row0 : a.rows_per_block);
+  for (int r = threadIdx.x; r < nr; r += 256) {
+    int64_t l;
+    prm[r] = grad_row<T>(a, row0 + r, l);
+    lab[r] = (int)l;
+  }
+  __syncthreads();
+  const int nvec = (c1 - c0 + VEC - 1) / VEC;
+  for (int i = threadIdx.x; i < nr * nvec; i += 256) {
+    const int r = i / nvec, c = c0 + (i - r * nvec) * VEC;
+    const GradRow p = prm[r];
+    const T* src = static_cast<const T*>(a.x) + (row0 + r) * a.stride;
+    const uint8_t* mask = a.allowed ? a.allowed + (row0 + r) * a.allowed_stride : nullptr;
+    T* dst = static_cast<T*>(a.grad) + (row0 + r) * a.grad_stride;
+    float f[VEC];
+    load_masked(src, mask, c, c1, f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = grad_dense(p, f[e]);
+    if (c + VEC <= c1) {
+      store16(dst + c, pack16<T>(f));
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (c + e < c1) dst[c + e] = Elem<T>::from(f[e]);
+    }
+  }
+  __syncthreads();      // the block's own stores are complete: the named elements are written over them
+  const int names = a.top_k + 1;
+  for (int i = threadIdx.x; i < nr * names; i += 256) {
+    const int r = i / names, k = i - r * names;
+    const int64_t row = row0 + r;
+    const int64_t id = k == 0 ? lab[r] : (lab[r] == -2 ? -1 : a.top_ids[row * a.top_k + k - 1]);
+    if (id < c0 || id >= c1) continue;
+    if (a.allowed && !a.allowed[row * a.allowed_stride + id]) continue;
+    const float x = Elem<T>::load(static_cast<const T*>(a.x) + row * a.stride + id);
+    if (x == neg_inf()) continue;
+    // every name of this element adds up here: threads that share an element write the same sum
+    float g = grad_dense(prm[r], x);
+    if (lab[r] == id) g += a.d_logprob[row];
+    for (int j = 0; j < a.top_k; ++j)
+      if (a.top_ids[row * a.top_k + j] == id) g += a.d_top[row * a.top_k + j];
+    static_cast<T*>(a.grad)[row * a.grad_stride + id] = Elem<T>::from(g);
+  }
+}
+
+}  // namespace pclseg
+
+#endif  // PCLSEG_SCORE_H_

@@ -41,7 +41,11 @@ EXPORTS = [
   "pclseg_num_tensors", "pclseg_tensor_info", "pclseg_read_tensor", "pclseg_op_normalize",
   "pclseg_op_conv2d", "pclseg_op_conv2d_transpose", "pclseg_op_max_pool", "pclseg_op_head",
   "pclseg_op_confusion_matrix", "pclseg_op_project", "pclseg_op_project_ex", "pclseg_op_split_f16_roundtrip",
+  "pclseg_i8_row_bytes", "pclseg_op_quantize_rows", "pclseg_op_matmul_i8", "pclseg_op_linear_i8_workspace",
+  "pclseg_op_linear_i8", "pclseg_op_label_logprobs_workspace", "pclseg_op_label_logprobs", "pclseg_op_label_logprobs_grad",
 ]
+
+DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}     # pclseg_dtype of a torch dtype's name
 
 
 class Desc(ctypes.Structure):
@@ -137,12 +141,23 @@ def load_library():
   lib.pclseg_op_project_ex.argtypes = [ctypes.POINTER(ProjDesc), vp, i32, ctypes.c_size_t, vp, vp, vp, vp, i32,
                                        vp, vp, vp, vp]
   lib.pclseg_op_split_f16_roundtrip.argtypes = [f32p, i32, i32, i32, i32, vp, vp]
+  i64, sz = ctypes.c_int64, ctypes.c_size_t
+  lib.pclseg_i8_row_bytes.argtypes = [i64]
+  lib.pclseg_op_quantize_rows.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp]
+  lib.pclseg_op_matmul_i8.argtypes = [vp, vp, vp, vp, i64, i64, i64, vp, i32, vp, i64, vp, i64, i32, vp]
+  lib.pclseg_op_linear_i8_workspace.argtypes = [i64, i64, i64, ctypes.POINTER(sz)]
+  lib.pclseg_op_linear_i8.argtypes = [vp, i32, i64, vp, vp, i64, i64, i64, vp, i32, vp, i64, vp, i64, i32, vp, sz, vp]
+  lib.pclseg_op_label_logprobs_workspace.argtypes = [i64, i64, i32, ctypes.POINTER(sz)]
+  lib.pclseg_op_label_logprobs.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp, i64, i32, vp, vp, vp, vp, vp, vp, sz, vp]
+  lib.pclseg_op_label_logprobs_grad.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp, i64, vp, vp, vp, vp, vp, vp, i32, vp,
+                                                i64, vp]
   for name in EXPORTS:
     fn = getattr(lib, name)
-    if name not in ("pclseg_last_error", "pclseg_host_alloc", "pclseg_build_sha"):
+    if name not in ("pclseg_last_error", "pclseg_host_alloc", "pclseg_build_sha", "pclseg_i8_row_bytes"):
       fn.restype = ctypes.c_int
   lib.pclseg_host_alloc.restype = ctypes.c_void_p
   lib.pclseg_build_sha.restype = ctypes.c_char_p
+  lib.pclseg_i8_row_bytes.restype = ctypes.c_int64
   _lib = lib
   return lib
 

@@ -1,0 +1,577 @@
+"""Row operators on the MI355X against float64 restatements of their formulas (tensors are copied to the CPU first).
+
+Tolerances count roundings: u = 2^-24 for each float32 operation, half a step of the output type for the final one
+(finfo(t).eps / 2 relative).  `chain` is the longest chain of additions a sum can pass through."""
+import math
+
+import pytest
+import torch
+
+from pclsegmentation_amd import ops
+
+pytestmark = [pytest.mark.gpu, pytest.mark.needs_hip]
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [F32, BF16, F16]
+
+
+def half_step(t):
+  return torch.finfo(t).eps / 2
+
+
+def tiny(t):
+  return torch.finfo(t).smallest_normal * torch.finfo(t).eps      # half a subnormal step and more
+
+
+def rnd(seed, *shape):
+  return torch.randn(shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64)
+
+
+def close(got, want, bound):
+  """|got - want| <= bound elementwise; the same infinities and NaNs."""
+  got = got.detach().cpu().double()
+  assert got.shape == want.shape, (got.shape, want.shape)
+  fin = torch.isfinite(want)
+  assert torch.equal(torch.nan_to_num(got[~fin], nan=7e77), torch.nan_to_num(want[~fin], nan=7e77))
+  excess = ((got - want).abs() - bound)[fin]
+  assert excess.numel() == 0 or excess.max() <= 0, "off by %g over the bound" % excess.max()
+
+
+# ---------------------------------------------------------------------------------------------- quantisation
+
+def quant64(x):
+  """codes and scales by the definition: the scale is a float32, the quotient exact to 2^-53."""
+  x = x.double()
+  scale = (x.abs().amax(-1).double() / 127.0).float()
+  s = scale.double().unsqueeze(-1)
+  q = torch.where(s > 0, torch.round(x / torch.where(s > 0, s, 1.0)), 0.0).clamp(-127, 127)
+  return q.to(torch.int8), scale
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 64), (33, 65), (7, 250), (9, 256), (4, 257), (6, 1000), (3, 2048),
+                                       (3, 2049), (2, 8192), (2, 9001), (300, 16), (1, 131071)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_rows_is_exact(cuda, rows, cols, dtype):
+  x = (rnd(rows * cols, rows, cols) * torch.exp(rnd(5, rows, 1) * 3).clamp(1e-3, 1e3)).to(dtype)
+  x[0] = 0
+  got = ops.quantize_rows(x.to(cuda))
+  q, scale = quant64(x)
+  assert torch.equal(got.scale.cpu(), scale) and torch.equal(got.codes.cpu(), q)
+  assert not got.data[:, cols:].any()
+
+
+def test_quantize_rows_half_steps_and_extremes(cuda):
+  # a row whose maximum is 127 * 2^e has the scale 2^e: multiples of half a step are exact ties
+  ties = torch.cat([torch.arange(-253, 254) / 2.0, torch.tensor([127.0, -127.0])])
+  x = torch.stack([ties, ties * 2.0 ** 60, ties * 2.0 ** -100, ties * 2.0 ** -140])
+  got = ops.quantize_rows(x.to(cuda))
+  want = torch.round(ties).to(torch.int8)          # torch rounds halves to even
+  for r in range(3):
+    assert torch.equal(got.codes[r].cpu(), want)
+  # a subnormal scale: the row itself is a subnormal number of steps, codes times scale stay within its half step
+  assert (got.dequantize()[3].cpu() - x[3]).abs().max() <= 2.0 ** -141 + 127 * 2.0 ** -150
+  x = torch.ones(5, 40)
+  x[0, 3], x[1, 39], x[2, 0] = math.nan, math.inf, -math.inf
+  x[3, :] = torch.finfo(F32).max
+  got = ops.quantize_rows(x.to(cuda))
+  assert torch.isnan(got.scale[:3]).all() and not got.codes[:3].any()
+  assert (got.codes[3:] == 127).all() and torch.isfinite(got.scale[3:]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_rows_layouts(cuda, dtype):
+  base = rnd(1, 6, 5, 40).to(dtype).to(cuda)
+  for view in (base[..., 3:36], base[:, 1], base.transpose(0, 1), base[..., ::2], base[0, :1].expand(4, 40), base.permute(2, 0, 1)):
+    q, scale = quant64(view.cpu().reshape(-1, view.shape[-1]))
+    got = ops.quantize_rows(view)
+    assert torch.equal(got.codes.cpu(), q) and torch.equal(got.scale.cpu(), scale)
+
+
+# ---------------------------------------------------------------------------------------------- product
+
+ACT64 = {"none": lambda v: v, "relu": lambda v: v.clamp(min=0), "leaky": lambda v: torch.where(v > 0, v, 0.1 * v),
+         "sigmoid": torch.sigmoid}
+
+
+def product64(qa, sa, qb, sb, bias, act, residual):
+  p = (qa.double() @ qb.double().t().contiguous()) * sa.double()[:, None] * sb.double()[None, :]
+  v = p + (bias.double() if bias is not None else 0.0)
+  y = ACT64[act](v)
+  # float32: the int32 sum, two scales, the bias, the activation; the sigmoid has slope <= 1/4 and |v| s(1-s) <= 1/4
+  bound = 4 * U * p.abs() + 2 * U * v.abs() + (8 * U if act == "sigmoid" else 0.0)
+  if residual is not None:
+    y = y + residual.double()
+    bound = bound + U * y.abs()
+  return y, bound
+
+
+def check_product(got, want, bound, dtype):
+  close(got, want, bound + half_step(dtype) * (want.abs() + bound) + tiny(dtype))
+
+
+PRODUCTS = [  # m, n, k
+  (1, 1, 1), (1, 8, 16), (1, 4096, 512), (2, 17, 63), (5, 100, 65), (16, 33, 128), (17, 257, 1000), (32, 16, 4096), (33, 70, 300),
+  (64, 511, 257), (65, 1, 5), (65, 129, 64), (127, 300, 40), (130, 64, 129), (200, 1000, 1000), (257, 513, 384), (3000, 4100, 200),
+  (4100, 3001, 64), (5000, 2600, 256), (1, 40, 131071), (70, 40, 20000)]
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_matmul_i8(cuda, m, n, k):
+  act = ["none", "relu", "leaky", "sigmoid"][(m + n) % 4]
+  dtype = TYPES[(m + k) % 3]
+  g = torch.Generator().manual_seed(m * 7 + n * 3 + k)
+  qa = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8)
+  qb = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8)
+  sa, sb = torch.rand(m, generator=g) * 1e-2 + 1e-4, torch.rand(n, generator=g) * 1e-2 / k ** 0.5 + 1e-6
+  bias = rnd(1, n).float() if n % 2 else None
+  residual = rnd(2, m, n).to(dtype) if m % 2 else None
+  a, b = ops.Int8Rows.from_codes(qa.to(cuda), sa.to(cuda)), ops.Int8Rows.from_codes(qb.to(cuda), sb.to(cuda))
+  got = ops.matmul_i8(a, b, bias=None if bias is None else bias.to(cuda), act=act,
+                      residual=None if residual is None else residual.to(cuda), out_dtype=dtype)
+  assert got.dtype == dtype
+  want, bound = product64(qa, sa, qb, sb, bias, act, residual)
+  check_product(got, want, bound, dtype)
+
+
+def test_matmul_i8_sums_are_exact(cuda):
+  """The largest sum int32 holds, unit scales, float32 out: one rounding."""
+  k = 131071
+  a = torch.full((3, k), -128, dtype=torch.int8)
+  b = torch.full((70, k), -128, dtype=torch.int8)
+  b[1] = 127
+  a[2, ::2] = 127
+  ra = ops.Int8Rows.from_codes(a.to(cuda), torch.ones(3, device=cuda))
+  rb = ops.Int8Rows.from_codes(b.to(cuda), torch.ones(70, device=cuda))
+  want = (a.double() @ b.double().t().contiguous())
+  assert torch.equal(ops.matmul_i8(ra, rb).cpu(), want.float())
+  assert torch.equal(ops.matmul_i8(rb, ra).cpu(), want.t().float())
+
+
+@pytest.mark.parametrize("m", [1, 7, 48, 100, 600])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_i8(cuda, m, dtype):
+  k, n = 333, 260
+  x = rnd(m, m, k).to(dtype)
+  w = ops.quantize_rows((rnd(3, n, k) * 0.05).float().to(cuda))
+  bias, residual = rnd(4, n).float(), rnd(5, m, n).to(dtype)
+  got = ops.linear_i8(x.to(cuda), w, bias=bias.to(cuda), act="leaky", residual=residual.to(cuda))
+  q, s = quant64(x)
+  want, bound = product64(q, s, w.codes.cpu(), w.scale.cpu(), bias, "leaky", residual)
+  check_product(got, want, bound, dtype)
+  # the same numbers in two calls, another output type, batched axes, strided rows
+  assert torch.equal(ops.matmul_i8(ops.quantize_rows(x.to(cuda)), w, bias=bias.to(cuda), act="leaky",
+                                   residual=residual.to(cuda), out_dtype=dtype), got)
+  plain = ops.linear_i8(x.to(cuda), w, out_dtype=F32)
+  check_product(plain, *product64(q, s, w.codes.cpu(), w.scale.cpu(), None, "none", None), F32)
+  wide = torch.zeros(m, 2 * k, dtype=dtype, device=cuda)
+  wide[:, 5:5 + k] = x.to(cuda)
+  assert torch.equal(ops.linear_i8(wide[:, 5:5 + k], w, out_dtype=F32), plain)
+  assert torch.equal(ops.linear_i8(x.to(cuda).view(1, m, 1, k), w, out_dtype=F32), plain.view(1, m, 1, n))
+
+
+def test_linear_i8_bad_rows_stay_in_their_row(cuda):
+  x = rnd(1, 70, 100).float()
+  x[3, 5], x[60, 99] = math.nan, math.inf
+  w = ops.quantize_rows(rnd(2, 40, 100).float().to(cuda))
+  for rows in (70, 8):
+    y = ops.linear_i8(x[:rows].to(cuda), w, act="relu").cpu()
+    bad = torch.zeros(rows, dtype=torch.bool)
+    bad[3] = True
+    if rows > 60:
+      bad[60] = True
+    assert torch.isnan(y[bad]).all() and torch.isfinite(y[~bad]).all()
+
+
+def test_linear_i8_matches_a_1x1_convolution(cuda):
+  """Int8Rows.from_kernel takes the Keras kernel of op_conv2d: the two layers agree to the 8-bit codes' half steps."""
+  import numpy as np
+  from pclsegmentation_amd import engine as E
+  n, h, w, cin, cout = 1, 4, 16, 64, 32
+  x = rnd(1, n, h, w, cin).float().to(cuda)
+  kernel = (rnd(2, 1, 1, cin, cout) * 0.1).float()
+  bias = rnd(3, cout).float()
+  y = torch.empty((n, h, w, cout), dtype=F32, device=cuda)
+  E.op_conv2d(x, n, h, w, cin, kernel.numpy(), 1, bias.numpy(), None, "leaky", None, y, math="f32")
+  torch.cuda.synchronize()
+  weight = ops.Int8Rows.from_kernel(kernel.to(cuda))
+  got = ops.linear_i8(x, weight, bias=bias.to(cuda), act="leaky")
+  sx = x.abs().amax(-1, keepdim=True).double() / 127
+  sw = kernel.abs().amax(2).double().view(1, 1, 1, cout).to(cuda) / 127
+  # each factor is off by half a step: sum |x| sw/2 + |w| sx/2 + sx sw / 4
+  bound = x.abs().double().sum(-1, keepdim=True) * sw / 2 + (sx / 2) * kernel.abs().double().sum(2).view(1, 1, 1, cout).to(cuda)
+  bound = (bound + cin * sx * sw / 4).cpu() * (1 + 1e-4) + 1e-5
+  close(got, y.cpu().double(), bound)
+  assert isinstance(np.asarray(bias), np.ndarray)
+
+
+# ---------------------------------------------------------------------------------------------- log probabilities
+
+def score64(x, labels, top_k, allowed):
+  x = x.double()
+  v = x.shape[-1]
+  if allowed is not None:
+    x = torch.where(allowed.bool(), x, torch.full((), -math.inf, dtype=torch.float64))
+  m = x.amax(-1)
+  bad = torch.isnan(x).any(-1) | (m == math.inf)
+  empty = (m == -math.inf) & ~bad
+  mm = torch.where(torch.isfinite(m), m, torch.zeros_like(m))
+  z = x - mm[:, None]
+  e = torch.exp(z)
+  s = e.sum(-1)
+  lse = mm + torch.log(s)
+  p = torch.where(empty[:, None], torch.zeros_like(e), e / s[:, None])
+  zz = torch.where(p > 0, z, torch.zeros_like(z))
+  h = torch.where(empty, torch.zeros_like(s), torch.log(s) - (p * zz).sum(-1))
+  nan = torch.full_like(lse, math.nan)
+  out = {"x": x, "p": p, "empty": empty, "bad": bad, "a": (p * zz.abs()).sum(-1), "b": (p * zz * zz).sum(-1), "m": mm,
+         "logs": torch.log(s)}
+  if labels is not None:
+    lab = labels.long()
+    known = (lab >= 0) & (lab < v)
+    at = x.gather(1, lab.clamp(0, v - 1)[:, None])[:, 0]
+    # (x - m) - ln s: x - lse would lose ln s beside the extremes of the types
+    lp = torch.where(at == -math.inf, at, (at - mm) - torch.log(s))
+    out["logprob"] = torch.where(known, torch.where(bad, nan, lp), torch.zeros_like(lse))
+  out["entropy"] = torch.where(bad, nan, h)
+  out["lse"] = torch.where(bad, nan, torch.where(empty, torch.full_like(lse, -math.inf), lse))
+  xs = torch.where(bad[:, None], torch.full_like(x, -math.inf), x) + 0.0
+  order = torch.sort(xs, dim=-1, descending=True, stable=True)
+  k = min(top_k, v)
+  ids, best = order.indices[:, :k], order.values[:, :k]
+  gone = best == -math.inf
+  ids = torch.where(gone, -1, ids).to(torch.int32)
+  best = torch.where(gone, best, (best - mm[:, None]) - torch.log(s)[:, None])
+  best = torch.where(bad[:, None], nan[:, None], best)
+  pad = top_k - k
+  if pad:
+    ids = torch.cat([ids, torch.full((len(ids), pad), -1, dtype=torch.int32)], 1)
+    best = torch.cat([best, torch.full((len(ids), pad), -math.inf, dtype=torch.float64)], 1)
+    best = torch.where(bad[:, None], nan[:, None], best)
+  out["top_ids"], out["top_logprobs"] = ids, best
+  return out
+
+
+def check_score(got, ref, v, top_k):
+  chain = 64 + 32 * (v // 8192 + 1)
+  a, b, logs, m = ref["a"], ref["b"], ref["logs"].abs(), ref["m"].abs()
+  a, b, logs = [torch.nan_to_num(t, 0.0, 0.0, 0.0) for t in (a, b, logs)]
+  rel_s = U * (chain + 4 + 4 * a)
+  log_s = rel_s + 2 * U * logs                                      # logf
+  lse, h = [torch.nan_to_num(ref[t], 0.0, 0.0, 0.0).abs() for t in ("lse", "entropy")]
+  close(got.lse, ref["lse"], log_s + U * (m + lse))
+  close(got.entropy, ref["entropy"], log_s + rel_s * a + U * (4 * b + (8 + chain) * a + h))
+  if got.logprob is not None:
+    lp = torch.nan_to_num(ref["logprob"], 0.0, 0.0, 0.0).abs()
+    close(got.logprob, ref["logprob"], log_s + U * (lp + logs) + U * lp)      # |x - M| <= |logprob| + |ln S|
+  if top_k:
+    assert torch.equal(got.top_ids.cpu(), ref["top_ids"])
+    lp = torch.nan_to_num(ref["top_logprobs"], 0.0, 0.0, 0.0).abs()
+    close(got.top_logprobs, ref["top_logprobs"], log_s[:, None] + U * (lp + logs[:, None]) + U * lp)
+  else:
+    assert got.top_ids is None and got.top_logprobs is None
+
+
+def labels_for(rows, v, seed, dtype=torch.int32):
+  return torch.randint(-2, v + 2, (rows,), generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+SCORES = [(1, 1, 1), (5, 2, 3), (300, 3, 2), (257, 8, 8), (1000, 20, 3), (513, 31, 5), (70, 32, 32), (65, 33, 2), (40, 64, 64), (33, 100, 4),
+          (31, 256, 20), (17, 257, 3), (9, 511, 32), (10, 513, 1), (6, 1031, 64), (5, 2048, 20), (7, 2049, 20), (3, 4097, 5), (4, 8193, 64),
+          (2, 30001, 20), (600, 2500, 3), (1, 131072, 20), (3, 131071, 32), (1, 300000, 64), (1000, 5000, 0), (2, 9000, 0), (50, 77, 0)]
+
+
+@pytest.mark.parametrize("rows,v,top_k", SCORES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_label_logprobs(cuda, rows, v, top_k, dtype):
+  x = (rnd(v + rows, rows, v) * 3).to(dtype)
+  x[0] += 50
+  labels = labels_for(rows, v, v, torch.int64 if rows % 2 else torch.int32)
+  got = ops.label_logprobs(x.to(cuda), labels.to(cuda), top_k=top_k)
+  check_score(got, score64(x, labels, top_k, None), v, top_k)
+  again = ops.label_logprobs(x.to(cuda), labels.to(cuda), top_k=top_k)
+  assert all(u is None or torch.equal(u, w) for u, w in zip(got, again))
+
+
+@pytest.mark.parametrize("rows,v,top_k", [(40, 5, 3), (40, 20, 3), (20, 33, 7), (20, 300, 64), (20, 2000, 9), (12, 2100, 20), (12, 20003, 33)])
+@pytest.mark.parametrize("per_row", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_label_logprobs_masks(cuda, rows, v, top_k, per_row, dtype):
+  """Excluded classes hold whatever: NaN, infinities, the type's extremes.  Rows with nothing, one, or a few left."""
+  g = torch.Generator().manual_seed(v)
+  x = (rnd(v, rows, v) * 2).to(dtype)
+  allowed = torch.rand((rows, v) if per_row else (v,), generator=g) < 0.6
+  if per_row:
+    allowed[0] = False
+    allowed[1] = False
+    allowed[1, v - 1] = True
+    allowed[2] = torch.arange(v) < 2
+  else:
+    allowed[0], allowed[v - 1] = False, True
+  full = allowed.expand(rows, v)
+  fill = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(dtype).min, torch.finfo(dtype).max])
+  junk = fill[torch.randint(0, 5, (rows, v), generator=g)].to(dtype)
+  x = torch.where(full, x, junk)
+  labels = labels_for(rows, v, 3)
+  ref = score64(x, labels, top_k, full)
+  got = ops.label_logprobs(x.to(cuda), labels.to(cuda), top_k=top_k, allowed=allowed.to(cuda))
+  check_score(got, ref, v, top_k)
+  # the same mask as bytes, as a strided view, and its effect spelled as logits of -inf
+  wide = torch.zeros((rows, 2 * v + 3), dtype=torch.uint8, device=cuda)
+  wide[:, 1:1 + v] = full.to(cuda)
+  same = ops.label_logprobs(x.to(cuda), labels.to(cuda), top_k=top_k, allowed=wide[:, 1:1 + v])
+  inf = ops.label_logprobs(torch.where(full, x, torch.full((), -math.inf, dtype=dtype)).to(cuda), labels.to(cuda), top_k=top_k)
+  for other in (same, inf):
+    assert all(torch.equal(u, w) for u, w in zip(got, other))
+
+
+@pytest.mark.parametrize("v", [7, 32, 40, 500, 2048, 2049, 20000, 131072])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_label_logprobs_odd_rows(cuda, v, dtype):
+  """Equal logits (ids ascend), rising, falling, the lowest value throughout, all -inf, signed zeros, far outliers, NaN, +inf."""
+  lo, hi = torch.finfo(dtype).min, torch.finfo(dtype).max
+  ramp = torch.arange(v, dtype=torch.float64) * (8.0 / v)
+  rows = [torch.full((v,), 1.5), ramp, -ramp, torch.full((v,), lo), torch.full((v,), -math.inf), torch.zeros(v),
+          torch.where(torch.arange(v) == v // 2, 1e4, 0.0), torch.where(torch.arange(v) == 1, lo, 0.5), torch.full((v,), hi),
+          torch.where(torch.arange(v) == v - 1, math.nan, 1.0), torch.where(torch.arange(v) == 0, math.inf, 1.0),
+          torch.where(torch.arange(v) % 3 == 1, -math.inf, 2.0), torch.where(torch.arange(v) == v - 1, 1.0, -math.inf)]
+  x = torch.stack([r.double() for r in rows]).to(dtype)
+  x[5, ::2] = -0.0
+  labels = torch.arange(len(x), dtype=torch.int32) % v
+  k = min(v, 40)
+  ref = score64(x, labels, k, None)
+  check_score(ops.label_logprobs(x.to(cuda), labels.to(cuda), top_k=k), ref, v, k)
+  # one row at a time takes the split path of long rows
+  for r in range(len(x)):
+    one = {n: t[r:r + 1] for n, t in ref.items()}
+    check_score(ops.label_logprobs(x[r:r + 1].to(cuda), labels[r:r + 1].to(cuda), top_k=k), one, v, k)
+
+
+def test_label_logprobs_layouts(cuda):
+  base = rnd(1, 6, 4, 90).float().to(cuda)
+  for view in (base[..., 3:60], base[:, 2], base.transpose(0, 1), base[..., ::3], base[:1, :1].expand(5, 2, 90), base[0, 0]):
+    v = view.shape[-1]
+    flat = view.cpu().reshape(-1, v)
+    labels = labels_for(len(flat), v, 1).view(view.shape[:-1])
+    got = ops.label_logprobs(view, labels.to(cuda), top_k=2)
+    assert got.lse.shape == view.shape[:-1] and got.top_ids.shape == view.shape[:-1] + (2,)
+    ref = score64(flat, labels.reshape(-1), 2, None)
+    check_score(ops.LabelLogprobs(*[t.reshape(-1, *t.shape[view.dim() - 1:]) for t in got]), ref, v, 2)
+  assert ops.label_logprobs(base).logprob is None
+  none = ops.label_logprobs(base[:0], top_k=3)
+  assert none.lse.shape == (0, 4) and none.top_ids.shape == (0, 4, 3)
+
+
+# ---------------------------------------------------------------------------------------------- gradient
+
+def grad64(ref, labels, lse, entropy, d_lp, d_h, ids, d_top, dtype):
+  x = ref["x"]
+  v = x.shape[1]
+  lse = torch.where(ref["empty"], torch.zeros_like(lse), lse)
+  z = torch.where(x == -math.inf, torch.zeros_like(x), x - lse[:, None])
+  p = torch.where(x == -math.inf, torch.zeros_like(x), torch.exp(z))
+  named, named_abs = torch.zeros_like(p), torch.zeros_like(p)
+  if d_lp is not None:
+    lab = labels.long()
+    known = (lab >= 0) & (lab < v)
+    g = torch.where(known, d_lp, torch.zeros_like(d_lp))
+    named.scatter_add_(1, lab.clamp(0, v - 1)[:, None], g[:, None])
+    named_abs.scatter_add_(1, lab.clamp(0, v - 1)[:, None], g.abs()[:, None])
+  k = 1
+  if d_top is not None:
+    g = torch.where(ids >= 0, d_top, torch.zeros_like(d_top))
+    named.scatter_add_(1, ids.long().clamp(min=0), g)
+    named_abs.scatter_add_(1, ids.long().clamp(min=0), g.abs())
+    k += ids.shape[1]
+  w, w_abs = named.sum(1, keepdim=True), named_abs.sum(1, keepdim=True)
+  ge = d_h[:, None] if d_h is not None else torch.zeros_like(w)
+  h = (entropy if d_h is not None else torch.zeros_like(lse))[:, None]
+  grad = named - p * (w + ge * (z + h))
+  # p: x - lse, the product with log2 e, the exponential; the bracket: k + 1 sums and one fma
+  inner = w_abs + ge.abs() * (z.abs() + (h - lse[:, None]).abs() + lse[:, None].abs())
+  bound = p * inner * U * (3 * z.abs() + k + 10) + U * (k + 1) * (named_abs + p * inner)
+  off = (x == -math.inf) | ref["empty"][:, None]
+  grad, bound = [torch.where(off, torch.zeros_like(t), t) for t in (grad, bound)]
+  bound = bound + half_step(dtype) * (grad.abs() + bound) + tiny(dtype) + 2.0 ** -140
+  return grad, bound
+
+
+@pytest.mark.parametrize("rows,v,top_k", [(1, 1, 1), (700, 20, 3), (300, 3, 2), (9, 33, 40), (64, 100, 5), (33, 1031, 32), (5, 4099, 20),
+                                          (3, 8192, 2), (3, 8193, 3), (2, 50001, 20), (1, 131072, 64), (2000, 2, 1)])
+@pytest.mark.parametrize("parts", ["lp", "h", "top", "lp+h+top"])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_label_logprobs_grad(cuda, rows, v, top_k, parts, dtype):
+  x = (rnd(v, rows, v) * 2).to(dtype)
+  g = torch.Generator().manual_seed(v)
+  allowed = torch.rand((rows, v), generator=g) < 0.8 if v > 1 and rows % 2 else None
+  if allowed is not None:
+    allowed[0] = False
+    x[1 % rows][~allowed[1 % rows]] = math.nan
+  labels = labels_for(rows, v, 9, torch.int64 if v % 2 else torch.int32)
+  ref = score64(x, labels, top_k, allowed)
+  dev = lambda t: None if t is None else t.to(cuda)
+  fwd = ops.label_logprobs(dev(x), dev(labels), top_k=top_k, allowed=dev(allowed))
+  d_lp = rnd(1, rows).float() if "lp" in parts else None
+  d_h = rnd(2, rows).float() if "h" in parts.split("+") else None
+  d_top = rnd(3, rows, top_k).float() if "top" in parts else None
+  got = ops.label_logprobs_grad(dev(x), dev(labels), fwd.lse, d_logprob=dev(d_lp), entropy=fwd.entropy, d_entropy=dev(d_h),
+                                top_ids=fwd.top_ids, d_top=dev(d_top), allowed=dev(allowed))
+  assert got.dtype == dtype and got.shape == x.shape
+  d64 = [None if t is None else t.double() for t in (d_lp, d_h, d_top)]
+  want, bound = grad64(ref, labels, fwd.lse.cpu().double(), fwd.entropy.cpu().double(), d64[0], d64[1], fwd.top_ids.cpu(), d64[2], dtype)
+  close(got, want, bound)
+
+
+def test_label_logprobs_grad_against_differences(cuda):
+  """Central differences of the float64 loss; h = 1e-4 leaves a truncation below 1e-7 and a cancellation below 1e-10."""
+  rows, v, k = 4, 37, 3
+  x = rnd(1, rows, v)
+  labels = torch.tensor([0, 36, -1, 5], dtype=torch.int32)
+  a, b, c = rnd(2, rows), rnd(3, rows), rnd(4, rows, k)
+  allowed = torch.rand((rows, v), generator=torch.Generator().manual_seed(5)) < 0.8
+  allowed[:, 0], allowed[:, 36], allowed[:, 5] = True, True, True
+  x = x.float().double()
+  ids = score64(x, labels, k, allowed)["top_ids"]
+
+  def loss(y):
+    r = score64(y, labels, k, allowed)
+    top = (y - r["lse"][:, None]).gather(1, ids.long())
+    return (r["logprob"] * a + r["entropy"] * b).sum() + (top * c).sum()
+
+  h, want = 1e-4, torch.zeros_like(x)
+  for r in range(rows):
+    for j in range(v):
+      if allowed[r, j]:
+        d = torch.zeros_like(x)
+        d[r, j] = h
+        want[r, j] = (loss(x + d) - loss(x - d)) / (2 * h)
+  dev = lambda t: t.float().to(cuda)
+  fwd = ops.label_logprobs(dev(x), labels.to(cuda), top_k=k, allowed=allowed.to(cuda))
+  got = ops.label_logprobs_grad(dev(x), labels.to(cuda), fwd.lse, d_logprob=dev(a), entropy=fwd.entropy, d_entropy=dev(b),
+                                top_ids=fwd.top_ids, d_top=dev(c), allowed=allowed.to(cuda))
+  assert (got.cpu().double() - want).abs().max() <= 1e-5        # 40 roundings of terms up to 5
+
+
+def test_label_logprobs_grad_names_that_coincide(cuda):
+  """The label among the alternatives, and the same alternative named twice: their gradients add up."""
+  x = rnd(1, 3, 50).float()
+  labels = torch.tensor([4, 4, 9], dtype=torch.int32)
+  ids = torch.tensor([[4, 4, 7], [1, 2, -1], [9, 9, 9]], dtype=torch.int32)
+  d_lp, d_top = rnd(2, 3), rnd(3, 3, 3)
+  ref = score64(x, labels, 3, None)
+  got = ops.label_logprobs_grad(x.to(cuda), labels.to(cuda), ref["lse"].float().to(cuda), d_logprob=d_lp.float().to(cuda),
+                                top_ids=ids.to(cuda), d_top=d_top.float().to(cuda))
+  want, bound = grad64(ref, labels, ref["lse"].float().double(), None, d_lp.float().double(), None, ids, d_top.float().double(), F32)
+  close(got, want, bound)
+
+
+def test_label_logprobs_grad_layouts(cuda):
+  base = rnd(1, 6, 4, 90).to(BF16).to(cuda)
+  for view in (base[..., 3:60], base[:, 2], base.transpose(0, 1), base[..., ::3]):
+    v = view.shape[-1]
+    labels = labels_for(view[..., 0].numel(), v, 1).view(view.shape[:-1]).to(cuda)
+    fwd = ops.label_logprobs(view, labels)
+    one = torch.ones((), device=cuda).expand(view.shape[:-1])       # the gradient of a sum: a broadcast scalar
+    got = ops.label_logprobs_grad(view, labels, fwd.lse, d_logprob=one)
+    want = ops.label_logprobs_grad(view.contiguous(), labels.contiguous(), fwd.lse.contiguous(), d_logprob=one.contiguous())
+    assert got.shape == view.shape and torch.equal(got, want)
+
+
+# ---------------------------------------------------------------------------------------------- together
+
+def chain(x, w, bias, labels, allowed, d_lp, d_h):
+  logits = ops.linear_i8(x, w, bias=bias)
+  fwd = ops.label_logprobs(logits, labels, top_k=5, allowed=allowed)
+  grad = ops.label_logprobs_grad(logits, labels, fwd.lse, d_logprob=d_lp, entropy=fwd.entropy, d_entropy=d_h, allowed=allowed)
+  return (logits,) + tuple(fwd) + (grad,)
+
+
+def chain_inputs(cuda, m, k, v, seed, dtype=BF16):
+  x = rnd(seed, m, k).to(dtype).to(cuda)
+  w = ops.quantize_rows((rnd(seed + 1, v, k) * 0.1).float().to(cuda))
+  allowed = (torch.arange(v) != 0).to(cuda)
+  return [x, w, rnd(seed + 2, v).float().to(cuda), labels_for(m, v, seed).to(cuda), allowed, rnd(seed + 3, m).float().to(cuda),
+          rnd(seed + 4, m).float().to(cuda)]
+
+
+@pytest.mark.parametrize("m,k,v", [(1, 256, 40000), (130, 100, 20), (70, 512, 1000)])
+def test_a_layer_its_scores_and_their_gradient(cuda, m, k, v):
+  a = chain_inputs(cuda, m, k, v, 11)
+  logits, lp, h, lse, ids, tops, grad = chain(*a)
+  x, w, bias, labels, allowed, d_lp, d_h = [t.cpu() if torch.is_tensor(t) else t for t in a]
+  q, s = quant64(x)
+  check_product(logits, *product64(q, s, w.codes.cpu(), w.scale.cpu(), bias, "none", None), BF16)
+  ref = score64(logits.cpu(), labels, 5, allowed.expand(m, v))
+  check_score(ops.LabelLogprobs(lp, h, lse, ids, tops), ref, v, 5)
+  want, bound = grad64(ref, labels, lse.cpu().double(), h.cpu().double(), d_lp.double(), d_h.double(), None, None, BF16)
+  close(grad, want, bound)
+
+
+@pytest.mark.parametrize("m,k,v", [(1, 256, 40000), (300, 100, 20)])
+def test_captured_and_replayed(cuda, m, k, v):
+  """Two graphs of the chain, replayed in turn with new inputs and eager calls between: every replay equals the eager result."""
+  side = torch.cuda.Stream(cuda)
+  static = [chain_inputs(cuda, m, k, v, 20), chain_inputs(cuda, m, k, v, 30)]
+  chain(*static[0])
+  torch.cuda.synchronize()
+  graphs, outs = [], []
+  for s in static:
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+      outs.append(chain(*s))
+    graphs.append(g)
+  for it in range(4):
+    for n in (0, 1):
+      fresh = chain_inputs(cuda, m, k, v, 40 + 7 * it + n)
+      for dst, src in zip(static[n], fresh):
+        if torch.is_tensor(dst):
+          dst.copy_(src)
+        else:
+          dst.data.copy_(src.data)
+          dst.scale.copy_(src.scale)
+    want = [chain(*s) for s in static]
+    torch.cuda.synchronize()
+    for g in graphs:
+      g.replay()
+    torch.cuda.synchronize()
+    for n in (0, 1):
+      for got, ref in zip(outs[n], want[n]):
+        assert torch.equal(got, ref)
+
+
+def test_two_streams_at_once(cuda):
+  ins = [chain_inputs(cuda, 1, 256, 40000, 50), chain_inputs(cuda, 90, 256, 3001, 60)]
+  want = [chain(*i) for i in ins]
+  torch.cuda.synchronize()
+  streams = [torch.cuda.Stream(cuda), torch.cuda.Stream(cuda)]
+  got = [[], []]
+  for _ in range(5):
+    for n in (0, 1):
+      with torch.cuda.stream(streams[n]):
+        got[n].append(chain(*ins[n]))
+  torch.cuda.synchronize()
+  for n in (0, 1):
+    for run in got[n]:
+      assert all(torch.equal(a, b) for a, b in zip(run, want[n]))
+
+
+def test_only_the_rows_are_written(cuda):
+  """The C entry points write the outputs' rows and nothing beside them."""
+  from pclsegmentation_amd import engine as E
+  lib, stream = E.load_library(), E.stream_handle(cuda)
+  for m, n, k in ((3, 21, 70), (70, 33, 130)):
+    w = ops.quantize_rows(rnd(1, n, k).float().to(cuda))
+    x = ops.quantize_rows(rnd(2, m, k).float().to(cuda))
+    y = torch.full((m + 2, n + 7), 5.0, device=cuda)
+    E.check(lib.pclseg_op_matmul_i8(x.data.data_ptr(), x.scale.data_ptr(), w.data.data_ptr(), w.scale.data_ptr(), m, n, k, None, 0,
+                                    None, 0, y.data_ptr(), n + 7, 0, stream))
+    assert (y[m:] == 5).all() and (y[:, n:] == 5).all() and torch.equal(y[:m, :n], ops.matmul_i8(x, w))
+  for m, v in ((5, 21), (3, 9001)):
+    logits = rnd(3, m, v).float().to(cuda)
+    labels = labels_for(m, v, 1).to(cuda)
+    fwd = ops.label_logprobs(logits, labels)
+    d = torch.ones(m, device=cuda)
+    grad = torch.full((m + 1, v + 5), 5.0, device=cuda)
+    E.check(lib.pclseg_op_label_logprobs_grad(logits.data_ptr(), 0, m, v, v, labels.data_ptr(), 4, None, 0, fwd.lse.data_ptr(), None,
+                                              d.data_ptr(), None, None, None, 0, grad.data_ptr(), v + 5, stream))
+    assert (grad[m:] == 5).all() and (grad[:, v:] == 5).all()
+    assert torch.equal(grad[:m, :v], ops.label_logprobs_grad(logits, labels, fwd.lse, d_logprob=d))

@@ -1,0 +1,174 @@
+"""Row operators without a GPU: every refusal of the C entry points and of pclsegmentation_amd.ops (a refused call launches
+nothing), the layout helper, the exception barrier."""
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+from pclsegmentation_amd import engine as E
+from pclsegmentation_amd import ops
+
+BUF = (ctypes.c_uint8 * 4096)()
+P = (ctypes.addressof(BUF) + 255) // 256 * 256        # an aligned address that a refused call must not touch
+
+
+def _refused(fn, args, code, word):
+  lib = E.load_library()
+  assert getattr(lib, fn)(*args) == code
+  assert word in lib.pclseg_last_error(None).decode(), lib.pclseg_last_error(None)
+
+
+def test_row_bytes():
+  f = E.load_library().pclseg_i8_row_bytes
+  assert [f(k) for k in (0, -1, 131072, 1 << 40)] == [0, 0, 0, 0]
+  assert [f(k) for k in (1, 64, 65, 128, 129, 1000, 131071)] == [64, 64, 128, 128, 256, 1024, 131072]
+
+
+QUANT = dict(x=P, dtype=0, rows=2, cols=8, x_stride=8, q=P, scale=P, stream=None)
+
+
+@pytest.mark.parametrize("change,code,word", [
+  (dict(dtype=3), -1, "dtype"), (dict(rows=-1), -2, "rows"), (dict(rows=1 << 31), -2, "rows"), (dict(cols=0), -2, "cols"),
+  (dict(cols=131072), -2, "cols"), (dict(x_stride=7), -2, "stride"), (dict(x=None), -1, "NULL"), (dict(q=None), -1, "NULL"),
+  (dict(scale=None), -1, "NULL"), (dict(x=P + 2), -1, "misaligned"), (dict(q=P + 4), -1, "misaligned"),
+])
+def test_quantize_rows_refuses(change, code, word):
+  _refused("pclseg_op_quantize_rows", list({**QUANT, **change}.values()), code, word)
+
+
+MATMUL = dict(a=P, a_scale=P, b=P, b_scale=P, m=2, n=3, k=8, bias=None, act=0, residual=None, residual_stride=0, y=P, y_stride=3,
+              dtype=1, stream=None)
+
+
+@pytest.mark.parametrize("change,code,word", [
+  (dict(dtype=-1), -1, "dtype"), (dict(act=4), -1, "activation"), (dict(m=-1), -2, "m must"), (dict(n=0), -2, "n must"),
+  (dict(n=1 << 31), -2, "n must"), (dict(k=0), -2, "k must"), (dict(k=131072), -2, "k must"), (dict(a=None), -1, "NULL"),
+  (dict(b=None), -1, "NULL"), (dict(y=None), -1, "NULL"), (dict(a=P + 8), -1, "aligned"), (dict(b=P + 8), -1, "aligned"),
+  (dict(y_stride=2), -2, "stride"), (dict(residual=P, residual_stride=2), -2, "stride"), (dict(y=P + 1), -1, "misaligned"),
+  (dict(m=1 << 40, n=1 << 20, y_stride=1 << 20), -2, "tiles"),
+])
+def test_matmul_i8_refuses(change, code, word):
+  _refused("pclseg_op_matmul_i8", list({**MATMUL, **change}.values()), code, word)
+
+
+LINEAR = dict(x=P, dtype=0, x_stride=8, weight=P, weight_scale=P, m=2, n=3, k=8, bias=None, act=0, residual=None,
+              residual_stride=0, y=P, y_stride=3, y_dtype=1, workspace=P, workspace_bytes=2 * 68, stream=None)
+
+
+@pytest.mark.parametrize("change,code,word", [
+  (dict(dtype=7), -1, "dtype"), (dict(y_dtype=7), -1, "dtype"), (dict(x_stride=7), -2, "stride"), (dict(x=None), -1, "NULL"),
+  (dict(workspace=None), -1, "NULL"), (dict(workspace_bytes=2 * 68 - 1), -1, "workspace"), (dict(workspace=P + 8), -1, "misaligned"),
+  (dict(m=1 << 31), -2, "m must"), (dict(x=P + 1), -1, "misaligned"),
+])
+def test_linear_i8_refuses(change, code, word):
+  _refused("pclseg_op_linear_i8", list({**LINEAR, **change}.values()), code, word)
+
+
+def test_workspace_sizes():
+  lib, size = E.load_library(), ctypes.c_size_t()
+  assert lib.pclseg_op_linear_i8_workspace(5, 7, 65, ctypes.byref(size)) == 0 and size.value >= 5 * (128 + 4)
+  assert lib.pclseg_op_linear_i8_workspace(5, 7, 0, ctypes.byref(size)) == -2
+  assert lib.pclseg_op_linear_i8_workspace(5, 7, 8, None) == -1
+  for rows, classes in ((1, 20), (1, 2048), (1 << 20, 50000)):
+    assert lib.pclseg_op_label_logprobs_workspace(rows, classes, 5, ctypes.byref(size)) == 0 and size.value == 0
+  assert lib.pclseg_op_label_logprobs_workspace(1, 131072, 5, ctypes.byref(size)) == 0 and size.value > 0
+  assert lib.pclseg_op_label_logprobs_workspace(0, 131072, 5, ctypes.byref(size)) == 0 and size.value == 0
+  assert lib.pclseg_op_label_logprobs_workspace(1, 0, 5, ctypes.byref(size)) == -2
+  assert lib.pclseg_op_label_logprobs_workspace(1, 5, 65, ctypes.byref(size)) == -1
+
+
+SCORE = dict(logits=P, dtype=0, rows=2, classes=4, stride=4, labels=P, label_bytes=4, allowed=None, allowed_stride=0, top_k=0,
+             logprob=P, entropy=P, lse=P, top_ids=None, top_logprobs=None, workspace=None, workspace_bytes=0, stream=None)
+
+
+@pytest.mark.parametrize("change,code,word", [
+  (dict(dtype=9), -1, "dtype"), (dict(rows=-1), -2, "rows"), (dict(classes=0), -2, "classes"), (dict(classes=1 << 31), -2, "classes"),
+  (dict(stride=3), -2, "stride"), (dict(top_k=65), -1, "top_k"), (dict(top_k=-1), -1, "top_k"), (dict(logits=None), -1, "NULL"),
+  (dict(label_bytes=2), -1, "int32"), (dict(labels=P + 2), -1, "misaligned"), (dict(labels=None), -1, "labels"),
+  (dict(top_k=2), -1, "top_ids"), (dict(allowed=P, allowed_stride=3), -2, "mask"), (dict(logits=P + 2), -1, "misaligned"),
+  (dict(classes=131072, stride=131072, rows=1), -1, "workspace"),
+])
+def test_label_logprobs_refuses(change, code, word):
+  _refused("pclseg_op_label_logprobs", list({**SCORE, **change}.values()), code, word)
+
+
+GRAD = dict(logits=P, dtype=0, rows=2, classes=4, stride=4, labels=P, label_bytes=4, allowed=None, allowed_stride=0, lse=P,
+            entropy=P, d_logprob=P, d_entropy=P, top_ids=P, d_top=P, top_k=2, grad=P + 1024, grad_stride=4, stream=None)
+
+
+@pytest.mark.parametrize("change,code,word", [
+  (dict(dtype=9), -1, "dtype"), (dict(stride=3), -2, "stride"), (dict(grad_stride=3), -2, "gradient stride"),
+  (dict(d_logprob=None, d_entropy=None, d_top=None), -1, "no gradient"), (dict(labels=None), -1, "labels"),
+  (dict(entropy=None), -1, "entropy"), (dict(top_ids=None), -1, "top_ids"), (dict(top_k=0), -1, "top_ids"),
+  (dict(lse=None), -1, "NULL"), (dict(grad=None), -1, "NULL"), (dict(grad=P), -1, "overlaps"), (dict(grad=P + 28), -1, "overlaps"),
+  (dict(grad=P + 1025), -1, "misaligned"), (dict(rows=1 << 40), -2, "blocks"),
+])
+def test_label_logprobs_grad_refuses(change, code, word):
+  if "rows" in change:
+    change = dict(change, grad=P + (1 << 46))      # 2^40 rows of 16 bytes: do not overlap
+  _refused("pclseg_op_label_logprobs_grad", list({**GRAD, **change}.values()), code, word)
+
+
+def test_no_rows_is_no_work():
+  lib = E.load_library()
+  assert lib.pclseg_op_quantize_rows(*{**QUANT, "rows": 0, "x": None}.values()) == 0
+  assert lib.pclseg_op_matmul_i8(*{**MATMUL, "m": 0, "a": None, "y": None}.values()) == 0
+  assert lib.pclseg_op_linear_i8(*{**LINEAR, "m": 0, "x": None, "y": None, "workspace": None}.values()) == 0
+  assert lib.pclseg_op_label_logprobs(*{**SCORE, "rows": 0, "logits": None}.values()) == 0
+  assert lib.pclseg_op_label_logprobs_grad(*{**GRAD, "rows": 0, "logits": None}.values()) == 0
+
+
+def test_every_entry_point_is_behind_the_exception_barrier():
+  src = open(os.path.join(os.path.dirname(E.__file__), "csrc", "pclseg_ops.hip")).read()
+  body = src[src.index('extern "C" {'):src.index('}  // extern "C"')]
+  defs = re.findall(r"^int (pclseg_\w+)\([^;{]*\)( try)? \{$", body, re.M)
+  assert len(defs) == 7 and all(t for _, t in defs) and body.count("OP_CATCH") == 7
+
+
+# ---- the Python layer: with on_device answered as if host tensors were device tensors, every refusal comes before a launch
+
+@pytest.fixture
+def host_as_device(monkeypatch):
+  monkeypatch.setattr(E, "on_device", lambda x: True)
+
+
+def _rows8(n=3, k=8):
+  return ops.Int8Rows(torch.zeros((n, 64), dtype=torch.int8), torch.ones(n), k)
+
+
+def test_host_tensors_are_refused():
+  x = torch.zeros(2, 8)
+  for call in (lambda: ops.quantize_rows(x), lambda: ops.linear_i8(x, _rows8()), lambda: ops.label_logprobs(x),
+               lambda: ops.label_logprobs_grad(x, None, x[:, 0]), lambda: ops.Int8Rows.from_codes(x.to(torch.int8), x[:, 0])):
+    with pytest.raises(ValueError, match="on the device"):
+      call()
+
+
+def test_python_layer_refuses(host_as_device):
+  x, i = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int32)
+  v = torch.zeros(2)
+  bad = [
+    lambda: ops.quantize_rows(x.double()), lambda: ops.quantize_rows(torch.zeros(())), lambda: ops.quantize_rows(torch.zeros(2, 0)),
+    lambda: ops.Int8Rows.from_codes(x, v), lambda: ops.Int8Rows.from_codes(x.to(torch.int8), torch.zeros(3)),
+    lambda: ops.Int8Rows.from_kernel(torch.zeros(3, 3, 8, 4)),
+    lambda: ops.linear_i8(x, _rows8(k=9)), lambda: ops.linear_i8(x, x), lambda: ops.linear_i8(x, _rows8(), act="tanh"),
+    lambda: ops.linear_i8(x, _rows8(), bias=torch.zeros(4)), lambda: ops.linear_i8(x, _rows8(), bias=torch.zeros(3).half()),
+    lambda: ops.linear_i8(x, _rows8(), residual=torch.zeros(2, 4)), lambda: ops.linear_i8(x, _rows8(), residual=torch.zeros(2, 3).half()),
+    lambda: ops.linear_i8(x, _rows8(), out_dtype=torch.float64), lambda: ops.matmul_i8(_rows8(), _rows8(k=9)),
+    lambda: ops.matmul_i8(x, _rows8()),
+    lambda: ops.label_logprobs(x.long()), lambda: ops.label_logprobs(torch.zeros(2, 0)), lambda: ops.label_logprobs(x, i[:1]),
+    lambda: ops.label_logprobs(x, i.float()), lambda: ops.label_logprobs(x, i, top_k=65),
+    lambda: ops.label_logprobs(x, i, top_k=-1), lambda: ops.label_logprobs(x, allowed=torch.ones(7, dtype=torch.bool)),
+    lambda: ops.label_logprobs(x, allowed=torch.ones(8)), lambda: ops.label_logprobs_grad(x, i, v),
+    lambda: ops.label_logprobs_grad(x, None, v, d_logprob=v), lambda: ops.label_logprobs_grad(x, i, v, d_entropy=v),
+    lambda: ops.label_logprobs_grad(x, i, v, d_top=v), lambda: ops.label_logprobs_grad(x, i, v[:1], d_logprob=v),
+    lambda: ops.label_logprobs_grad(x, i, v, d_logprob=v.double()),
+    lambda: ops.label_logprobs_grad(x, i, v, d_top=torch.zeros(2, 3), top_ids=torch.zeros((2, 2), dtype=torch.int32)),
+    lambda: ops.label_logprobs_grad(x, i, v, d_top=torch.zeros(2, 2), top_ids=torch.zeros((2, 2), dtype=torch.int64)),
+  ]
+  for n, call in enumerate(bad):
+    with pytest.raises(ValueError):
+      call()
+      pytest.fail("call %d was accepted" % n)
