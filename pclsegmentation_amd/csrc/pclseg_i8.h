@@ -161,13 +161,14 @@ struct I8Args {
   int64_t ldy;
 };
 
+__device__ __forceinline__ float relu(float v) { return v > 0.f ? v : (v != v ? v : 0.f); }
+__device__ __forceinline__ float leaky(float v) { return v > 0.f ? v : 0.1f * v; }
+// v_exp_f32 and v_rcp_f32, one unit in the last place each: within 4 * 2^-24 of the sigmoid, whose slope is 1/4
+__device__ __forceinline__ float sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
+}
 __device__ __forceinline__ float activate(float v, int act) {
-  switch (act) {
-    case ACT_RELU: return v > 0.f ? v : (v != v ? v : 0.f);
-    case ACT_LEAKY: return v > 0.f ? v : 0.1f * v;
-    case ACT_SIGMOID: return 1.f / (1.f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
-    default: return v;
-  }
+  return act == ACT_RELU ? relu(v) : act == ACT_LEAKY ? leaky(v) : act == ACT_SIGMOID ? sigmoid(v) : v;
 }
 
 template <typename T>
@@ -246,30 +247,96 @@ __device__ __forceinline__ int lds_chunk(int row, int chunk) {
   return row * BK + ((chunk ^ (row * C / 8)) & (C - 1)) * 16;
 }
 
+// Where a thread's 16-byte pieces of a tile of ROWS rows come from: offsets from the tile's first byte, fixed for all steps.
 template <int ROWS, int BK, int THREADS>
-__device__ __forceinline__ void stage_tile(const int8_t* src, int64_t ld, int64_t row0, int64_t rows, int k0, int8_t* lds) {
-  constexpr int C = BK / 16, N = ROWS * C;
-  static_assert(N % THREADS == 0, "whole waves");
-  const int wave0 = (threadIdx.x & ~63);
+struct TileSource {
+  static constexpr int C = BK / 16, N = ROWS * C / THREADS;
+  static_assert(ROWS * C % THREADS == 0, "whole waves");
+  const int8_t* base;      // uniform
+  uint32_t off[N];
+  __device__ __forceinline__ TileSource(const int8_t* src, int64_t ld, int64_t row0, int64_t rows) : base(src + row0 * ld) {
 #pragma unroll
-  for (int i = 0; i < N / THREADS; ++i) {
-    const int pos = i * THREADS + threadIdx.x;
-    const int r = pos / C, ch = (pos ^ (r * C / 8)) & (C - 1);
-    const int64_t row = row0 + r < rows ? row0 + r : rows - 1;       // rows behind the last repeat it
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + row * ld + k0 + ch * 16),
-                                     (__attribute__((address_space(3))) void*)(lds + (i * THREADS + wave0) * 16), 16, 0, 0);
+    for (int i = 0; i < N; ++i) {
+      const int pos = i * THREADS + threadIdx.x;
+      const int r = pos / C, ch = (pos ^ (r * C / 8)) & (C - 1);
+      const int rr = row0 + r < rows ? r : (int)(rows - 1 - row0);       // rows behind the last repeat it
+      off[i] = (uint32_t)rr * (uint32_t)ld + ch * 16;
+    }
+  }
+  __device__ __forceinline__ void stage(int64_t k0, int8_t* lds, int wave) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + k0 + off[i]),
+                                       (__attribute__((address_space(3))) void*)(lds + (i * THREADS + wave * 64) * 16), 16, 0, 0);
+  }
+};
+
+// four neighbouring outputs of a row
+template <typename T> struct Quad;
+template <> struct Quad<float> {
+  static __device__ __forceinline__ void load(const float* p, float* f) {
+    const u32x4 v = load16(p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[e]);
+  }
+  static __device__ __forceinline__ void store(float* p, const float* f) { store16(p, pack16<float>(f)); }
+};
+struct __attribute__((packed, aligned(2))) Pack8a2 { u32x2 v; };
+template <typename T> struct Quad16 {
+  static __device__ __forceinline__ void load(const T* p, float* f) {
+    const u32x2 v = reinterpret_cast<const Pack8a2*>(p)->v;
+    const u32x4 w{v[0], v[1], 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = Elem<T>::get(w, e);
+  }
+  static __device__ __forceinline__ void store(T* p, const float* f) {
+    typedef T T2 __attribute__((ext_vector_type(2)));
+    typedef float F2 __attribute__((ext_vector_type(2)));
+    u32x2 v;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) v[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(F2{f[2 * e], f[2 * e + 1]}, T2));
+    reinterpret_cast<Pack8a2*>(p)->v = v;
+  }
+};
+template <> struct Quad<__bf16> : Quad16<__bf16> {};
+template <> struct Quad<_Float16> : Quad16<_Float16> {};
+
+// act is uniform: one scalar branch for four values
+__device__ __forceinline__ void activate4(float* v, int act) {
+  if (act == ACT_RELU) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = relu(v[e]);
+  } else if (act == ACT_LEAKY) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = leaky(v[e]);
+  } else if (act == ACT_SIGMOID) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = sigmoid(v[e]);
   }
 }
 
+// The loop: a step's fragments are read from LDS one 32-byte slice of k ahead of the matrix instructions that use them, and
+// the barrier that hands a buffer over lies before the step's last slice, whose fragments are already in registers: the first
+// reads of the next tile run under those matrix instructions.
+// The epilogue goes through LDS, 32 rows of a wave at a time in a slab of its own: the accumulators hold one column a lane,
+// memory wants whole 128-byte lines of a row.
 template <typename T, int BM, int BN, int BK, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void i8_tiles(I8Args p, unsigned tiles_n) {
+__global__ __launch_bounds__(WM * WN * 64) void i8_tiles(I8Args p, unsigned tiles_m, unsigned tiles_n) {
   constexpr int THREADS = WM * WN * 64;
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32;      // 32x32 tiles of a wave
-  __shared__ __attribute__((aligned(128))) int8_t lds[2][(BM + BN) * BK];
+  constexpr int KK = BK / 32, TILE = (BM + BN) * BK;
+  static_assert(KK % 2 == 0, "slices alternate between two sets of registers");
+  constexpr int SW = TN * 32, SLD = SW + 8;                // slab: 32 rows of SW floats; + 8: a lane's two row groups differ by 32 banks
+  constexpr int SLABS = WM * WN * 32 * SLD * 4;
+  __shared__ __attribute__((aligned(128))) int8_t lds[2 * TILE > SLABS ? 2 * TILE : SLABS];
+  // an XCD works on neighbouring tiles, taken from groups of 4 tile rows column by column: 32 blocks of an XCD share 4 tiles
+  // of a and 8 of b
   const unsigned id = xcd_contiguous(blockIdx.x, gridDim.x);
-  const int64_t m0 = (int64_t)(id / tiles_n) * BM;
-  const int n0 = (int)(id % tiles_n) * BN;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned group = id / (4 * tiles_n), in_group = id - group * 4 * tiles_n;
+  const unsigned gm = tiles_m - group * 4 < 4 ? tiles_m - group * 4 : 4;
+  const int64_t m0 = (int64_t)(group * 4 + in_group % gm) * BM;
+  const int n0 = (int)(in_group / gm) * BN;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
   i32x16 acc[TM][TN];
 #pragma unroll
@@ -279,41 +346,113 @@ __global__ __launch_bounds__(WM * WN * 64) void i8_tiles(I8Args p, unsigned tile
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
   const int steps = p.kp / BK;
-  stage_tile<BM, BK, THREADS>(p.a, p.lda, m0, p.m, 0, lds[0]);
-  stage_tile<BN, BK, THREADS>(p.b, p.ldb, n0, p.n, 0, lds[0] + BM * BK);
-  for (int s = 0; s < steps; ++s) {
-    __syncthreads();      // this step's tile has landed (vmcnt 0), the other buffer is read no more
-    if (s + 1 < steps) {
-      stage_tile<BM, BK, THREADS>(p.a, p.lda, m0, p.m, (s + 1) * BK, lds[(s + 1) & 1]);
-      stage_tile<BN, BK, THREADS>(p.b, p.ldb, n0, p.n, (s + 1) * BK, lds[(s + 1) & 1] + BM * BK);
-    }
-    const int8_t* la = lds[s & 1];
+  const TileSource<BM, BK, THREADS> sa(p.a, p.lda, m0, p.m);
+  const TileSource<BN, BK, THREADS> sb(p.b, p.ldb, n0, p.n);
+  i32x4 fa[2][TM], fb[2][TN];
+  auto fragments = [&](int buf, int kk, int slot) {
+    const int8_t* la = lds + buf * TILE;
     const int8_t* lb = la + BM * BK;
+    const int ch = kk * 2 + (lane >> 5), r = lane & 31;
 #pragma unroll
-    for (int kk = 0; kk < BK / 32; ++kk) {
-      i32x4 fa[TM], fb[TN];
-      const int ch = kk * 2 + (lane >> 5), r = lane & 31;
+    for (int i = 0; i < TM; ++i) fa[slot][i] = *reinterpret_cast<const i32x4*>(la + lds_chunk<BK>(wm + i * 32 + r, ch));
 #pragma unroll
-      for (int i = 0; i < TM; ++i) fa[i] = *reinterpret_cast<const i32x4*>(la + lds_chunk<BK>(wm + i * 32 + r, ch));
+    for (int j = 0; j < TN; ++j) fb[slot][j] = *reinterpret_cast<const i32x4*>(lb + lds_chunk<BK>(wn + j * 32 + r, ch));
+  };
+  auto multiply = [&](int slot) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) fb[j] = *reinterpret_cast<const i32x4*>(lb + lds_chunk<BK>(wn + j * 32 + r, ch));
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int i = 0; i < TM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[slot][i], fb[slot][j], acc[i][j], 0, 0, 0);
+  };
+  auto interleave = [&]() {      // the slice's LDS reads spread over its matrix instructions, and nothing moved out of the slice
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
+    for (int i = 0; i < TM * TN; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      constexpr int each = (TM + TN + TM * TN - 1) / (TM * TN);
+      if (i * each < TM + TN) __builtin_amdgcn_sched_group_barrier(0x100, each, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  sa.stage(0, lds, wave);
+  sb.stage(0, lds + BM * BK, wave);
+  __syncthreads();
+  if (steps > 1) {
+    sa.stage(BK, lds + TILE, wave);
+    sb.stage(BK, lds + TILE + BM * BK, wave);
+  }
+  fragments(0, 0, 0);
+  for (int s = 0; s + 1 < steps; ++s) {
+#pragma unroll
+    for (int kk = 0; kk + 1 < KK; ++kk) {
+      fragments(s & 1, kk + 1, (kk + 1) & 1);
+      multiply(kk & 1);
+      interleave();
+    }
+    __syncthreads();      // the next tile has landed, this one is read no more
+    if (s + 2 < steps) {
+      sa.stage((int64_t)(s + 2) * BK, lds + (s & 1) * TILE, wave);
+      sb.stage((int64_t)(s + 2) * BK, lds + (s & 1) * TILE + BM * BK, wave);
+    }
+    fragments((s + 1) & 1, 0, 0);
+    multiply((KK - 1) & 1);
+    interleave();
   }
 #pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int col = n0 + wn + j * 32 + (lane & 31);
-    if (col >= p.n) continue;
-    const float sb = p.sb[col], bias = p.bias ? p.bias[col] : 0.f;
+  for (int kk = 0; kk < KK; ++kk) {
+    if (kk + 1 < KK) fragments((steps - 1) & 1, kk + 1, (kk + 1) & 1);
+    multiply(kk & 1);
+  }
+  __syncthreads();      // the tiles are read no more: the waves' slabs take their place
+  float* slab = reinterpret_cast<float*>(lds) + wave * 32 * SLD;
+  constexpr int QR = SW / 4, RP = 64 / QR;       // lanes a row, rows a pass
+  const int qc = (lane % QR) * 4, qr = lane / QR;
+  const int col = n0 + wn + qc;
+  float scale[4], bias[4];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
+  for (int e = 0; e < 4; ++e) {
+    scale[e] = col + e < p.n ? p.sb[col + e] : 0.f;
+    bias[e] = p.bias && col + e < p.n ? p.bias[col + e] : 0.f;
+  }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t row = m0 + wm + i * 32 + (e >> 2) * 8 + (lane >> 5) * 4 + (e & 3);
-        if (row < p.m) i8_store<T>(p, row, col, acc[i][j][e], p.sa[row], sb, bias);
+  for (int i = 0; i < TM; ++i) {
+    wave_lds_fence();
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        slab[((e >> 2) * 8 + (lane >> 5) * 4 + (e & 3)) * SLD + j * 32 + (lane & 31)] = (float)acc[i][j][e];
+    wave_lds_fence();
+#pragma unroll 4
+    for (int r = qr; r < 32; r += RP) {
+      const int64_t row = m0 + wm + i * 32 + r;
+      if (row >= p.m || col >= p.n) continue;
+      const u32x4 w = *reinterpret_cast<const u32x4*>(slab + r * SLD + qc);
+      const float s = p.sa[row];
+      float v[4], res[4];
+      const bool whole = col + 4 <= p.n;
+      const T* rp = static_cast<const T*>(p.residual) + row * p.ldr + col;
+      T* yp = static_cast<T*>(p.y) + row * p.ldy + col;
+      if (p.residual) {
+        if (whole) {
+          Quad<T>::load(rp, res);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) res[e] = col + e < p.n ? Elem<T>::load(rp + e) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(__uint_as_float(w[e]) * s, scale[e], bias[e]);
+      activate4(v, p.act);
+      if (p.residual) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += res[e];
+      }
+      if (whole) {
+        Quad<T>::store(yp, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < p.n) yp[e] = Elem<T>::from(v[e]);
       }
     }
   }

@@ -63,7 +63,7 @@ int quantize(const char* op, const void* x, int dtype, int64_t rows, int64_t col
 template <typename T, int BM, int BN, int BK, int WM, int WN>
 void launch_tiles(const I8Args& p, hipStream_t s) {
   const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
-  i8_tiles<T, BM, BN, BK, WM, WN><<<dim3((unsigned)(tm * tn)), dim3(WM * WN * 64), 0, s>>>(p, (unsigned)tn);
+  i8_tiles<T, BM, BN, BK, WM, WN><<<dim3((unsigned)(tm * tn)), dim3(WM * WN * 64), 0, s>>>(p, (unsigned)tm, (unsigned)tn);
 }
 
 int matmul(const char* op, const I8Args& p, int dtype, hipStream_t s) {
