@@ -27,9 +27,33 @@ struct QuantArgs {
   float* scale;
 };
 
-// A row's code needs round(x / s) to be the nearest integer of the exact quotient: x * (1/s) is within two roundings of it,
-// so rint() of that is the nearest integer or its neighbour, and the remainder x - q s — exact in one fma, |q| <= 128 —
-// says which.  Rows below 2^-60 are scaled by 2^64 first, so that s and 1/s stay normal numbers.
+// The largest magnitude of a row is taken on the bits: without the sign they order like unsigned integers, infinities and
+// NaN above everything finite, and 16-bit elements go two to an instruction.
+template <typename T> struct RowMax {
+  typedef uint16_t U2 __attribute__((ext_vector_type(2)));
+  U2 m{0, 0};
+  static constexpr uint32_t kInf = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+  __device__ __forceinline__ void add(const u32x4& v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(U2, v[e] & 0x7fff7fffu));
+  }
+  __device__ __forceinline__ uint32_t bits() const { return m[0] > m[1] ? m[0] : m[1]; }
+  static __device__ __forceinline__ float value(uint32_t b) {
+    return Elem<T>::get(u32x4{b, 0u, 0u, 0u}, 0);
+  }
+};
+template <> struct RowMax<float> {
+  uint32_t m = 0;
+  static constexpr uint32_t kInf = 0x7f800000u;
+  __device__ __forceinline__ void add(const u32x4& v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = max(m, v[e] & 0x7fffffffu);
+  }
+  __device__ __forceinline__ uint32_t bits() const { return m; }
+  static __device__ __forceinline__ float value(uint32_t b) { return __uint_as_float(b); }
+};
+
+// Rows below 2^-60 are scaled by 2^64 (pre), so that s and 1 / s stay normal numbers.
 struct RowScale { float pre, s, inv, half; };
 __device__ __forceinline__ RowScale row_scale(float amax) {
   RowScale r;
@@ -39,108 +63,122 @@ __device__ __forceinline__ RowScale row_scale(float amax) {
   r.half = 0.5f * r.s;
   return r;
 }
-__device__ __forceinline__ int quant(float x, const RowScale& r) {
-  const float v = x * r.pre;
-  float q = rintf(v * r.inv);
-  const float t = fmaf(-q, r.s, v), m = fabsf(t);
-  const bool odd = ((int)q & 1) != 0;
-  if (m > r.half || (m == r.half && odd)) q += t > 0.f ? 1.f : -1.f;
-  return (int)fminf(fmaxf(q, -127.f), 127.f);
+constexpr float kRound = 12582912.f;      // 1.5 * 2^23: x + kRound rounds x to an integer, whose code is the sum's low byte
+// The code of x has to be the integer nearest to the exact quotient x / s.  u = x * (1/s) + kRound, one fma, holds the nearest
+// integer or, within 2^-17 of a half step, its neighbour; the remainder t = x - q s, exact in one fma, says which: below half
+// a step the code stands, otherwise (rare: some lane of the wave, in one of 2^17 elements) `nearest` decides.
+__device__ __forceinline__ float quant(float x, const RowScale& r, float& worst) {
+  const float u = fmaf(x, r.inv, kRound), t = fmaf(-(u - kRound), r.s, x);
+  worst = fmaxf(worst, fabsf(t));
+  return u;
 }
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-  return (uint32_t)(a & 0xff) | ((uint32_t)(b & 0xff) << 8) | ((uint32_t)(c & 0xff) << 16) | ((uint32_t)(d & 0xff) << 24);
+__device__ __forceinline__ float nearest(float x, const RowScale& r) {
+  const float u = fmaf(x, r.inv, kRound), q = u - kRound, t = fmaf(-q, r.s, x), m = fabsf(t);
+  const bool odd = __float_as_uint(u) & 1;
+  return m > r.half || (m == r.half && odd) ? u + (t > 0.f ? 1.f : -1.f) : u;
+}
+__device__ __forceinline__ uint32_t pack4(const float* u) {
+  const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(u[1]), __float_as_uint(u[0]), 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(u[3]), __float_as_uint(u[2]), 0x04000c0cu);
+  return lo | hi;
 }
 
-// elements [c, c + 8) of a row, 0 behind its end
-template <typename T> __device__ __forceinline__ void load8_zero(const T* row, int c, int cols, float* f) {
-  constexpr int VEC = Elem<T>::VEC;
-  if (c + 8 <= cols) {
+// eight elements of a row: 16 bytes, or 32 of floats
+template <typename T> struct Eight {
+  static constexpr int N = 8 / Elem<T>::VEC;
+  u32x4 v[N];
+  __device__ __forceinline__ void load(const T* row, int c, int cols) {      // 0 behind the row's end
+    if (c + 8 <= cols) {
 #pragma unroll
-    for (int h = 0; h < 8 / VEC; ++h) {
-      const u32x4 v = load16(row + c + h * VEC);
+      for (int h = 0; h < N; ++h) v[h] = load16(row + c + h * Elem<T>::VEC);
+    } else {
+      float f[8];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) f[h * VEC + e] = Elem<T>::get(v, e);
+      for (int e = 0; e < 8; ++e) f[e] = c + e < cols ? Elem<T>::load(row + c + e) : 0.f;
+#pragma unroll
+      for (int h = 0; h < N; ++h) v[h] = pack16<T>(f + h * Elem<T>::VEC);
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = c + e < cols ? Elem<T>::load(row + c + e) : 0.f;
   }
-}
-__device__ __forceinline__ float amax8(const float* f, float a) {
-  // NaN has to survive the maximum: a row with a NaN or an infinity has no scale
+  __device__ __forceinline__ void add_to(RowMax<T>& m) const {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) a = (fabsf(f[e]) > a || f[e] != f[e]) ? fabsf(f[e]) : a;
-  return a;
-}
-__device__ __forceinline__ u32x2 quant8(const float* f, const RowScale& r, bool finite) {
-  int q[8];
+    for (int h = 0; h < N; ++h) m.add(v[h]);
+  }
+  __device__ __forceinline__ u32x2 codes(const RowScale& r) const {
+    float x[8], u[8], worst = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) q[e] = finite ? quant(f[e], r) : 0;
-  return u32x2{pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7])};
-}
+    for (int e = 0; e < 8; ++e) x[e] = Elem<T>::get(v[e / Elem<T>::VEC], e % Elem<T>::VEC);
+    if (r.pre != 1.f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= r.pre;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = quant(x[e], r, worst);
+    if (worst >= r.half) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e] = nearest(x[e], r);
+    }
+    return u32x2{pack4(u), pack4(u + 4)};
+  }
+};
 
-// G lanes own a row, each 8 elements of every stretch of 8 G; NV stretches are kept in registers, so a row of up to
-// 8 G NV elements is read once.  Longer rows (REREAD) are read twice, the second time from the L2.  A row with an
-// infinity or a NaN gets the scale NaN and codes 0: its outputs are NaN, like those of a float32 product.
+// G lanes own a row, each 8 elements of every stretch of 8 G; four stretches are kept in registers, so a row of up to 32 G
+// elements is read once.  Longer rows (REREAD) are read twice, the second time from the L2.  A row with an infinity or a
+// NaN gets the scale NaN and codes 0: its outputs are NaN, like those of a float32 product.
 template <typename T, int G, bool REREAD>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
   constexpr int NV = 4;
-  __shared__ float red[4];
+  __shared__ uint32_t red[4];
   const int g = threadIdx.x % G;
   const int64_t row0 = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
   const bool live = row0 < a.rows;
   const int64_t row = live ? row0 : a.rows - 1;
   const T* src = static_cast<const T*>(a.x) + row * a.stride;
   const int nv = (a.cols + 8 * G - 1) / (8 * G);
-  float f[NV][8], amax = 0.f;
+  Eight<T> x[NV];
+  RowMax<T> mx;
 #pragma unroll
   for (int v = 0; v < NV; ++v)
-    if (v < nv) load8_zero(src, (v * G + g) * 8, a.cols, f[v]);
+    if (v < nv) x[v].load(src, (v * G + g) * 8, a.cols);
 #pragma unroll
   for (int v = 0; v < NV; ++v)
-    if (v < nv) amax = amax8(f[v], amax);
+    if (v < nv) x[v].add_to(mx);
   if constexpr (REREAD) {
     for (int v = NV; v < nv; ++v) {
-      float t[8];
-      load8_zero(src, (v * G + g) * 8, a.cols, t);
-      amax = amax8(t, amax);
+      Eight<T> t;
+      t.load(src, (v * G + g) * 8, a.cols);
+      t.add_to(mx);
     }
   }
+  uint32_t top = mx.bits();
 #pragma unroll
-  for (int d = 1; d < (G < 64 ? G : 64); d <<= 1) {
-    const float o = __shfl_xor(amax, d);
-    amax = (o > amax || o != o) ? o : amax;
-  }
+  for (int d = 1; d < (G < 64 ? G : 64); d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
   if constexpr (G == 256) {
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = amax;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 4; ++w) amax = (red[w] > amax || red[w] != red[w]) ? red[w] : amax;
+    top = max(max(red[0], red[1]), max(red[2], red[3]));
   }
-  const bool finite = amax < __builtin_inff();      // false for NaN too
-  const RowScale r = row_scale(finite ? amax : 0.f);
+  const bool finite = top < RowMax<T>::kInf;
+  const RowScale r = row_scale(finite ? RowMax<T>::value(top) : 0.f);
   if (!live) return;
   if (g == 0) a.scale[row] = finite ? r.s / r.pre : __builtin_nanf("");
+  const bool zero = r.inv == 0.f;      // nothing but zeros, or no scale
   int8_t* dst = a.q + row * a.ld;
   const int nq = (int)((a.ld + 8 * G - 1) / (8 * G));      // the zeros behind the row too
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int c = (v * G + g) * 8;
-    if (v < nv) {
-      if (c < a.ld) *reinterpret_cast<u32x2*>(dst + c) = quant8(f[v], r, finite);
-    }
+    if (v < nv && c < a.ld) *reinterpret_cast<u32x2*>(dst + c) = zero ? u32x2{0u, 0u} : x[v].codes(r);
   }
   for (int v = nv < NV ? nv : NV; v < nq; ++v) {
     const int c = (v * G + g) * 8;
     if (c >= a.ld) break;
-    float t[8];
-    if (REREAD && c < a.cols) {
-      load8_zero(src, c, a.cols, t);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) t[e] = 0.f;
+    u32x2 w{0u, 0u};
+    if (REREAD && c < a.cols && !zero) {
+      Eight<T> t;
+      t.load(src, c, a.cols);
+      w = t.codes(r);
     }
-    *reinterpret_cast<u32x2*>(dst + c) = quant8(t, r, finite);
+    *reinterpret_cast<u32x2*>(dst + c) = w;
   }
 }
 
@@ -239,13 +277,14 @@ __global__ __launch_bounds__(NW * 64) void i8_few_rows(I8Args p) {
 // ---- tiles
 // BM x BN outputs a block, BK bytes of k a step, WM x WN waves.  Both operands go straight from memory into LDS (16 bytes a
 // lane, no registers between), two buffers: the next step's tile is in flight while this one is multiplied.  A row of a tile
-// is BK bytes; its 16-byte chunks are permuted by the row number, so that the 8 lanes an LDS read serves at once, one chunk
-// of 8 neighbouring rows, lie in different banks.  The permutation is made on the global side: LDS is written linearly.
+// is BK bytes; its 16-byte chunks are permuted by the row number, so that the 16 lanes an LDS read serves at once, the same
+// chunk of 16 rows, lie in 16 different places of the 64 banks (256 bytes hold 256 / BK rows, hence the shift; with rows
+// permuted by row % 8, counters showed every second cycle of the LDS lost to conflicts).  The permutation is made on the
+// global side: LDS is written linearly.
 template <int BK>
-__device__ __forceinline__ int lds_chunk(int row, int chunk) {
-  constexpr int C = BK / 16;
-  return row * BK + ((chunk ^ (row * C / 8)) & (C - 1)) * 16;
-}
+__device__ __forceinline__ int swizzle(int row) { return (row * BK / 256) & (BK / 16 - 1); }
+template <int BK>
+__device__ __forceinline__ int lds_chunk(int row, int chunk) { return row * BK + (chunk ^ swizzle<BK>(row)) * 16; }
 
 // Where a thread's 16-byte pieces of a tile of ROWS rows come from: offsets from the tile's first byte, fixed for all steps.
 template <int ROWS, int BK, int THREADS>
@@ -258,7 +297,7 @@ struct TileSource {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int pos = i * THREADS + threadIdx.x;
-      const int r = pos / C, ch = (pos ^ (r * C / 8)) & (C - 1);
+      const int r = pos / C, ch = (pos % C) ^ swizzle<BK>(r);
       const int rr = row0 + r < rows ? r : (int)(rows - 1 - row0);       // rows behind the last repeat it
       off[i] = (uint32_t)rr * (uint32_t)ld + ch * 16;
     }
@@ -301,32 +340,34 @@ template <typename T> struct Quad16 {
 template <> struct Quad<__bf16> : Quad16<__bf16> {};
 template <> struct Quad<_Float16> : Quad16<_Float16> {};
 
-// act is uniform: one scalar branch for four values
-__device__ __forceinline__ void activate4(float* v, int act) {
+// act is uniform: one scalar branch for all values
+template <int N> __device__ __forceinline__ void activate_all(float* v, int act) {
   if (act == ACT_RELU) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = relu(v[e]);
+    for (int e = 0; e < N; ++e) v[e] = relu(v[e]);
   } else if (act == ACT_LEAKY) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = leaky(v[e]);
+    for (int e = 0; e < N; ++e) v[e] = leaky(v[e]);
   } else if (act == ACT_SIGMOID) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = sigmoid(v[e]);
+    for (int e = 0; e < N; ++e) v[e] = sigmoid(v[e]);
   }
 }
 
 // The loop: a step's fragments are read from LDS one 32-byte slice of k ahead of the matrix instructions that use them, and
 // the barrier that hands a buffer over lies before the step's last slice, whose fragments are already in registers: the first
 // reads of the next tile run under those matrix instructions.
-// The epilogue goes through LDS, 32 rows of a wave at a time in a slab of its own: the accumulators hold one column a lane,
-// memory wants whole 128-byte lines of a row.
-template <typename T, int BM, int BN, int BK, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void i8_tiles(I8Args p, unsigned tiles_m, unsigned tiles_n) {
+// The epilogue goes through LDS, 32 rows of a wave at a time in a slab of its own: the weights are the matrix instruction's
+// first operand, so a lane's accumulators are four neighbouring channels of one row, and memory wants whole 128-byte lines
+// of a row.  Tiles inside the output take a path without a test; loads (scales, residual) are in flight before the slab is
+// written.  (With one tested, branching store after the other the epilogue alone took 155 us of 134 M outputs.)
+template <typename T, int BM, int BN, int BK, int WM, int WN, int OCC>
+__global__ __launch_bounds__(WM * WN * 64, OCC) void i8_tiles(I8Args p, unsigned tiles_m, unsigned tiles_n) {
   constexpr int THREADS = WM * WN * 64;
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32;      // 32x32 tiles of a wave
   constexpr int KK = BK / 32, TILE = (BM + BN) * BK;
   static_assert(KK % 2 == 0, "slices alternate between two sets of registers");
-  constexpr int SW = TN * 32, SLD = SW + 8;                // slab: 32 rows of SW floats; + 8: a lane's two row groups differ by 32 banks
+  constexpr int SW = TN * 32, SLD = SW + 4;                // slab: 32 rows of SW floats; + 4: 16 rows' quads fill 64 banks
   constexpr int SLABS = WM * WN * 32 * SLD * 4;
   __shared__ __attribute__((aligned(128))) int8_t lds[2 * TILE > SLABS ? 2 * TILE : SLABS];
   // an XCD works on neighbouring tiles, taken from groups of 4 tile rows column by column: 32 blocks of an XCD share 4 tiles
@@ -362,7 +403,7 @@ __global__ __launch_bounds__(WM * WN * 64) void i8_tiles(I8Args p, unsigned tile
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int i = 0; i < TM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[slot][i], fb[slot][j], acc[i][j], 0, 0, 0);
+      for (int i = 0; i < TM; ++i) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[slot][j], fa[slot][i], acc[i][j], 0, 0, 0);
   };
   auto interleave = [&]() {      // the slice's LDS reads spread over its matrix instructions, and nothing moved out of the slice
 #pragma unroll
@@ -404,7 +445,7 @@ __global__ __launch_bounds__(WM * WN * 64) void i8_tiles(I8Args p, unsigned tile
   }
   __syncthreads();      // the tiles are read no more: the waves' slabs take their place
   float* slab = reinterpret_cast<float*>(lds) + wave * 32 * SLD;
-  constexpr int QR = SW / 4, RP = 64 / QR;       // lanes a row, rows a pass
+  constexpr int QR = SW / 4, RP = 64 / QR, NR = 32 / RP;       // lanes a row, rows a pass, passes
   const int qc = (lane % QR) * 4, qr = lane / QR;
   const int col = n0 + wn + qc;
   float scale[4], bias[4];
@@ -413,46 +454,72 @@ __global__ __launch_bounds__(WM * WN * 64) void i8_tiles(I8Args p, unsigned tile
     scale[e] = col + e < p.n ? p.sb[col + e] : 0.f;
     bias[e] = p.bias && col + e < p.n ? p.bias[col + e] : 0.f;
   }
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
+  auto to_slab = [&](int i) {
     wave_lds_fence();
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        slab[((e >> 2) * 8 + (lane >> 5) * 4 + (e & 3)) * SLD + j * 32 + (lane & 31)] = (float)acc[i][j][e];
+      for (int q = 0; q < 4; ++q) {
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = __float_as_uint((float)acc[i][j][q * 4 + e]);
+        *reinterpret_cast<u32x4*>(slab + (lane & 31) * SLD + j * 32 + q * 8 + (lane >> 5) * 4) = w;
+      }
     wave_lds_fence();
-#pragma unroll 4
+  };
+  if (m0 + BM <= p.m && n0 + BN <= p.n && p.ldy < (1 << 26) && p.ldr < (1 << 26)) {
+    // uniform row addresses plus a lane's 32-bit offset; four passes at a time bound the registers
+    const uint32_t yo = (uint32_t)(qr * (int)p.ldy + qc) * sizeof(T), ro = (uint32_t)(qr * (int)p.ldr + qc) * sizeof(T);
+    constexpr int HR = NR < 4 ? NR : 4;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      to_slab(i);
+#pragma unroll
+      for (int h = 0; h < NR; h += HR) {
+        const int64_t row0 = m0 + wm + i * 32 + h * RP;
+        const char* rb = static_cast<const char*>(p.residual) + (row0 * p.ldr + n0 + wn) * (int64_t)sizeof(T);
+        char* yb = static_cast<char*>(p.y) + (row0 * p.ldy + n0 + wn) * (int64_t)sizeof(T);
+        float s[HR], res[HR][4], v[HR][4];
+        if (p.residual) {
+#pragma unroll
+          for (int r = 0; r < HR; ++r)
+            Quad<T>::load(reinterpret_cast<const T*>(rb + r * RP * p.ldr * (int64_t)sizeof(T) + ro), res[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < HR; ++r) s[r] = (p.sa + row0 + r * RP)[qr];
+#pragma unroll
+        for (int r = 0; r < HR; ++r) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(slab + ((h + r) * RP + qr) * SLD + qc);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[r][e] = fmaf(__uint_as_float(w[e]) * s[r], scale[e], bias[e]);
+        }
+        activate_all<HR * 4>(&v[0][0], p.act);
+        if (p.residual) {
+#pragma unroll
+          for (int r = 0; r < HR; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[r][e] += res[r][e];
+        }
+#pragma unroll
+        for (int r = 0; r < HR; ++r) Quad<T>::store(reinterpret_cast<T*>(yb + r * RP * p.ldy * (int64_t)sizeof(T) + yo), v[r]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    to_slab(i);
     for (int r = qr; r < 32; r += RP) {
       const int64_t row = m0 + wm + i * 32 + r;
-      if (row >= p.m || col >= p.n) continue;
-      const u32x4 w = *reinterpret_cast<const u32x4*>(slab + r * SLD + qc);
+      if (row >= p.m) continue;
       const float s = p.sa[row];
-      float v[4], res[4];
-      const bool whole = col + 4 <= p.n;
-      const T* rp = static_cast<const T*>(p.residual) + row * p.ldr + col;
-      T* yp = static_cast<T*>(p.y) + row * p.ldy + col;
-      if (p.residual) {
-        if (whole) {
-          Quad<T>::load(rp, res);
-        } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) res[e] = col + e < p.n ? Elem<T>::load(rp + e) : 0.f;
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(__uint_as_float(w[e]) * s, scale[e], bias[e]);
-      activate4(v, p.act);
-      if (p.residual) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += res[e];
-      }
-      if (whole) {
-        Quad<T>::store(yp, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < p.n) yp[e] = Elem<T>::from(v[e]);
+      for (int e = 0; e < 4; ++e) {
+        if (col + e >= p.n) continue;
+        float v = activate(fmaf(slab[r * SLD + qc + e] * s, scale[e], bias[e]), p.act);
+        if (p.residual) v += Elem<T>::load(static_cast<const T*>(p.residual) + row * p.ldr + col + e);
+        static_cast<T*>(p.y)[row * p.ldy + col + e] = Elem<T>::from(v);
       }
     }
   }

@@ -60,10 +60,10 @@ int quantize(const char* op, const void* x, int dtype, int64_t rows, int64_t col
   return launched(op);
 }
 
-template <typename T, int BM, int BN, int BK, int WM, int WN>
+template <typename T, int BM, int BN, int BK, int WM, int WN, int OCC>
 void launch_tiles(const I8Args& p, hipStream_t s) {
   const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
-  i8_tiles<T, BM, BN, BK, WM, WN><<<dim3((unsigned)(tm * tn)), dim3(WM * WN * 64), 0, s>>>(p, (unsigned)tm, (unsigned)tn);
+  i8_tiles<T, BM, BN, BK, WM, WN, OCC><<<dim3((unsigned)(tm * tn)), dim3(WM * WN * 64), 0, s>>>(p, (unsigned)tm, (unsigned)tn);
 }
 
 int matmul(const char* op, const I8Args& p, int dtype, hipStream_t s) {
@@ -75,10 +75,12 @@ int matmul(const char* op, const I8Args& p, int dtype, hipStream_t s) {
     if (p.m <= 16) i8_few_rows<T, 1, 8><<<few, dim3(512), 0, s>>>(p);
     else if (p.m <= 32) i8_few_rows<T, 2, 8><<<few, dim3(512), 0, s>>>(p);
     else if (p.m <= 64) i8_few_rows<T, 4, 8><<<few, dim3(512), 0, s>>>(p);
-    else if (p.kp == 64) launch_tiles<T, 128, 128, 64, 2, 2>(p, s);
-    else if (tiles(256, 256) >= 192) launch_tiles<T, 256, 256, 128, 2, 4>(p, s);
-    else if (tiles(128, 128) >= 192) launch_tiles<T, 128, 128, 128, 2, 2>(p, s);
-    else launch_tiles<T, 64, 64, 128, 2, 2>(p, s);
+    // the largest tile that still gives most of the 256 CUs one: 8192x8192x4096 takes 297 us with 256x256 tiles, 299 with
+    // 128x128, 423 with 64x64; 8192x512x1024 18.8 / 10.5 / 11.5 us; 512x4096x4096 44 / 20.6 / 18.0 us
+    else if (p.kp == 64) launch_tiles<T, 128, 128, 64, 2, 2, 3>(p, s);
+    else if (tiles(256, 256) >= 192) launch_tiles<T, 256, 256, 128, 2, 4, 2>(p, s);
+    else if (tiles(128, 128) >= 192) launch_tiles<T, 128, 128, 128, 4, 2, 4>(p, s);
+    else launch_tiles<T, 64, 64, 128, 2, 2, 4>(p, s);
   });
   return launched(op);
 }
