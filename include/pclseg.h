@@ -361,9 +361,9 @@ int pclseg_op_matmul_i8(const int8_t* a, const float* a_scale, const int8_t* b, 
                         int64_t n, int64_t k, const float* bias, int act, const void* residual, int64_t residual_stride,
                         void* y, int64_t y_stride, int dtype, void* hip_stream);
 
-/* The layer on float rows: op_quantize_rows of x into the workspace, then op_matmul_i8.
+/* The layer on float rows: op_quantize_rows of x into the workspace, then op_matmul_i8 (a few rows: one launch, no workspace).
  *   x      [m, k] dtype; weight codes and scales as for b above
- *   workspace  pclseg_op_linear_i8_workspace bytes, 16-byte aligned; two calls in flight need two */
+ *   workspace  pclseg_op_linear_i8_workspace bytes (may be 0), 16-byte aligned; two calls in flight need two */
 int pclseg_op_linear_i8_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes);
 int pclseg_op_linear_i8(const void* x, int dtype, int64_t x_stride, const int8_t* weight, const float* weight_scale,
                         int64_t m, int64_t n, int64_t k, const float* bias, int act, const void* residual,

@@ -150,8 +150,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
     }
   }
   uint32_t top = mx.bits();
-#pragma unroll
-  for (int d = 1; d < (G < 64 ? G : 64); d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+  top = group_reduce<(G < 64 ? G : 64)>(top, [](uint32_t a, uint32_t b) { return max(a, b); });
   if constexpr (G == 256) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
     __syncthreads();
@@ -271,6 +270,83 @@ __global__ __launch_bounds__(NW * 64) void i8_few_rows(I8Args p) {
 #pragma unroll
     for (int w = 0; w < NW; ++w) v += part[w][o >> 8][o & 255];
     i8_store<T>(p, i, j, v, p.sa[i], p.sb[j], p.bias ? p.bias[j] : 0.f);
+  }
+}
+
+// ---- one to four rows: quantisation and product in one launch
+// Every block quantises all rows again (m k elements, 8 k of them a thread's share at k = 4096 and one row) while its first
+// weights are on their way; a launch of its own would cost more than the whole product.  Codes and scales of the rows stay
+// in LDS.
+constexpr int kFusedRows = 4, kFusedBytes = 49152;      // rows, and bytes of codes, a block takes
+template <typename T, typename Y, int NW>
+__global__ __launch_bounds__(NW * 64) void i8_fused_rows(I8Args p, const T* x, int64_t x_stride, int k) {
+  extern __shared__ __attribute__((aligned(16))) int8_t codes[];      // [m][kp]
+  __shared__ int part[NW][256];
+  __shared__ uint32_t tops[kFusedRows][NW];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, ko = (lane >> 4) * 16;
+  const int n0 = blockIdx.x * 16, m = (int)p.m;
+  const int jn = n0 + r < p.n ? n0 + r : p.n - 1;
+  const int steps = p.kp / 64, s0 = steps * wave / NW, s1 = steps * (wave + 1) / NW;      // a wave's stretch of k
+  const int8_t* wb = p.b + (int64_t)jn * p.ldb + ko;
+  constexpr int D = 8;
+  i32x4 w[D];
+#pragma unroll
+  for (int u = 0; u < D; ++u) w[u] = *reinterpret_cast<const i32x4*>(wb + (int64_t)(s0 + u < s1 ? s0 + u : steps - 1) * 64);
+  for (int i = 0; i < m; ++i) {
+    RowMax<T> mx;
+    for (int c = threadIdx.x * 8; c < k; c += NW * 512) {
+      Eight<T> e;
+      e.load(x + i * x_stride, c, k);
+      e.add_to(mx);
+    }
+    const uint32_t top = group_reduce<64>(mx.bits(), [](uint32_t a, uint32_t b) { return max(a, b); });
+    if (lane == 0) tops[i][wave] = top;
+  }
+  __syncthreads();
+  float sa[kFusedRows];
+#pragma unroll
+  for (int i = 0; i < kFusedRows; ++i) {
+    if (i >= m) break;
+    uint32_t top = 0;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) top = max(top, tops[i][v]);
+    const bool finite = top < RowMax<T>::kInf;
+    const RowScale q = row_scale(finite ? RowMax<T>::value(top) : 0.f);
+    sa[i] = finite ? q.s / q.pre : __builtin_nanf("");
+    for (int c = threadIdx.x * 8; c < p.kp; c += NW * 512) {
+      u32x2 o{0u, 0u};
+      if (c < k && q.inv != 0.f) {
+        Eight<T> e;
+        e.load(x + i * x_stride, c, k);
+        o = e.codes(q);
+      }
+      *reinterpret_cast<u32x2*>(codes + i * p.kp + c) = o;
+    }
+  }
+  __syncthreads();
+  i32x4 acc{0, 0, 0, 0};
+  const int8_t* xa = codes + (r < m ? r : 0) * p.kp + ko;      // rows behind m are not stored
+  for (int s = s0; s < s1; s += D) {
+#pragma unroll
+    for (int u = 0; u < D; ++u) {
+      if (s + u < s1) {
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const i32x4*>(xa + (s + u) * 64), w[u], acc, 0, 0, 0);
+        if (s + u + D < s1) w[u] = *reinterpret_cast<const i32x4*>(wb + (int64_t)(s + u + D) * 64);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) part[wave][((lane >> 4) * 4 + i) * 16 + r] = acc[i];
+  __syncthreads();
+  for (int o = threadIdx.x; o < m * 16; o += NW * 64) {
+    const int i = o / 16, j = n0 + (o & 15);
+    if (j >= p.n) continue;
+    int v = 0;
+#pragma unroll
+    for (int u = 0; u < NW; ++u) v += part[u][o];
+    const float s = i == 0 ? sa[0] : i == 1 ? sa[1] : i == 2 ? sa[2] : sa[3];
+    i8_store<Y>(p, i, j, v, s, p.sb[j], p.bias ? p.bias[j] : 0.f);
   }
 }
 

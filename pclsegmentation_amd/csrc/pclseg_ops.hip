@@ -85,6 +85,12 @@ int matmul(const char* op, const I8Args& p, int dtype, hipStream_t s) {
   return launched(op);
 }
 
+// one to four rows whose codes fit into a block's LDS: one launch, no workspace (see i8_fused_rows)
+bool fused_rows(int64_t m, int64_t k) { return m <= kFusedRows && m * row_bytes(k) <= kFusedBytes; }
+size_t linear_workspace(int64_t m, int64_t k) {
+  return fused_rows(m, k) ? 0 : (size_t)m * ((size_t)row_bytes(k) + sizeof(float));
+}
+
 int check_product(const char* op, int64_t m, int64_t n, int64_t k, const int8_t* b, const float* b_scale, int act,
                   const void* residual, int64_t residual_stride, const void* y, int64_t y_stride, int dtype) {
   if (!dtype_ok(dtype)) return bad(op, "unknown dtype");
@@ -99,7 +105,7 @@ int check_product(const char* op, int64_t m, int64_t n, int64_t k, const int8_t*
 }
 
 // ---------------------------------------------------------------------------------------------- log probabilities
-constexpr int kThreadRow = 32, kGroupRow = 2048, kPiece = 2048, kWaves = 4;
+constexpr int kThreadRow = 32, kGroupRow = 2048, kPiece = 2048, kWaves = 4, kRounds = 4;
 
 // pieces a long row is cut into so that few rows still fill the chip: a block streams kWaves pieces of 2048 elements at a
 // time, and 512 blocks hide the memory's latency
@@ -121,16 +127,20 @@ template <typename T> void launch_score(const ScoreArgs& a, hipStream_t s) {
     else if (v <= 16) logprob_thread_rows<T, 16><<<g, b, 0, s>>>(a);
     else if (v <= 24) logprob_thread_rows<T, 24><<<g, b, 0, s>>>(a);
     else logprob_thread_rows<T, 32><<<g, b, 0, s>>>(a);
-  } else if (v <= kGroupRow) {
+  } else if (v <= kGroupRow && !(v > 256 && a.top_k > kRounds)) {
     auto grid = [&](int g) { return dim3((unsigned)((a.rows + 256 / g - 1) / (256 / g))); };
     if (v <= 8 * 32) logprob_group_rows<T, 8><<<grid(8), dim3(256), 0, s>>>(a);
     else if (v <= 16 * 32) logprob_group_rows<T, 16><<<grid(16), dim3(256), 0, s>>>(a);
     else if (v <= 32 * 32) logprob_group_rows<T, 32><<<grid(32), dim3(256), 0, s>>>(a);
     else logprob_group_rows<T, 64><<<grid(64), dim3(256), 0, s>>>(a);
   } else {
-    const dim3 g((unsigned)(a.rows * a.segs)), b(kWaves * 64);
-    if (a.top_k) logprob_wave_rows<T, kWaves, true><<<g, b, 0, s>>>(a);
-    else logprob_wave_rows<T, kWaves, false><<<g, b, 0, s>>>(a);
+    const dim3 g((unsigned)(a.rows * a.segs));
+    if (v > kPiece) {
+      if (a.top_k) logprob_wave_rows<T, kWaves, true><<<g, dim3(kWaves * 64), 0, s>>>(a);
+      else logprob_wave_rows<T, kWaves, false><<<g, dim3(kWaves * 64), 0, s>>>(a);
+    } else {
+      logprob_wave_rows<T, 1, true><<<g, dim3(64), 0, s>>>(a);
+    }
     if (a.segs > 1) {
       if (a.top_k) logprob_join<T, true><<<dim3((unsigned)a.rows), dim3(256), 0, s>>>(a);
       else logprob_join<T, false><<<dim3((unsigned)a.rows), dim3(256), 0, s>>>(a);
@@ -189,7 +199,7 @@ int pclseg_op_linear_i8_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes
   const char* op = "op_linear_i8_workspace";
   if (!bytes) return bad(op, "bytes is NULL");
   if (m < 0 || m > kMaxBlocks || n < 1 || !row_bytes(k)) return bad_shape(op, "m must be in [0, 2^31), n positive, k in [1, 131071]");
-  *bytes = (size_t)m * ((size_t)row_bytes(k) + sizeof(float));
+  *bytes = linear_workspace(m, k);
   return PCLSEG_OK;
 } OP_CATCH
 
@@ -203,10 +213,22 @@ int pclseg_op_linear_i8(const void* x, int dtype, int64_t x_stride, const int8_t
   if (!dtype_ok(dtype)) return bad(op, "unknown dtype");
   if (m > kMaxBlocks || x_stride < k) return bad_shape(op, "m must be below 2^31, the row stride at least k");
   if (m == 0) return PCLSEG_OK;
-  if (!x || !workspace) return bad(op, "NULL buffer");
-  if (!aligned(x, dtype_size(dtype)) || !aligned(workspace, 16)) return bad(op, "misaligned x or workspace");
+  if (!x) return bad(op, "NULL buffer");
+  if (!aligned(x, dtype_size(dtype))) return bad(op, "misaligned x");
   const int64_t ld = row_bytes(k);
-  if (workspace_bytes < (size_t)m * ((size_t)ld + sizeof(float))) return bad(op, "workspace too small");
+  if (fused_rows(m, k)) {
+    I8Args p{nullptr, weight, nullptr, weight_scale, ld, ld, m, (int)n, (int)ld, bias, act, residual, residual_stride, y, y_stride};
+    with_type(dtype, [&](auto t) {
+      with_type(y_dtype, [&](auto u) {
+        typedef decltype(t) T;
+        i8_fused_rows<T, decltype(u), 8><<<dim3((unsigned)((n + 15) / 16)), dim3(512), (size_t)(m * ld), (hipStream_t)hip_stream>>>(
+            p, static_cast<const T*>(x), x_stride, (int)k);
+      });
+    });
+    return launched(op);
+  }
+  if (!workspace || workspace_bytes < linear_workspace(m, k)) return bad(op, "workspace too small");
+  if (!aligned(workspace, 16)) return bad(op, "misaligned workspace");
   int8_t* q = static_cast<int8_t*>(workspace);
   float* scale = reinterpret_cast<float*>(q + m * ld);
   const int rq = quantize(op, x, dtype, m, k, x_stride, q, scale, (hipStream_t)hip_stream);

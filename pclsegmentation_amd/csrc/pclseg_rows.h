@@ -74,6 +74,40 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// The value of lane ^ D, in the vector pipe alone (DPP within rows of 16 lanes, row swaps beyond): a step of a reduction or
+// of a sort takes tens of cycles, an exchange through the LDS crossbar more than a hundred.
+template <int D> __device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  static_assert(D == 1 || D == 2 || D == 4 || D == 8 || D == 16 || D == 32, "a power of two below 64");
+  if constexpr (D == 1) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true);        // quad_perm 1,0,3,2
+  else if constexpr (D == 2) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true);   // quad_perm 2,3,0,1
+  else if constexpr (D == 4) {      // ^ 7 (row_half_mirror), then ^ 3 (quad_perm 3,2,1,0)
+    const int h = __builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true);
+    return (uint32_t)__builtin_amdgcn_mov_dpp(h, 0x1B, 0xF, 0xF, true);
+  } else if constexpr (D == 8) return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xF, 0xF, true);   // row_ror 8
+  else if constexpr (D == 16) {      // rows 0 0 2 2 and 1 1 3 3
+    const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return (threadIdx.x & 16) ? s[0] : s[1];
+  } else {
+    const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return (threadIdx.x & 32) ? s[0] : s[1];
+  }
+}
+template <int D> __device__ __forceinline__ float lane_xor(float v) { return __uint_as_float(lane_xor<D>(__float_as_uint(v))); }
+template <int D> __device__ __forceinline__ int lane_xor(int v) { return (int)lane_xor<D>((uint32_t)v); }
+template <int D> __device__ __forceinline__ unsigned long long lane_xor(unsigned long long v) {
+  return ((unsigned long long)lane_xor<D>((uint32_t)(v >> 32)) << 32) | lane_xor<D>((uint32_t)v);
+}
+// f(partner's value) over the lanes of a group of G
+template <int G, typename V, typename F> __device__ __forceinline__ V group_reduce(V v, F f) {
+  if constexpr (G > 1) v = f(v, lane_xor<1>(v));
+  if constexpr (G > 2) v = f(v, lane_xor<2>(v));
+  if constexpr (G > 4) v = f(v, lane_xor<4>(v));
+  if constexpr (G > 8) v = f(v, lane_xor<8>(v));
+  if constexpr (G > 16) v = f(v, lane_xor<16>(v));
+  if constexpr (G > 32) v = f(v, lane_xor<32>(v));
+  return v;
+}
+
 // Blocks are dealt round robin over the 8 XCDs: give each XCD one contiguous range of tiles, so neighbours share an L2.
 // A bijection of [0, total) for every total.
 __device__ __forceinline__ unsigned xcd_contiguous(unsigned block, unsigned total) {

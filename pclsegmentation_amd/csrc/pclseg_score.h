@@ -168,16 +168,25 @@ __global__ __launch_bounds__(256) void logprob_thread_rows(ScoreArgs a) {
   }
 }
 
+// A class as one 64-bit key: the float mapped to an unsigned of the same order above the complement of the index, so one
+// comparison decides value first and lowest index among equals; 0 is no entry.
+typedef unsigned long long Key;
+__device__ __forceinline__ Key make_key(float x, int idx) {
+  const uint32_t u = __float_as_uint(x + 0.0f);       // -0 and +0 are equal: one key
+  const uint32_t o = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return ((Key)o << 32) | (uint32_t)~(uint32_t)idx;
+}
+__device__ __forceinline__ float key_value(Key k) {
+  const uint32_t o = (uint32_t)(k >> 32);
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+__device__ __forceinline__ int key_index(Key k) { return (int)~(uint32_t)k; }
 // ---- V <= 2048: G lanes own a row
 template <int G> __device__ __forceinline__ float group_max(float v) {
-#pragma unroll
-  for (int d = 1; d < G; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
+  return group_reduce<G>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 template <int G> __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int d = 1; d < G; d <<= 1) v += __shfl_xor(v, d);
-  return v;
+  return group_reduce<G>(v, [](float a, float b) { return a + b; });
 }
 
 template <typename T, int G>
@@ -222,16 +231,10 @@ __global__ __launch_bounds__(256) void logprob_group_rows(ScoreArgs a) {
   const RowOut o = row_out(st);
   if (g == 0 && live) write_row<T>(a, row, o);
   for (int k = 0; k < a.top_k; ++k) {
-    float best = bv;
-    int id = bi;
-#pragma unroll
-    for (int d = 1; d < G; d <<= 1) {
-      const float ov = __shfl_xor(best, d);
-      const int oi = __shfl_xor(id, d);
-      const bool b = ov > best || (ov == best && oi < id);
-      best = b ? ov : best;
-      id = b ? oi : id;
-    }
+    // value first, then the lowest index: one key (-0 counts as 0)
+    const Key win = group_reduce<G>(bi == 0x7fffffff ? (Key)0 : make_key(bv, bi), [](Key a, Key b) { return a > b ? a : b; });
+    const float best = win ? key_value(win) : neg_inf();
+    const int id = win ? key_index(win) : 0x7fffffff;
     const bool none = best == neg_inf();
     if (g == 0 && live) {
       a.top_ids[row * a.top_k + k] = none || o.bad ? -1 : id;
@@ -256,62 +259,39 @@ __global__ __launch_bounds__(256) void logprob_group_rows(ScoreArgs a) {
   }
 }
 
-// ---- longer rows: waves stream pieces of 2048 elements
-// The top list of a wave is one 64-bit key per lane, sorted downwards: the float mapped to an unsigned of the same order
-// above the complement of the index, so one comparison decides value first and lowest index among equals; 0 is no entry.
-typedef unsigned long long Key;
-__device__ __forceinline__ Key make_key(float x, int idx) {
-  const uint32_t u = __float_as_uint(x + 0.0f);       // -0 and +0 are equal: one key
-  const uint32_t o = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return ((Key)o << 32) | (uint32_t)~(uint32_t)idx;
+// ---- longer rows: waves stream pieces of 2048 elements.  A wave's top list is one key per lane, sorted downwards.
+// lane `src` (uniform)
+__device__ __forceinline__ float read_lane(float v, int src) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), src));
 }
-__device__ __forceinline__ float key_value(Key k) {
-  const uint32_t o = (uint32_t)(k >> 32);
-  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+__device__ __forceinline__ Key read_lane(Key k, int src) {
+  return ((Key)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), src) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, src);
 }
-__device__ __forceinline__ int key_index(Key k) { return (int)~(uint32_t)k; }
-__device__ __forceinline__ Key shfl_key(Key k, int src) {
-  return ((Key)(uint32_t)__shfl((int)(k >> 32), src) << 32) | (uint32_t)__shfl((int)(uint32_t)k, src);
+// one step of a bitonic network: lane and lane ^ D keep the larger and the smaller; `up` lanes keep the smaller of a pair's
+// lower lane
+template <int D, typename V> __device__ __forceinline__ V bitonic_step(V v, int lane, bool up) {
+  const V o = lane_xor<D>(v);
+  const bool want_max = !(lane & D) != up;
+  return ((o > v) == want_max) ? o : v;
 }
-__device__ __forceinline__ Key shfl_xor_key(Key k, int d) {
-  return ((Key)(uint32_t)__shfl_xor((int)(k >> 32), d) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)k, d);
+template <int D, typename V> __device__ __forceinline__ V bitonic_tail(V v, int lane, bool up) {      // steps D, D / 2, ... 1
+  v = bitonic_step<D>(v, lane, up);
+  if constexpr (D > 1) v = bitonic_tail<D / 2>(v, lane, up);
+  return v;
 }
-// 64 keys of a wave that rise and then fall (or any rotation): sorted downwards
-__device__ __forceinline__ Key bitonic_clean(Key k, int lane) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    const Key o = shfl_xor_key(k, d);
-    const bool want_max = !(lane & d);
-    k = ((o > k) == want_max) ? o : k;
-  }
-  return k;
-}
-__device__ __forceinline__ Key bitonic_sort(Key k, int lane) {
-#pragma unroll
-  for (int w = 2; w <= 64; w <<= 1) {
-#pragma unroll
-    for (int d = w >> 1; d > 0; d >>= 1) {
-      const Key o = shfl_xor_key(k, d);
-      const bool want_max = (!(lane & d)) == (!(lane & w));
-      k = ((o > k) == want_max) ? o : k;
-    }
-  }
-  return k;
+// 64 values of a wave that rise and then fall (or any rotation): sorted downwards
+template <typename V> __device__ __forceinline__ V bitonic_clean(V v, int lane) { return bitonic_tail<32>(v, lane, false); }
+template <bool UP, typename V> __device__ __forceinline__ V bitonic_sort(V v, int lane) {
+  v = bitonic_tail<1>(v, lane, !(lane & 2) == UP);
+  v = bitonic_tail<2>(v, lane, !(lane & 4) == UP);
+  v = bitonic_tail<4>(v, lane, !(lane & 8) == UP);
+  v = bitonic_tail<8>(v, lane, !(lane & 16) == UP);
+  v = bitonic_tail<16>(v, lane, !(lane & 32) == UP);
+  return bitonic_tail<32>(v, lane, UP);
 }
 // the 64 largest of two lists sorted downwards: the second is given reversed
 __device__ __forceinline__ Key merge_lists(Key a, Key b_reversed, int lane) {
   return bitonic_clean(a > b_reversed ? a : b_reversed, lane);
-}
-__device__ __forceinline__ float bitonic_sort_f(float v, int lane) {
-#pragma unroll
-  for (int w = 2; w <= 64; w <<= 1) {
-#pragma unroll
-    for (int d = w >> 1; d > 0; d >>= 1) {
-      const float o = __shfl_xor(v, d);
-      v = ((!(lane & d)) == (!(lane & w))) ? fmaxf(v, o) : fminf(v, o);
-    }
-  }
-  return v;
 }
 
 __device__ __forceinline__ Stat wave_join(Stat st) {
@@ -349,11 +329,10 @@ __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
     wave_lds_fence();
     Key k = lane < count ? cand[wave][lane] : 0;
     const Key rest = cand[wave][64 + lane];
-    k = bitonic_sort(k, lane);
-    list = merge_lists(list, shfl_key(k, 63 - lane), lane);
+    list = merge_lists(list, bitonic_sort<true>(k, lane), lane);
     wave_lds_fence();
     cand[wave][lane] = rest;
-    const Key kth = shfl_key(list, a.top_k - 1);
+    const Key kth = read_lane(list, a.top_k - 1);
     if (kth) {
       thr_key = kth;
       thr = key_value(kth);
@@ -386,7 +365,7 @@ __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
       for (int v = 0; v < NV; ++v) lane_max = fmaxf(lane_max, vm[v]);
       const Key over = __ballot(lane_max >= thr);
       if (__popcll(over) > a.top_k || thr == neg_inf()) {
-        const float bound = __shfl(bitonic_sort_f(lane_max, lane), a.top_k - 1);
+        const float bound = read_lane(bitonic_sort<false>(lane_max, lane), a.top_k - 1);
         if (bound > thr) {
           thr = bound;
           thr_key = 0;

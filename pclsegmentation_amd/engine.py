@@ -45,8 +45,6 @@ EXPORTS = [
   "pclseg_op_linear_i8", "pclseg_op_label_logprobs_workspace", "pclseg_op_label_logprobs", "pclseg_op_label_logprobs_grad",
 ]
 
-DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}     # pclseg_dtype of a torch dtype's name
-
 
 class Desc(ctypes.Structure):
   _fields_ = [("arch", ctypes.c_int32), ("height", ctypes.c_int32), ("width", ctypes.c_int32),
@@ -245,7 +243,10 @@ def torch_device(index=0):
 def stream_handle(device):
   """Raw hipStream_t of torch's current stream on ``device`` (what pclseg_set_stream takes)."""
   import torch
-  return torch.cuda.current_stream(device).cuda_stream
+  index = getattr(device, "index", None)
+  if index is None:
+    return torch.cuda.current_stream(device).cuda_stream
+  return torch._C._cuda_getCurrentRawStream(index)      # the same handle without a Stream object: 0.1 us instead of 1.9
 
 
 def on_device(x):

@@ -12,6 +12,7 @@ rows may have any stride as long as their elements are adjacent (others are copi
 stream of the tensors' device, allocate their outputs and workspace through torch and keep nothing, so they can be captured
 into a graph.  Like the rest of the package they compute outside of autograd.  All arithmetic is in libpclseg.so."""
 import ctypes
+import functools
 from collections import namedtuple
 
 import torch
@@ -21,19 +22,22 @@ from . import engine as _engine
 LabelLogprobs = namedtuple("LabelLogprobs", "logprob entropy lse top_ids top_logprobs")
 
 
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # pclseg_dtype
+
+
 def _fail(what):
   raise ValueError("pclseg: " + what)
 
 
 def _dtype(t, name):
-  d = _engine.DTYPES.get(str(t.dtype))
+  d = _DTYPES.get(t.dtype)
   if d is None:
     _fail("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
   return d
 
 
 def _on(t, dev, name):
-  if not isinstance(t, torch.Tensor) or not _engine.on_device(t) or (dev is not None and t.device != dev):
+  if not isinstance(t, torch.Tensor) or (t.device != dev if dev is not None else not _engine.on_device(t)):
     _fail("%s must be a tensor on %s" % (name, dev or "the device"))
 
 
@@ -56,12 +60,28 @@ def _ptr(t):
   return None if t is None else t.data_ptr()
 
 
+@functools.lru_cache(maxsize=None)
+def _several_devices():
+  return torch.cuda.device_count() > 1
+
+
 def _call(dev, fn, *args):
   """fn(*args, stream) with `dev` current: kernels are launched on the current device."""
-  if torch.cuda.is_available() and torch.cuda.current_device() != dev.index:
+  if _several_devices() and torch.cuda.current_device() != dev.index:
     with torch.cuda.device(dev):
-      return _engine.check(fn(*args, _engine.stream_handle(dev)))
-  return _engine.check(fn(*args, _engine.stream_handle(dev)))
+      rc = fn(*args, _engine.stream_handle(dev))
+  else:
+    rc = fn(*args, _engine.stream_handle(dev))
+  if rc:
+    _engine.check(rc)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(name, *sizes):
+  """Bytes of workspace a call of these sizes takes."""
+  size = ctypes.c_size_t()
+  _engine.check(getattr(_engine.load_library(), name)(*sizes, ctypes.byref(size)))
+  return size.value
 
 
 class Int8Rows:
@@ -134,7 +154,7 @@ def quantize_rows(x):
 def _epilogue(dev, m, n, shape, weight, bias, act, residual, dtype):
   if act not in _engine.ACT:
     _fail("unknown activation %r" % (act,))
-  if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+  if dtype not in _DTYPES:
     _fail("out_dtype must be float32, bfloat16 or float16, got %s" % (dtype,))
   if not isinstance(weight, Int8Rows) or weight.data.device != dev:
     _fail("weight must be Int8Rows on %s" % (dev,))
@@ -160,7 +180,7 @@ def matmul_i8(a, b, bias=None, act="none", residual=None, out_dtype=torch.float3
   if m and n:
     _call(dev, _engine.load_library().pclseg_op_matmul_i8, a.data.data_ptr(), a.scale.data_ptr(), b.data.data_ptr(),
           b.scale.data_ptr(), m, n, a.k, _ptr(bias), _engine.ACT[act], _ptr(residual), rstride, y.data_ptr(), n,
-          _engine.DTYPES[str(out_dtype)])
+          _DTYPES[out_dtype])
   return y
 
 
@@ -179,13 +199,11 @@ def linear_i8(x, weight, bias=None, act="none", residual=None, out_dtype=None):
   bias, residual, rstride = _epilogue(dev, m, n, shape, weight, bias, act, residual, out_dtype)
   y = torch.empty(shape, dtype=out_dtype, device=dev)
   if m and n:
-    lib = _engine.load_library()
-    size = ctypes.c_size_t()
-    _engine.check(lib.pclseg_op_linear_i8_workspace(m, n, k, ctypes.byref(size)))
-    work = torch.empty(size.value, dtype=torch.uint8, device=dev)
-    _call(dev, lib.pclseg_op_linear_i8, r.data_ptr(), dt, stride, weight.data.data_ptr(), weight.scale.data_ptr(), m, n, k,
-          _ptr(bias), _engine.ACT[act], _ptr(residual), rstride, y.data_ptr(), n, _engine.DTYPES[str(out_dtype)],
-          work.data_ptr(), size.value)
+    size = _workspace("pclseg_op_linear_i8_workspace", m, n, k)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _call(dev, _engine.load_library().pclseg_op_linear_i8, r.data_ptr(), dt, stride, weight.data.data_ptr(), weight.scale.data_ptr(), m, n, k,
+          _ptr(bias), _engine.ACT[act], _ptr(residual), rstride, y.data_ptr(), n, _DTYPES[out_dtype],
+          _ptr(work), size)
   return y
 
 
@@ -233,20 +251,18 @@ def label_logprobs(logits, labels=None, top_k=0, allowed=None):
   mstride = 0
   if allowed is not None:
     allowed, mstride = _mask(allowed, logits)
-  lib = _engine.load_library()
-  size = ctypes.c_size_t()
-  _engine.check(lib.pclseg_op_label_logprobs_workspace(m, v, top_k, ctypes.byref(size)))
-  stats = torch.empty((3,) + shape, dtype=torch.float32, device=dev)
-  logprob, entropy, lse = stats.unbind(0)
+  size = _workspace("pclseg_op_label_logprobs_workspace", m, v, top_k)
+  logprob = torch.empty(shape, dtype=torch.float32, device=dev) if labels is not None else None
+  entropy = torch.empty(shape, dtype=torch.float32, device=dev)
+  lse = torch.empty(shape, dtype=torch.float32, device=dev)
   ids = torch.empty(shape + (top_k,), dtype=torch.int32, device=dev) if top_k else None
   tops = torch.empty(shape + (top_k,), dtype=torch.float32, device=dev) if top_k else None
   if m:
-    work = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
-    _call(dev, lib.pclseg_op_label_logprobs, r.data_ptr(), dt, m, v, stride, _ptr(labels),
-          labels.element_size() if labels is not None else 0, _ptr(allowed), mstride, top_k,
-          logprob.data_ptr() if labels is not None else None, entropy.data_ptr(), lse.data_ptr(), _ptr(ids), _ptr(tops),
-          _ptr(work), size.value)
-  return LabelLogprobs(logprob if labels is not None else None, entropy, lse, ids, tops)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _call(dev, _engine.load_library().pclseg_op_label_logprobs, r.data_ptr(), dt, m, v, stride, _ptr(labels),
+          labels.element_size() if labels is not None else 0, _ptr(allowed), mstride, top_k, _ptr(logprob), entropy.data_ptr(),
+          lse.data_ptr(), _ptr(ids), _ptr(tops), _ptr(work), size)
+  return LabelLogprobs(logprob, entropy, lse, ids, tops)
 
 
 def label_logprobs_grad(logits, labels, lse, d_logprob=None, entropy=None, d_entropy=None, top_ids=None, d_top=None,

@@ -147,10 +147,11 @@ def test_matmul_i8_sums_are_exact(cuda):
   assert torch.equal(ops.matmul_i8(rb, ra).cpu(), want.t().float())
 
 
-@pytest.mark.parametrize("m", [1, 7, 48, 100, 600])
+@pytest.mark.parametrize("m,k,n", [(1, 333, 260), (7, 333, 260), (48, 333, 260), (100, 333, 260), (600, 333, 260),
+                                   # up to four rows take one launch, as long as their codes fit into a block's LDS
+                                   (1, 1, 1), (2, 64, 5), (3, 65, 16), (4, 4097, 33), (4, 12288, 20), (4, 12289, 20), (1, 49153, 9)])
 @pytest.mark.parametrize("dtype", TYPES)
-def test_linear_i8(cuda, m, dtype):
-  k, n = 333, 260
+def test_linear_i8(cuda, m, k, n, dtype):
   x = rnd(m, m, k).to(dtype)
   w = ops.quantize_rows((rnd(3, n, k) * 0.05).float().to(cuda))
   bias, residual = rnd(4, n).float(), rnd(5, m, n).to(dtype)
@@ -163,7 +164,7 @@ def test_linear_i8(cuda, m, dtype):
                                    residual=residual.to(cuda), out_dtype=dtype), got)
   plain = ops.linear_i8(x.to(cuda), w, out_dtype=F32)
   check_product(plain, *product64(q, s, w.codes.cpu(), w.scale.cpu(), None, "none", None), F32)
-  wide = torch.zeros(m, 2 * k, dtype=dtype, device=cuda)
+  wide = torch.zeros(m, k + 9, dtype=dtype, device=cuda)
   wide[:, 5:5 + k] = x.to(cuda)
   assert torch.equal(ops.linear_i8(wide[:, 5:5 + k], w, out_dtype=F32), plain)
   assert torch.equal(ops.linear_i8(x.to(cuda).view(1, m, 1, k), w, out_dtype=F32), plain.view(1, m, 1, n))
