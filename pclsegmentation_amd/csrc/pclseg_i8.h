@@ -87,10 +87,13 @@ __device__ __forceinline__ uint32_t pack4(const float* u) {
 template <typename T> struct Eight {
   static constexpr int N = 8 / Elem<T>::VEC;
   u32x4 v[N];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int h = 0; h < N; ++h) v[h] = load16(p + h * Elem<T>::VEC);
+  }
   __device__ __forceinline__ void load(const T* row, int c, int cols) {      // 0 behind the row's end
     if (c + 8 <= cols) {
-#pragma unroll
-      for (int h = 0; h < N; ++h) v[h] = load16(row + c + h * Elem<T>::VEC);
+      load(row + c);
     } else {
       float f[8];
 #pragma unroll
@@ -137,8 +140,12 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
   Eight<T> x[NV];
   RowMax<T> mx;
 #pragma unroll
+  for (int v = 0; v < NV; ++v) {      // stretches inside the row for all lanes first: a uniform test, all loads in flight
+    if ((v + 1) * 8 * G <= a.cols) x[v].load(src + (v * G + g) * 8);
+  }
+#pragma unroll
   for (int v = 0; v < NV; ++v)
-    if (v < nv) x[v].load(src, (v * G + g) * 8, a.cols);
+    if (v < nv && (v + 1) * 8 * G > a.cols) x[v].load(src, (v * G + g) * 8, a.cols);
 #pragma unroll
   for (int v = 0; v < NV; ++v)
     if (v < nv) x[v].add_to(mx);

@@ -105,7 +105,7 @@ int check_product(const char* op, int64_t m, int64_t n, int64_t k, const int8_t*
 }
 
 // ---------------------------------------------------------------------------------------------- log probabilities
-constexpr int kThreadRow = 32, kGroupRow = 2048, kPiece = 2048, kWaves = 4, kRounds = 4;
+constexpr int kThreadRow = 32, kGroupRow = 2048, kPiece = 2048, kWaves = 4, kRounds = 4, kManyRows = 2048;
 
 // pieces a long row is cut into so that few rows still fill the chip: a block streams kWaves pieces of 2048 elements at a
 // time, and 512 blocks hide the memory's latency
@@ -119,27 +119,32 @@ size_t score_workspace(int64_t rows, int64_t classes, int top_k) {
   return segs == 1 ? 0 : (size_t)rows * segs * (sizeof(ScorePart) + (top_k ? 64 * sizeof(Key) : 0));
 }
 
-template <typename T> void launch_score(const ScoreArgs& a, hipStream_t s) {
+template <typename T, bool MASK, int CAP> void launch_thread_rows(const ScoreArgs& a, hipStream_t s) {
+  if constexpr (CAP > Elem<T>::VEC) {
+    if (a.classes <= CAP - Elem<T>::VEC) return launch_thread_rows<T, MASK, CAP - Elem<T>::VEC>(a, s);
+  }
+  logprob_thread_rows<T, CAP, MASK><<<dim3((unsigned)((a.rows + 255) / 256)), dim3(256), 0, s>>>(a);
+}
+
+template <typename T, bool MASK> void launch_score(const ScoreArgs& a, hipStream_t s) {
   const int v = a.classes;
   if (v <= kThreadRow) {
-    const dim3 g((unsigned)((a.rows + 255) / 256)), b(256);
-    if (v <= 8) logprob_thread_rows<T, 8><<<g, b, 0, s>>>(a);
-    else if (v <= 16) logprob_thread_rows<T, 16><<<g, b, 0, s>>>(a);
-    else if (v <= 24) logprob_thread_rows<T, 24><<<g, b, 0, s>>>(a);
-    else logprob_thread_rows<T, 32><<<g, b, 0, s>>>(a);
+    launch_thread_rows<T, MASK, kThreadRow>(a, s);
   } else if (v <= kGroupRow && !(v > 256 && a.top_k > kRounds)) {
     auto grid = [&](int g) { return dim3((unsigned)((a.rows + 256 / g - 1) / (256 / g))); };
-    if (v <= 8 * 32) logprob_group_rows<T, 8><<<grid(8), dim3(256), 0, s>>>(a);
-    else if (v <= 16 * 32) logprob_group_rows<T, 16><<<grid(16), dim3(256), 0, s>>>(a);
-    else if (v <= 32 * 32) logprob_group_rows<T, 32><<<grid(32), dim3(256), 0, s>>>(a);
-    else logprob_group_rows<T, 64><<<grid(64), dim3(256), 0, s>>>(a);
+    if (v <= 8 * 32) logprob_group_rows<T, 8, MASK><<<grid(8), dim3(256), 0, s>>>(a);
+    else if (v <= 16 * 32) logprob_group_rows<T, 16, MASK><<<grid(16), dim3(256), 0, s>>>(a);
+    else if (v <= 32 * 32) logprob_group_rows<T, 32, MASK><<<grid(32), dim3(256), 0, s>>>(a);
+    else logprob_group_rows<T, 64, MASK><<<grid(64), dim3(256), 0, s>>>(a);
   } else {
     const dim3 g((unsigned)(a.rows * a.segs));
-    if (v > kPiece) {
-      if (a.top_k) logprob_wave_rows<T, kWaves, true><<<g, dim3(kWaves * 64), 0, s>>>(a);
-      else logprob_wave_rows<T, kWaves, false><<<g, dim3(kWaves * 64), 0, s>>>(a);
+    // one wave a row where that fills the chip: a list is kept and merged once a row instead of four times
+    if (v > kPiece && a.rows < kManyRows) {
+      if (a.top_k) logprob_wave_rows<T, kWaves, true, MASK><<<g, dim3(kWaves * 64), 0, s>>>(a);
+      else logprob_wave_rows<T, kWaves, false, MASK><<<g, dim3(kWaves * 64), 0, s>>>(a);
     } else {
-      logprob_wave_rows<T, 1, true><<<g, dim3(64), 0, s>>>(a);
+      if (a.top_k) logprob_wave_rows<T, 1, true, MASK><<<g, dim3(64), 0, s>>>(a);
+      else logprob_wave_rows<T, 1, false, MASK><<<g, dim3(64), 0, s>>>(a);
     }
     if (a.segs > 1) {
       if (a.top_k) logprob_join<T, true><<<dim3((unsigned)a.rows), dim3(256), 0, s>>>(a);
@@ -261,7 +266,10 @@ int pclseg_op_label_logprobs(const void* logits, int dtype, int64_t rows, int64_
   ScoreArgs a{logits, rows, stride, (int)classes, labels, label_bytes == 8, allowed, allowed_stride, top_k,
               logprob, entropy, lse, top_ids, top_logprobs, workspace, score_segs(rows, classes)};
   if (rows > kMaxBlocks || rows * a.segs > kMaxBlocks) return bad_shape(op, "more rows than a launch has blocks");
-  with_type(dtype, [&](auto t) { launch_score<decltype(t)>(a, (hipStream_t)hip_stream); });
+  with_type(dtype, [&](auto t) {
+    if (allowed) launch_score<decltype(t), true>(a, (hipStream_t)hip_stream);
+    else launch_score<decltype(t), false>(a, (hipStream_t)hip_stream);
+  });
   return launched(op);
 } OP_CATCH
 
@@ -298,7 +306,8 @@ int pclseg_op_label_logprobs_grad(const void* logits, int dtype, int64_t rows, i
   const int64_t blocks = a.pieces > 1 ? rows * a.pieces : (rows + a.rows_per_block - 1) / a.rows_per_block;
   if (rows > kMaxBlocks * 256 || blocks > kMaxBlocks) return bad_shape(op, "more rows than a launch has blocks");
   with_type(dtype, [&](auto t) {
-    logprob_grad<decltype(t)><<<dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream>>>(a);
+    if (allowed) logprob_grad<decltype(t), true><<<dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream>>>(a);
+    else logprob_grad<decltype(t), false><<<dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream>>>(a);
   });
   return launched(op);
 } OP_CATCH

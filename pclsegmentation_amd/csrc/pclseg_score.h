@@ -97,54 +97,63 @@ template <typename T> __device__ __forceinline__ void write_row(const ScoreArgs&
   }
 }
 
-// elements [c, c + VEC) of a row of `classes`, -inf behind its end and where the mask is 0
-template <typename T>
-__device__ __forceinline__ void load_masked(const T* row, const uint8_t* mask, int c, int classes, float* f) {
-  constexpr int VEC = Elem<T>::VEC;
-  if (c + VEC <= classes) {
-    const u32x4 v = load16(row + c);
+// 16 bytes of a row and the bytes of its mask (MASK): requested first, looked at later, so that a lane's loads are all in
+// flight
+template <typename T, bool MASK> struct Piece {
+  static constexpr int VEC = Elem<T>::VEC;
+  u32x4 v;
+  uint32_t mk[MASK ? VEC / 4 : 1];
+  // elements [c, c + VEC) of a row, all inside it
+  __device__ __forceinline__ void load(const T* row, const uint8_t* mask, int64_t c) {
+    v = load16(row + c);
+    if constexpr (MASK) {
+#pragma unroll
+      for (int h = 0; h < VEC / 4; ++h) mk[h] = reinterpret_cast<const Pack4a1*>(mask + c + h * 4)->v;
+    }
+  }
+  __device__ __forceinline__ void expand(float* f) const {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) f[e] = Elem<T>::get(v, e);
-    if (mask) {
-      if constexpr (VEC == 8) {
-        const uint64_t mk = reinterpret_cast<const Pack8a1*>(mask + c)->v;
+    if constexpr (MASK) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = ((mk >> (8 * e)) & 0xff) ? f[e] : neg_inf();
-      } else {
-        const uint32_t mk = reinterpret_cast<const Pack4a1*>(mask + c)->v;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = ((mk >> (8 * e)) & 0xff) ? f[e] : neg_inf();
-      }
+      for (int e = 0; e < VEC; ++e) f[e] = (mk[e / 4] >> (8 * (e % 4))) & 0xff ? f[e] : neg_inf();
     }
+  }
+};
+// the same where the row may begin (c < 0) or end inside: -inf outside of it
+template <typename T, bool MASK>
+__device__ __forceinline__ void load_tail(const T* row, const uint8_t* mask, int c, int classes, float* f) {
+  constexpr int VEC = Elem<T>::VEC;
+  if (c >= 0 && c + VEC <= classes) {
+    Piece<T, MASK> m;
+    m.load(row, mask, c);
+    m.expand(f);
   } else {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       f[e] = neg_inf();
-      if (c + e < classes && (!mask || mask[c + e])) f[e] = Elem<T>::load(row + c + e);
+      if (c + e >= 0 && c + e < classes && (!MASK || mask[c + e])) f[e] = Elem<T>::load(row + c + e);
     }
   }
 }
 
 // ---- V <= 32: a thread owns a row
-// CAP = the row's registers.  A row of 20 floats is 80 bytes: the 16-byte loads of a wave touch 40 lines, five times over,
-// all of them in the L1 after the first.
-template <typename T, int CAP>
-__global__ __launch_bounds__(256) void logprob_thread_rows(ScoreArgs a) {
-  constexpr int VEC = Elem<T>::VEC;
+// CAP = classes rounded up to whole 16 bytes: only the last of the row's pieces can be cut.  A row of 20 floats is 80 bytes:
+// the 16-byte loads of a wave touch 40 lines, five times over, all of them in the L1 after the first.
+template <typename T, int CAP, bool MASK>
+__global__ __launch_bounds__(256, CAP <= 20 ? 6 : 4) void logprob_thread_rows(ScoreArgs a) {
+  constexpr int VEC = Elem<T>::VEC, NV = CAP / VEC;
   const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (row >= a.rows) return;
   const T* src = static_cast<const T*>(a.x) + row * a.stride;
-  const uint8_t* mask = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+  const uint8_t* mask = MASK ? a.allowed + row * a.allowed_stride : nullptr;
   float x[CAP];
+  Piece<T, MASK> raw[NV];
 #pragma unroll
-  for (int v = 0; v < CAP / VEC; ++v) {
-    if (v * VEC < a.classes) {
-      load_masked(src, mask, v * VEC, a.classes, x + v * VEC);
-    } else {
+  for (int v = 0; v + 1 < NV; ++v) raw[v].load(src, mask, v * VEC);
+  load_tail<T, MASK>(src, mask, CAP - VEC, a.classes, x + CAP - VEC);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) x[v * VEC + e] = neg_inf();
-    }
-  }
+  for (int v = 0; v + 1 < NV; ++v) raw[v].expand(x + v * VEC);
   Stat st{kLowest, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < CAP; ++j) st.m = fmaxf(st.m, x[j]);
@@ -152,6 +161,33 @@ __global__ __launch_bounds__(256) void logprob_thread_rows(ScoreArgs a) {
   for (int j = 0; j < CAP; ++j) stat_add(st, x[j]);
   const RowOut o = row_out(st);
   write_row<T>(a, row, o);
+  if (a.top_k == 0) return;
+  int32_t* ids = a.top_ids + row * a.top_k;
+  float* tops = a.top_logprobs + row * a.top_k;
+  if (a.top_k <= 4 && !o.bad) {
+    // up to four alternatives: the four largest values by insertion (a maximum and three medians an element), their indices
+    // by comparison, downwards so that the lowest stays; equal values among them take the rounds below
+    float b[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+#pragma unroll
+    for (int j = 0; j < CAP; ++j) {
+      b[3] = __builtin_amdgcn_fmed3f(b[2], b[3], x[j]);
+      b[2] = __builtin_amdgcn_fmed3f(b[1], b[2], x[j]);
+      b[1] = __builtin_amdgcn_fmed3f(b[0], b[1], x[j]);
+      b[0] = fmaxf(b[0], x[j]);
+    }
+    if (b[0] != b[1] && b[1] != b[2] && b[2] != b[3]) {      // (-inf, -inf: fewer than four classes, the rounds too)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (k >= a.top_k) break;
+        int id = -1;
+#pragma unroll
+        for (int j = CAP - 1; j >= 0; --j) id = x[j] == b[k] ? j : id;
+        ids[k] = b[k] == neg_inf() ? -1 : id;
+        tops[k] = row_logprob(o, b[k]);
+      }
+      return;
+    }
+  }
   for (int k = 0; k < a.top_k; ++k) {
     float best = neg_inf();
     int id = -1;
@@ -163,8 +199,8 @@ __global__ __launch_bounds__(256) void logprob_thread_rows(ScoreArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < CAP; ++j) x[j] = j == id ? neg_inf() : x[j];
-    a.top_ids[row * a.top_k + k] = o.bad ? -1 : id;
-    a.top_logprobs[row * a.top_k + k] = row_logprob(o, best);
+    ids[k] = o.bad ? -1 : id;
+    tops[k] = row_logprob(o, best);
   }
 }
 
@@ -189,7 +225,7 @@ template <int G> __device__ __forceinline__ float group_sum(float v) {
   return group_reduce<G>(v, [](float a, float b) { return a + b; });
 }
 
-template <typename T, int G>
+template <typename T, int G, bool MASK>
 __global__ __launch_bounds__(256) void logprob_group_rows(ScoreArgs a) {
   constexpr int VEC = Elem<T>::VEC, NV = 32 / VEC;
   const int g = threadIdx.x & (G - 1);
@@ -197,14 +233,19 @@ __global__ __launch_bounds__(256) void logprob_group_rows(ScoreArgs a) {
   const bool live = row0 < a.rows;
   const int64_t row = live ? row0 : a.rows - 1;      // lanes behind the last row repeat it and write nothing
   const T* src = static_cast<const T*>(a.x) + row * a.stride;
-  const uint8_t* mask = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+  const uint8_t* mask = MASK ? a.allowed + row * a.allowed_stride : nullptr;
   const int nv = (a.classes + G * VEC - 1) / (G * VEC);   // uniform
   float x[NV][VEC];
   float bv = neg_inf();      // this lane's largest element that is left, and its index
   int bi = 0x7fffffff;
+  Piece<T, MASK> raw[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v)      // stretches that lie inside the row for all lanes: a uniform test, all loads in flight
+    if ((v + 1) * G * VEC <= a.classes) raw[v].load(src, mask, (v * G + g) * VEC);
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
-    if (v < nv) load_masked(src, mask, (v * G + g) * VEC, a.classes, x[v]);
+    if ((v + 1) * G * VEC <= a.classes) raw[v].expand(x[v]);
+    else if (v < nv) load_tail<T, MASK>(src, mask, (v * G + g) * VEC, a.classes, x[v]);
   }
   Stat st{kLowest, 0.f, 0.f};
 #pragma unroll
@@ -267,6 +308,12 @@ __device__ __forceinline__ float read_lane(float v, int src) {
 __device__ __forceinline__ Key read_lane(Key k, int src) {
   return ((Key)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), src) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, src);
 }
+// the next float above a finite one (NaN and infinities do not get here)
+__device__ __forceinline__ float next_above(float f) {
+  const uint32_t u = __float_as_uint(f + 0.0f);
+  return __uint_as_float((u & 0x80000000u) ? u - 1 : u + 1);
+}
+
 // one step of a bitonic network: lane and lane ^ D keep the larger and the smaller; `up` lanes keep the smaller of a pair's
 // lower lane
 template <int D, typename V> __device__ __forceinline__ V bitonic_step(V v, int lane, bool up) {
@@ -305,93 +352,130 @@ __device__ __forceinline__ Stat wave_join(Stat st) {
 // a piece's statistics and list in the workspace: [row * segs + seg]
 struct ScorePart { float m, s, t, pad; };
 
-template <typename T, int NW, bool TOP>
+template <typename T, int NW, bool TOP, bool MASK>
 __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
   constexpr int VEC = Elem<T>::VEC, NV = 32 / VEC, PIECE = 64 * 32;
   __shared__ Key cand[TOP ? NW : 1][128];
   __shared__ Key lists[TOP ? NW : 1][64];
   __shared__ Stat stats[NW];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ float seen[NW];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = blockIdx.x / (unsigned)a.segs;
   const int seg = (int)(blockIdx.x % (unsigned)a.segs);
   const T* src = static_cast<const T*>(a.x) + row * a.stride;
-  const uint8_t* mask = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-  const int pieces = (int)(((int64_t)a.classes + PIECE - 1) / PIECE);
+  const uint8_t* mask = MASK ? a.allowed + row * a.allowed_stride : nullptr;
+  // pieces begin at multiples of 16 bytes, `pad` elements before the row's first: rows of an odd length read at the rate of
+  // the others (4096 x 50001 bf16 without a top list 93 us unaligned, 80 aligned)
+  const int pad = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
+  const int pieces = (int)(((int64_t)a.classes + pad + PIECE - 1) / PIECE);
   const int p0 = (int)((int64_t)pieces * seg / a.segs), p1 = (int)((int64_t)pieces * (seg + 1) / a.segs);
 
   Stat st{kLowest, 0.f, 0.f};
   Key list = 0;
-  float thr = neg_inf();      // a candidate is at least thr and behind no listed entry: key > thr_key
-  Key thr_key = 0;
+  // An element is offered to the list when it is at least thr.  A wave that has seen top_k elements of at least b takes the
+  // next float above b: its later pieces hold higher indices, an equal value stays behind.  The other waves' b hold as they
+  // are; they are read from LDS without a barrier, an old value only offers more.
+  float thr = kLowest;
+  if (TOP && NW > 1 && lane == 0) seen[wave] = kLowest;
+  if (TOP && NW > 1) __syncthreads();
+  auto raise = [&](float b) {
+    thr = fmaxf(thr, next_above(b));
+    if (NW > 1 && lane == 0) *const_cast<volatile float*>(&seen[wave]) = b;
+  };
   int n = 0;                  // candidates waiting in cand[wave]
 
   auto flush = [&](int count) {   // the first 64 (count of them valid) into the list
     wave_lds_fence();
-    Key k = lane < count ? cand[wave][lane] : 0;
+    const Key k = lane < count ? cand[wave][lane] : 0;
     const Key rest = cand[wave][64 + lane];
     list = merge_lists(list, bitonic_sort<true>(k, lane), lane);
     wave_lds_fence();
     cand[wave][lane] = rest;
     const Key kth = read_lane(list, a.top_k - 1);
-    if (kth) {
-      thr_key = kth;
-      thr = key_value(kth);
-    }
+    if (kth) raise(key_value(kth));
   };
 
-  for (int p = p0 + wave; p < p1; p += NW) {
-    float x[NV][VEC], vm[NV];
-    const int base = p * PIECE;
+  // whole pieces are requested one ahead: the next one's loads are in flight while this one is worked on
+  const int first = pad ? 1 : 0, past = (a.classes + pad) / PIECE;
+  auto whole = [&](int p) { return p >= first && p < past && p < p1; };
+  Piece<T, MASK> raw[NV];
+  auto request = [&](int p) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) load_masked(src, mask, base + (v * 64 + lane) * VEC, a.classes, x[v]);
-    float cm = kLowest;
+    for (int v = 0; v < NV; ++v) raw[v].load(src, mask, (int64_t)p * PIECE - pad + (v * 64 + lane) * VEC);
+  };
+  if (whole(p0 + wave)) request(p0 + wave);
+  for (int p = p0 + wave; p < p1; p += NW) {
+    float x[NV][VEC];
+    const int base = p * PIECE - pad;
+    if (whole(p)) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) raw[v].expand(x[v]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < NV; ++v) load_tail<T, MASK>(src, mask, base + (v * 64 + lane) * VEC, a.classes, x[v]);
+    }
+    if (whole(p + NW)) request(p + NW);
+    float vec_max[NV], lane_max = neg_inf();
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      vm[v] = x[v][0];
+      vec_max[v] = x[v][0];
 #pragma unroll
-      for (int e = 1; e < VEC; ++e) vm[v] = fmaxf(vm[v], x[v][e]);
-      cm = fmaxf(cm, vm[v]);
+      for (int e = 1; e < VEC; ++e) vec_max[v] = fmaxf(vec_max[v], x[v][e]);
+      lane_max = fmaxf(lane_max, vec_max[v]);
     }
-    st = stat_shift(st, fmaxf(st.m, cm));
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) stat_add(st, x[v][e]);
+    uint32_t offers = 0;      // bit v VEC + e: the element is offered to the list
+    float least = thr, bound = kLowest;
+    bool some = false;
     if constexpr (TOP) {
       // at least top_k elements of this piece are not below the top_k-th largest of the lanes' maxima: a bound that keeps
       // the first piece from offering all of its elements, and a rising row from offering all of every piece
-      float lane_max = neg_inf();
+      if constexpr (NW > 1) {
 #pragma unroll
-      for (int v = 0; v < NV; ++v) lane_max = fmaxf(lane_max, vm[v]);
-      const Key over = __ballot(lane_max >= thr);
-      if (__popcll(over) > a.top_k || thr == neg_inf()) {
-        const float bound = read_lane(bitonic_sort<false>(lane_max, lane), a.top_k - 1);
-        if (bound > thr) {
-          thr = bound;
-          thr_key = 0;
-        }
+        for (int w = 0; w < NW; ++w) least = fmaxf(least, *const_cast<volatile float*>(&seen[w]));
       }
-      if (__ballot(lane_max >= thr)) {
+      const Key over = __ballot(lane_max >= least);
+      if (over) {
+        some = true;
+        if (__popcll(over) >= a.top_k) {
+          bound = read_lane(bitonic_sort<false>(lane_max, lane), a.top_k - 1);
+          least = fmaxf(least, bound);
+        }
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-          if (__ballot(vm[v] >= thr)) {
+          if (__ballot(vec_max[v] >= least)) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const int idx = base + (v * 64 + lane) * VEC + e;
-              const Key key = make_key(x[v][e], idx);
-              const bool take = x[v][e] >= thr && x[v][e] > neg_inf() && key > thr_key;
-              const Key who = __ballot(take);
-              if (who) {
-                if (take) cand[wave][n + __popcll(who & ((1ull << lane) - 1))] = key;
-                n += (int)__popcll(who);
-                if (n >= 64) {
-                  flush(64);
-                  n -= 64;
-                }
-              }
-            }
+            for (int e = 0; e < VEC; ++e) offers |= x[v][e] >= least ? 1u << (v * VEC + e) : 0u;
           }
         }
+      }
+    }
+    st = stat_shift(st, fmaxf(st.m, lane_max));
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) stat_add(st, x[v][e]);
+      __builtin_amdgcn_sched_barrier(0);      // 8 exponentials in flight at a time: more would only cost registers, and waves
+    }
+    if constexpr (TOP) {
+      if (some) {
+        // a lane's only offer is its maximum; several are read again (a register cannot be chosen by a lane)
+        const bool several = offers & (offers - 1);
+        for (Key who = __ballot(offers != 0); who; who = __ballot(offers != 0)) {      // one element of every lane that has one
+          if (offers) {
+            const int bit = __builtin_ctz(offers);
+            const int idx = base + ((bit / VEC) * 64 + lane) * VEC + bit % VEC;
+            float f = lane_max;
+            if (several) f = Elem<T>::load(src + idx);
+            offers &= offers - 1;
+            cand[wave][n + __popcll(who & ((1ull << lane) - 1))] = make_key(f, idx);
+          }
+          n += (int)__popcll(who);
+          if (n >= 64) {
+            flush(64);
+            n -= 64;
+          }
+        }
+        if (bound > kLowest && next_above(bound) > thr) raise(bound);
       }
     }
   }
@@ -401,7 +485,6 @@ __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
   if constexpr (TOP) lists[wave][lane] = list;
   __syncthreads();
   if constexpr (TOP) {
-#pragma unroll
     for (int h = NW / 2; h > 0; h >>= 1) {
       if (wave < h) {
         list = merge_lists(list, lists[wave + h][63 - lane], lane);
@@ -515,7 +598,7 @@ __device__ __forceinline__ GradRow grad_row(const GradArgs& a, int64_t row, int6
   return r;
 }
 
-template <typename T>
+template <typename T, bool MASK>
 __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
   constexpr int VEC = Elem<T>::VEC;
   constexpr int MAXR = 256;
@@ -536,10 +619,10 @@ __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
     const int r = i / nvec, c = c0 + (i - r * nvec) * VEC;
     const GradRow p = prm[r];
     const T* src = static_cast<const T*>(a.x) + (row0 + r) * a.stride;
-    const uint8_t* mask = a.allowed ? a.allowed + (row0 + r) * a.allowed_stride : nullptr;
+    const uint8_t* mask = MASK ? a.allowed + (row0 + r) * a.allowed_stride : nullptr;
     T* dst = static_cast<T*>(a.grad) + (row0 + r) * a.grad_stride;
     float f[VEC];
-    load_masked(src, mask, c, c1, f);
+    load_tail<T, MASK>(src, mask, c, c1, f);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) f[e] = grad_dense(p, f[e]);
     if (c + VEC <= c1) {
@@ -557,7 +640,7 @@ __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
     const int64_t row = row0 + r;
     const int64_t id = k == 0 ? lab[r] : (lab[r] == -2 ? -1 : a.top_ids[row * a.top_k + k - 1]);
     if (id < c0 || id >= c1) continue;
-    if (a.allowed && !a.allowed[row * a.allowed_stride + id]) continue;
+    if (MASK && !a.allowed[row * a.allowed_stride + id]) continue;
     const float x = Elem<T>::load(static_cast<const T*>(a.x) + row * a.stride + id);
     if (x == neg_inf()) continue;
     // every name of this element adds up here: threads that share an element write the same sum
