@@ -105,14 +105,15 @@ int check_product(const char* op, int64_t m, int64_t n, int64_t k, const int8_t*
 }
 
 // ---------------------------------------------------------------------------------------------- log probabilities
-constexpr int kThreadRow = 32, kGroupRow = 2048, kPiece = 2048, kWaves = 4, kRounds = 4, kManyRows = 2048;
+constexpr int kThreadRow = 32, kGroupRow = 2048, kPiece = 2048, kRounds = 4, kManyRows = 2048, kFewRows = 512;
+constexpr int kOneLaunch = 16, kFewWaves = 4;       // pieces one block of 16 waves takes, pieces that 4 waves are enough for
 
-// pieces a long row is cut into so that few rows still fill the chip: a block streams kWaves pieces of 2048 elements at a
-// time, and 512 blocks hide the memory's latency
+// blocks a row is cut into: one up to 32768 classes (a piece for each of 16 waves); beyond that as many as keep few rows
+// from waiting on few CUs (one row of 131072: 20 us in one block, 6.9 + 4.3 in 16 and a second launch that joins them)
 int score_segs(int64_t rows, int64_t classes) {
-  if (classes <= kGroupRow) return 1;
-  const int64_t most = (classes + (int64_t)kPiece * kWaves - 1) / ((int64_t)kPiece * kWaves);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(most, 64), 512 / rows));
+  const int64_t pieces = (classes + kPiece - 1) / kPiece;
+  if (pieces <= kOneLaunch) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(pieces / 4, 64), 256 / rows));
 }
 size_t score_workspace(int64_t rows, int64_t classes, int top_k) {
   const int segs = rows > 0 ? score_segs(rows, classes) : 1;
@@ -140,8 +141,13 @@ template <typename T, bool MASK> void launch_score(const ScoreArgs& a, hipStream
     const dim3 g((unsigned)(a.rows * a.segs));
     // one wave a row where that fills the chip: a list is kept and merged once a row instead of four times
     if (v > kPiece && a.rows < kManyRows) {
-      if (a.top_k) logprob_wave_rows<T, kWaves, true, MASK><<<g, dim3(kWaves * 64), 0, s>>>(a);
-      else logprob_wave_rows<T, kWaves, false, MASK><<<g, dim3(kWaves * 64), 0, s>>>(a);
+      if (v > kFewWaves * kPiece && a.rows <= kFewRows && a.segs == 1) {
+        if (a.top_k) logprob_wave_rows<T, 16, true, MASK><<<g, dim3(1024), 0, s>>>(a);
+        else logprob_wave_rows<T, 16, false, MASK><<<g, dim3(1024), 0, s>>>(a);
+      } else {
+        if (a.top_k) logprob_wave_rows<T, 4, true, MASK><<<g, dim3(256), 0, s>>>(a);
+        else logprob_wave_rows<T, 4, false, MASK><<<g, dim3(256), 0, s>>>(a);
+      }
     } else {
       if (a.top_k) logprob_wave_rows<T, 1, true, MASK><<<g, dim3(64), 0, s>>>(a);
       else logprob_wave_rows<T, 1, false, MASK><<<g, dim3(64), 0, s>>>(a);
@@ -294,20 +300,35 @@ int pclseg_op_label_logprobs_grad(const void* logits, int dtype, int64_t rows, i
   const uintptr_t g1 = g0 + ((uintptr_t)(rows - 1) * grad_stride + classes) * sz;
   if (g0 < x1 && x0 < g1) return bad(op, "grad overlaps the logits");
   GradArgs a{logits, rows, stride, (int)classes, labels, label_bytes == 8, allowed, allowed_stride, lse, entropy,
-             d_logprob, d_entropy, top_ids, d_top, d_top ? top_k : 0, grad, grad_stride, 1, (int)classes, 1};
-  // a block writes about 8192 elements: that many columns of a long row, or whole short rows
-  constexpr int kSpan = 8192;
-  if (classes > kSpan) {
-    a.span = kSpan;
-    a.pieces = (int)((classes + kSpan - 1) / kSpan);
+             d_logprob, d_entropy, top_ids, d_top, d_top ? top_k : 0, grad, grad_stride, 1, 1, 1, 0};
+  // a block takes 256 NI 16-byte pieces: that many of a long row, or whole short rows.  NI grows while the blocks are more
+  // than the 2048 that run at once
+  const int64_t vec = 16 / (int64_t)sz, nvec = (classes + vec - 1) / vec;
+  const int64_t all = rows > (int64_t(1) << 31) ? int64_t(1) << 40 : rows * nvec;
+  const int ni = all <= 2048 * 256 ? 1 : all <= 2 * 2048 * 256 ? 2 : 4;
+  if (nvec > 256 * ni) {
+    a.vecs = 256 * ni;
+    a.cuts = (int)((nvec + 1 + a.vecs - 1) / a.vecs);      // one piece more: a row may begin inside its first
   } else {
-    a.rows_per_block = (int)std::min<int64_t>(256, std::max<int64_t>(1, kSpan / classes));
+    a.vecs = (int)nvec;
+    a.rows_per_block = (int)std::min<int64_t>(std::min<int64_t>(256, 256 * ni / nvec), kGradNames / (a.top_k + 1));
   }
-  const int64_t blocks = a.pieces > 1 ? rows * a.pieces : (rows + a.rows_per_block - 1) / a.rows_per_block;
+  a.magic = (uint32_t)(((1u << 20) + a.vecs - 1) / a.vecs);
+  const int64_t blocks = a.cuts > 1 ? rows * a.cuts : (rows + a.rows_per_block - 1) / a.rows_per_block;
   if (rows > kMaxBlocks * 256 || blocks > kMaxBlocks) return bad_shape(op, "more rows than a launch has blocks");
   with_type(dtype, [&](auto t) {
-    if (allowed) logprob_grad<decltype(t), true><<<dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream>>>(a);
-    else logprob_grad<decltype(t), false><<<dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)hip_stream>>>(a);
+    typedef decltype(t) T;
+    const dim3 g((unsigned)blocks), b(256);
+    hipStream_t s = (hipStream_t)hip_stream;
+    if (allowed) {
+      if (ni == 1) logprob_grad<T, true, 1><<<g, b, 0, s>>>(a);
+      else if (ni == 2) logprob_grad<T, true, 2><<<g, b, 0, s>>>(a);
+      else logprob_grad<T, true, 4><<<g, b, 0, s>>>(a);
+    } else {
+      if (ni == 1) logprob_grad<T, false, 1><<<g, b, 0, s>>>(a);
+      else if (ni == 2) logprob_grad<T, false, 2><<<g, b, 0, s>>>(a);
+      else logprob_grad<T, false, 4><<<g, b, 0, s>>>(a);
+    }
   });
   return launched(op);
 } OP_CATCH

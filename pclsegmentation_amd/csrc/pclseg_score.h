@@ -544,8 +544,9 @@ __global__ __launch_bounds__(256) void logprob_join(ScoreArgs a) {
 // ---- gradient
 // With p_j = e^(x_j - lse) (0 where not allowed), H the row's entropy, gl / ge / gt the gradients that arrive:
 //   d loss / d x_j = gl [j = label] + sum_i gt_i [j = id_i] - p_j (gl + sum_i gt_i) - ge p_j (x_j - lse + H)
-// One read of the logits and one write of the gradient; a block owns whole rows (or a piece of one), writes the dense part
-// and then, behind a barrier, rewrites the few elements that the label and the alternatives name.
+// One read of the logits and one write of the gradient.  A block owns whole rows, or a piece of one; the classes that its
+// rows' labels and alternatives name, and what arrives for them, are put into LDS first, and every 16-byte piece is compared
+// with its row's names while it is in registers: no element is written twice, equal names add up.
 struct GradArgs {
   const void* x;
   int64_t rows, stride;
@@ -560,95 +561,113 @@ struct GradArgs {
   int top_k;
   void* grad;
   int64_t grad_stride;
-  int rows_per_block, span, pieces;     // a block: rows_per_block rows, or `span` columns of one row
+  // a block: 16-byte pieces of rows_per_block rows (vecs each), or vecs pieces of one row that takes `cuts` blocks
+  int rows_per_block, vecs, cuts;
+  uint32_t magic;      // ceil(2^20 / vecs): i / vecs = i magic >> 20 for i < 1024, vecs <= 1024
 };
 
-struct GradRow { float lse, w, ge, h; };   // w = gl + sum gt; h = entropy - lse; lse NaN-safe: empty rows have w = ge = 0
+struct GradRow { float lse, w, ge, h; };   // w = gl + sum gt; empty rows have all of them 0
 
 __device__ __forceinline__ float grad_dense(const GradRow& r, float x) {
-  if (x == neg_inf()) return 0.f;
   const float z = x - r.lse, p = fast_exp(z);
   // an underflowed p takes the entropy term with it (0 * -inf otherwise)
   return -p * fmaf(r.ge, fmaxf(z, -200.f) + r.h, r.w);
 }
 
-template <typename T>
-__device__ __forceinline__ GradRow grad_row(const GradArgs& a, int64_t row, int64_t& label) {
-  GradRow r;
-  const float lse = a.lse[row];
-  label = -1;
-  r.w = 0.f;
-  if (a.d_logprob) {
-    label = a.label64 ? static_cast<const int64_t*>(a.labels)[row] : static_cast<const int32_t*>(a.labels)[row];
-    if (label < 0 || label >= a.classes) label = -1;
-    if (label >= 0) r.w = a.d_logprob[row];
-  }
-  for (int k = 0; k < a.top_k; ++k) {
-    const int id = a.top_ids[row * a.top_k + k];
-    if (id >= 0 && id < a.classes) r.w += a.d_top[row * a.top_k + k];
-  }
-  r.ge = a.d_entropy ? a.d_entropy[row] : 0.f;
-  r.h = a.d_entropy ? a.entropy[row] : 0.f;
-  r.lse = lse;
-  if (lse == neg_inf()) {      // nothing is allowed: the row's gradient is 0
-    r.lse = 0.f;
-    r.w = r.ge = r.h = 0.f;
-    label = -2;
-  }
-  return r;
-}
+constexpr int kGradNames = 1024;      // names a block holds
 
-template <typename T, bool MASK>
+// NI 16-byte pieces a thread, requested before the names are looked up
+template <typename T, bool MASK, int NI>
 __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
   constexpr int VEC = Elem<T>::VEC;
-  constexpr int MAXR = 256;
-  __shared__ GradRow prm[MAXR];
-  __shared__ int lab[MAXR];
-  const int64_t row0 = a.pieces > 1 ? (int64_t)(blockIdx.x / (unsigned)a.pieces) : (int64_t)blockIdx.x * a.rows_per_block;
-  const int c0 = a.pieces > 1 ? (int)(blockIdx.x % (unsigned)a.pieces) * a.span : 0;
-  const int c1 = a.pieces > 1 ? (a.classes - c0 < a.span ? a.classes : c0 + a.span) : a.classes;
-  const int nr = a.pieces > 1 ? 1 : (int)(a.rows - row0 < a.rows_per_block ? a.rows - row0 : a.rows_per_block);
-  for (int r = threadIdx.x; r < nr; r += 256) {
-    int64_t l;
-    prm[r] = grad_row<T>(a, row0 + r, l);
-    lab[r] = (int)l;
+  __shared__ GradRow prm[256];
+  __shared__ int ids[kGradNames];
+  __shared__ float gs[kGradNames];
+  const int64_t row0 = a.cuts > 1 ? (int64_t)(blockIdx.x / (unsigned)a.cuts) : (int64_t)blockIdx.x * a.rows_per_block;
+  // the pieces of a long row begin at multiples of 16 bytes of the gradient, up to VEC - 1 elements before its first
+  const int pad = a.cuts > 1 ? (int)((reinterpret_cast<uintptr_t>(static_cast<T*>(a.grad) + row0 * a.grad_stride) & 15) / sizeof(T)) : 0;
+  const int c0 = a.cuts > 1 ? (int)(blockIdx.x % (unsigned)a.cuts) * a.vecs * VEC - pad : 0;
+  const int c1 = a.cuts > 1 && a.classes - c0 > a.vecs * VEC ? c0 + a.vecs * VEC : a.classes;
+  const int nr = a.cuts > 1 ? 1 : (int)(a.rows - row0 < a.rows_per_block ? a.rows - row0 : a.rows_per_block);
+  const int names = a.top_k + (a.d_logprob ? 1 : 0);
+  int rr[NI], cc[NI];
+  Piece<T, MASK> raw[NI];
+#pragma unroll
+  for (int n = 0; n < NI; ++n) {
+    const int i = n * 256 + threadIdx.x;
+    rr[n] = (int)(((uint32_t)i * a.magic) >> 20);
+    cc[n] = c0 + (i - rr[n] * a.vecs) * VEC;
+    if (rr[n] < nr && cc[n] >= 0 && cc[n] + VEC <= c1)
+      raw[n].load(static_cast<const T*>(a.x) + (row0 + rr[n]) * a.stride,
+                  MASK ? a.allowed + (row0 + rr[n]) * a.allowed_stride : nullptr, cc[n]);
+  }
+  for (int i = threadIdx.x; i < nr * names; i += 256) {
+    const int r = i / names, n = i - r * names;
+    const int64_t row = row0 + r;
+    int64_t id;
+    float g;
+    if (n < a.top_k) {
+      id = a.top_ids[row * a.top_k + n];
+      g = a.d_top[row * a.top_k + n];
+    } else {
+      id = a.label64 ? static_cast<const int64_t*>(a.labels)[row] : static_cast<const int32_t*>(a.labels)[row];
+      g = a.d_logprob[row];
+    }
+    const bool known = id >= 0 && id < a.classes;
+    ids[i] = known ? (int)id : -1;
+    gs[i] = known ? g : 0.f;
+  }
+  GradRow mine{0.f, 0.f, 0.f, 0.f};
+  if ((int)threadIdx.x < nr) {
+    const int64_t row = row0 + threadIdx.x;
+    mine.lse = a.lse[row];
+    if (a.d_entropy) {
+      mine.ge = a.d_entropy[row];
+      mine.h = a.entropy[row];
+    }
   }
   __syncthreads();
-  const int nvec = (c1 - c0 + VEC - 1) / VEC;
-  for (int i = threadIdx.x; i < nr * nvec; i += 256) {
-    const int r = i / nvec, c = c0 + (i - r * nvec) * VEC;
-    const GradRow p = prm[r];
-    const T* src = static_cast<const T*>(a.x) + (row0 + r) * a.stride;
-    const uint8_t* mask = MASK ? a.allowed + (row0 + r) * a.allowed_stride : nullptr;
-    T* dst = static_cast<T*>(a.grad) + (row0 + r) * a.grad_stride;
-    float f[VEC];
-    load_tail<T, MASK>(src, mask, c, c1, f);
+  if ((int)threadIdx.x < nr) {
+    const int n0 = threadIdx.x * names;
+    const bool empty = mine.lse == neg_inf();      // nothing is allowed: the row's gradient is 0
+    if (empty) mine = GradRow{0.f, 0.f, 0.f, 0.f};
+    for (int n = n0; n < n0 + names; ++n) {
+      if (empty) ids[n] = -1;
+      else mine.w += gs[n];
+    }
+    prm[threadIdx.x] = mine;
+  }
+  __syncthreads();
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = grad_dense(p, f[e]);
-    if (c + VEC <= c1) {
-      store16(dst + c, pack16<T>(f));
+  for (int n = 0; n < NI; ++n) {
+    const int r = rr[n], c = cc[n];
+    if (r >= nr || c >= c1) continue;
+    const GradRow p = prm[r];
+    float x[VEC], f[VEC];
+    const bool inside = c >= 0 && c + VEC <= c1;
+    if (inside) raw[n].expand(x);
+    else load_tail<T, MASK>(static_cast<const T*>(a.x) + (row0 + r) * a.stride,
+                            MASK ? a.allowed + (row0 + r) * a.allowed_stride : nullptr, c, c1, x);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = grad_dense(p, x[e]);
+    for (int k = r * names; k < (r + 1) * names; ++k) {
+      const int d = ids[k] - c;
+      if ((unsigned)d < (unsigned)VEC) {
+        const float g = gs[k];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] += e == d ? g : 0.f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = x[e] == neg_inf() ? 0.f : f[e];
+    T* dst = static_cast<T*>(a.grad) + (row0 + r) * a.grad_stride + c;
+    if (inside) {
+      store16(dst, pack16<T>(f));
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
-        if (c + e < c1) dst[c + e] = Elem<T>::from(f[e]);
+        if (c + e >= 0 && c + e < c1) dst[e] = Elem<T>::from(f[e]);
     }
-  }
-  __syncthreads();      // the block's own stores are complete: the named elements are written over them
-  const int names = a.top_k + 1;
-  for (int i = threadIdx.x; i < nr * names; i += 256) {
-    const int r = i / names, k = i - r * names;
-    const int64_t row = row0 + r;
-    const int64_t id = k == 0 ? lab[r] : (lab[r] == -2 ? -1 : a.top_ids[row * a.top_k + k - 1]);
-    if (id < c0 || id >= c1) continue;
-    if (MASK && !a.allowed[row * a.allowed_stride + id]) continue;
-    const float x = Elem<T>::load(static_cast<const T*>(a.x) + row * a.stride + id);
-    if (x == neg_inf()) continue;
-    // every name of this element adds up here: threads that share an element write the same sum
-    float g = grad_dense(prm[r], x);
-    if (lab[r] == id) g += a.d_logprob[row];
-    for (int j = 0; j < a.top_k; ++j)
-      if (a.top_ids[row * a.top_k + j] == id) g += a.d_top[row * a.top_k + j];
-    static_cast<T*>(a.grad)[row * a.grad_stride + id] = Elem<T>::from(g);
   }
 }
 

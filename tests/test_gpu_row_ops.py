@@ -278,7 +278,7 @@ def labels_for(rows, v, seed, dtype=torch.int32):
 
 SCORES = [(1, 1, 1), (5, 2, 3), (300, 3, 2), (257, 8, 8), (1000, 20, 3), (513, 31, 5), (70, 32, 32), (65, 33, 2), (40, 64, 64), (33, 100, 4),
           (31, 256, 20), (17, 257, 3), (9, 511, 32), (10, 513, 1), (6, 1031, 64), (5, 2048, 20), (7, 2049, 20), (3, 4097, 5), (4, 8193, 64),
-          (2, 30001, 20), (600, 2500, 3), (1, 131072, 20), (3, 131071, 32), (1, 300000, 64), (1000, 5000, 0), (2, 9000, 0), (50, 77, 0)]
+          (2, 30001, 20), (600, 2500, 3), (1, 131072, 20), (3, 131071, 32), (1, 300000, 64), (3, 131073, 7), (2, 1000003, 20), (1000, 5000, 0), (2100, 4099, 6), (2100, 2049, 0), (2, 9000, 0), (50, 77, 0)]
 
 
 @pytest.mark.parametrize("rows,v,top_k", SCORES)
@@ -397,7 +397,8 @@ def grad64(ref, labels, lse, entropy, d_lp, d_h, ids, d_top, dtype):
 
 
 @pytest.mark.parametrize("rows,v,top_k", [(1, 1, 1), (700, 20, 3), (300, 3, 2), (9, 33, 40), (64, 100, 5), (33, 1031, 32), (5, 4099, 20),
-                                          (3, 8192, 2), (3, 8193, 3), (2, 50001, 20), (1, 131072, 64), (2000, 2, 1)])
+                                          (3, 8192, 2), (3, 8193, 3), (2, 50001, 20), (1, 131072, 64), (2000, 2, 1), (300, 4099, 2), (40001, 20, 3),
+                                          (9000, 129, 1)])
 @pytest.mark.parametrize("parts", ["lp", "h", "top", "lp+h+top"])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_label_logprobs_grad(cuda, rows, v, top_k, parts, dtype):

@@ -73,10 +73,10 @@ def test_workspace_sizes():
   assert lib.pclseg_op_linear_i8_workspace(4, 7, 12289, ctypes.byref(size)) == 0 and size.value >= 4 * 12416
   assert lib.pclseg_op_linear_i8_workspace(5, 7, 0, ctypes.byref(size)) == -2
   assert lib.pclseg_op_linear_i8_workspace(5, 7, 8, None) == -1
-  for rows, classes in ((1, 20), (1, 2048), (1 << 20, 50000)):
+  for rows, classes in ((1, 20), (1, 2048), (1, 32768), (1 << 20, 50000)):
     assert lib.pclseg_op_label_logprobs_workspace(rows, classes, 5, ctypes.byref(size)) == 0 and size.value == 0
-  assert lib.pclseg_op_label_logprobs_workspace(1, 131072, 5, ctypes.byref(size)) == 0 and size.value > 0
-  assert lib.pclseg_op_label_logprobs_workspace(0, 131072, 5, ctypes.byref(size)) == 0 and size.value == 0
+  assert lib.pclseg_op_label_logprobs_workspace(1, 1 << 20, 5, ctypes.byref(size)) == 0 and size.value > 0
+  assert lib.pclseg_op_label_logprobs_workspace(0, 1 << 20, 5, ctypes.byref(size)) == 0 and size.value == 0
   assert lib.pclseg_op_label_logprobs_workspace(1, 0, 5, ctypes.byref(size)) == -2
   assert lib.pclseg_op_label_logprobs_workspace(1, 5, 65, ctypes.byref(size)) == -1
 
@@ -90,7 +90,7 @@ SCORE = dict(logits=P, dtype=0, rows=2, classes=4, stride=4, labels=P, label_byt
   (dict(stride=3), -2, "stride"), (dict(top_k=65), -1, "top_k"), (dict(top_k=-1), -1, "top_k"), (dict(logits=None), -1, "NULL"),
   (dict(label_bytes=2), -1, "int32"), (dict(labels=P + 2), -1, "misaligned"), (dict(labels=None), -1, "labels"),
   (dict(top_k=2), -1, "top_ids"), (dict(allowed=P, allowed_stride=3), -2, "mask"), (dict(logits=P + 2), -1, "misaligned"),
-  (dict(classes=131072, stride=131072, rows=1), -1, "workspace"),
+  (dict(classes=1 << 20, stride=1 << 20, rows=1), -1, "workspace"),
 ])
 def test_label_logprobs_refuses(change, code, word):
   _refused("pclseg_op_label_logprobs", list({**SCORE, **change}.values()), code, word)
