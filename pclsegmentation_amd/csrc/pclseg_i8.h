@@ -58,15 +58,19 @@ struct RowScale { float pre, s, inv, half; };
 __device__ __forceinline__ RowScale row_scale(float amax) {
   RowScale r;
   r.pre = amax < 0x1p-60f ? 0x1p64f : 1.f;
-  r.s = amax * r.pre / 127.f;
-  r.inv = r.s > 0.f ? 1.f / r.s : 0.f;
+  // amax / 127, rounded once: the quotient by the rounded reciprocal, corrected by its exact remainder (equal to the IEEE
+  // division for every mantissa)
+  constexpr float c = 1.f / 127.f;
+  const float a = amax * r.pre, q = a * c;
+  r.s = fmaf(fmaf(-127.f, q, a), c, q);
+  r.inv = r.s > 0.f ? __builtin_amdgcn_rcpf(r.s) : 0.f;      // one unit off: 2^-16 of a step in a code's quotient
   r.half = 0.5f * r.s;
   return r;
 }
 constexpr float kRound = 12582912.f;      // 1.5 * 2^23: x + kRound rounds x to an integer, whose code is the sum's low byte
 // The code of x has to be the integer nearest to the exact quotient x / s.  u = x * (1/s) + kRound, one fma, holds the nearest
-// integer or, within 2^-17 of a half step, its neighbour; the remainder t = x - q s, exact in one fma, says which: below half
-// a step the code stands, otherwise (rare: some lane of the wave, in one of 2^17 elements) `nearest` decides.
+// integer or, within 2^-16 of a half step, its neighbour; the remainder t = x - q s, exact in one fma, says which: below half
+// a step the code stands, otherwise (rare: one of 2^16 elements) `nearest` decides.
 __device__ __forceinline__ float quant(float x, const RowScale& r, float& worst) {
   const float u = fmaf(x, r.inv, kRound), t = fmaf(-(u - kRound), r.s, x);
   worst = fmaxf(worst, fabsf(t));
@@ -91,16 +95,28 @@ template <typename T> struct Eight {
 #pragma unroll
     for (int h = 0; h < N; ++h) v[h] = load16(p + h * Elem<T>::VEC);
   }
-  __device__ __forceinline__ void load(const T* row, int c, int cols) {      // 0 behind the row's end
-    if (c + 8 <= cols) {
-      load(row + c);
-    } else {
+  // elements [c, c + 8) of a row in two steps, so that all of a lane's loads are in flight before the first is waited for:
+  // request() reads 16 or 32 bytes inside the row whatever c is, settle() puts 0 behind the row's end
+  __device__ __forceinline__ void request(const T* row, int c, int cols) {
+    if (cols >= 8) load(row + (c + 8 <= cols ? c : 0));
+  }
+  __device__ __forceinline__ void settle(const T* row, int c, int cols) {
+    if (c + 8 > cols) {
       float f[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = c + e < cols ? Elem<T>::load(row + c + e) : 0.f;
+      for (int e = 0; e < 8; ++e) f[e] = 0.f;
+      if (c < cols) {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (c + e < cols) f[e] = Elem<T>::load(row + c + e);
+      }
 #pragma unroll
       for (int h = 0; h < N; ++h) v[h] = pack16<T>(f + h * Elem<T>::VEC);
     }
+  }
+  __device__ __forceinline__ void load(const T* row, int c, int cols) {
+    request(row, c, cols);
+    settle(row, c, cols);
   }
   __device__ __forceinline__ void add_to(RowMax<T>& m) const {
 #pragma unroll
@@ -140,12 +156,11 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a) {
   Eight<T> x[NV];
   RowMax<T> mx;
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {      // stretches inside the row for all lanes first: a uniform test, all loads in flight
-    if ((v + 1) * 8 * G <= a.cols) x[v].load(src + (v * G + g) * 8);
-  }
+  for (int v = 0; v < NV; ++v)
+    if (v < nv) x[v].request(src, (v * G + g) * 8, a.cols);
 #pragma unroll
   for (int v = 0; v < NV; ++v)
-    if (v < nv && (v + 1) * 8 * G > a.cols) x[v].load(src, (v * G + g) * 8, a.cols);
+    if (v < nv) x[v].settle(src, (v * G + g) * 8, a.cols);
 #pragma unroll
   for (int v = 0; v < NV; ++v)
     if (v < nv) x[v].add_to(mx);
@@ -280,80 +295,92 @@ __global__ __launch_bounds__(NW * 64) void i8_few_rows(I8Args p) {
   }
 }
 
-// ---- one to four rows: quantisation and product in one launch
-// Every block quantises all rows again (m k elements, 8 k of them a thread's share at k = 4096 and one row) while its first
-// weights are on their way; a launch of its own would cost more than the whole product.  Codes and scales of the rows stay
-// in LDS.
-constexpr int kFusedRows = 4, kFusedBytes = 49152;      // rows, and bytes of codes, a block takes
-template <typename T, typename Y, int NW>
-__global__ __launch_bounds__(NW * 64) void i8_fused_rows(I8Args p, const T* x, int64_t x_stride, int k) {
+// ---- up to 32 short rows: quantisation and product in one launch
+// Every block quantises all rows again (from the L2) while its first weights are on their way, where a launch of its own
+// costs 3 us on the device and as much on the host.  The rows are cut into items of 512 elements, eight a lane; a wave takes
+// up to eight items and holds them in registers between the maximum and the codes.  Codes and scales stay in LDS.  MT tiles
+// of 16 rows share a weight fragment.
+constexpr int kFusedRows = 32, kFusedItems = 64;
+template <typename T, typename Y, int MT>
+__global__ __launch_bounds__(512) void i8_fused_rows(I8Args p, const T* x, int64_t x_stride, int k) {
+  constexpr int NW = 8, D = 8;
   extern __shared__ __attribute__((aligned(16))) int8_t codes[];      // [m][kp]
-  __shared__ int part[NW][256];
-  __shared__ uint32_t tops[kFusedRows][NW];
+  __shared__ int part[NW][MT][256];
+  __shared__ uint32_t tops[16 * MT];
+  __shared__ float scales[16 * MT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, ko = (lane >> 4) * 16;
   const int n0 = blockIdx.x * 16, m = (int)p.m;
   const int jn = n0 + r < p.n ? n0 + r : p.n - 1;
   const int steps = p.kp / 64, s0 = steps * wave / NW, s1 = steps * (wave + 1) / NW;      // a wave's stretch of k
   const int8_t* wb = p.b + (int64_t)jn * p.ldb + ko;
-  constexpr int D = 8;
   i32x4 w[D];
 #pragma unroll
   for (int u = 0; u < D; ++u) w[u] = *reinterpret_cast<const i32x4*>(wb + (int64_t)(s0 + u < s1 ? s0 + u : steps - 1) * 64);
-  for (int i = 0; i < m; ++i) {
-    RowMax<T> mx;
-    for (int c = threadIdx.x * 8; c < k; c += NW * 512) {
-      Eight<T> e;
-      e.load(x + i * x_stride, c, k);
-      e.add_to(mx);
-    }
-    const uint32_t top = group_reduce<64>(mx.bits(), [](uint32_t a, uint32_t b) { return max(a, b); });
-    if (lane == 0) tops[i][wave] = top;
+  constexpr int IW = kFusedItems / NW;
+  const int cuts = (p.kp + 511) / 512, items = m * cuts;
+  Eight<T> e[IW];
+#pragma unroll
+  for (int h = 0; h < IW; ++h) {
+    const int it = h * NW + wave, row = it / cuts;
+    if (it < items) e[h].request(x + row * x_stride, (it - row * cuts) * 512 + lane * 8, k);
   }
+  if ((int)threadIdx.x < m) tops[threadIdx.x] = 0;
   __syncthreads();
-  float sa[kFusedRows];
 #pragma unroll
-  for (int i = 0; i < kFusedRows; ++i) {
-    if (i >= m) break;
-    uint32_t top = 0;
-#pragma unroll
-    for (int v = 0; v < NW; ++v) top = max(top, tops[i][v]);
-    const bool finite = top < RowMax<T>::kInf;
-    const RowScale q = row_scale(finite ? RowMax<T>::value(top) : 0.f);
-    sa[i] = finite ? q.s / q.pre : __builtin_nanf("");
-    for (int c = threadIdx.x * 8; c < p.kp; c += NW * 512) {
-      u32x2 o{0u, 0u};
-      if (c < k && q.inv != 0.f) {
-        Eight<T> e;
-        e.load(x + i * x_stride, c, k);
-        o = e.codes(q);
-      }
-      *reinterpret_cast<u32x2*>(codes + i * p.kp + c) = o;
+  for (int h = 0; h < IW; ++h) {
+    const int it = h * NW + wave, row = it / cuts;
+    if (it < items) {
+      e[h].settle(x + row * x_stride, (it - row * cuts) * 512 + lane * 8, k);
+      RowMax<T> mx;
+      e[h].add_to(mx);
+      const uint32_t top = group_reduce<64>(mx.bits(), [](uint32_t a, uint32_t b) { return max(a, b); });
+      if (lane == 0) atomicMax(&tops[row], top);
     }
   }
   __syncthreads();
-  i32x4 acc{0, 0, 0, 0};
-  const int8_t* xa = codes + (r < m ? r : 0) * p.kp + ko;      // rows behind m are not stored
+#pragma unroll
+  for (int h = 0; h < IW; ++h) {
+    const int it = h * NW + wave, row = it / cuts, c = (it - row * cuts) * 512 + lane * 8;
+    if (it < items) {
+      const uint32_t top = tops[row];
+      const bool finite = top < RowMax<T>::kInf;
+      const RowScale q = row_scale(finite ? RowMax<T>::value(top) : 0.f);
+      if (c == 0) scales[row] = finite ? q.s / q.pre : __builtin_nanf("");
+      if (c < p.kp) *reinterpret_cast<u32x2*>(codes + row * p.kp + c) = q.inv != 0.f ? e[h].codes(q) : u32x2{0u, 0u};
+    }
+  }
+  __syncthreads();
+  i32x4 acc[MT];
+  const int8_t* xa[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    acc[t] = i32x4{0, 0, 0, 0};
+    xa[t] = codes + (t * 16 + r < m ? t * 16 + r : 0) * p.kp + ko;      // rows behind m are not stored
+  }
   for (int s = s0; s < s1; s += D) {
 #pragma unroll
     for (int u = 0; u < D; ++u) {
       if (s + u < s1) {
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const i32x4*>(xa + (s + u) * 64), w[u], acc, 0, 0, 0);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const i32x4*>(xa[t] + (s + u) * 64), w[u], acc[t], 0, 0, 0);
         if (s + u + D < s1) w[u] = *reinterpret_cast<const i32x4*>(wb + (int64_t)(s + u + D) * 64);
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) part[wave][((lane >> 4) * 4 + i) * 16 + r] = acc[i];
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[wave][t][((lane >> 4) * 4 + i) * 16 + r] = acc[t][i];
   __syncthreads();
   for (int o = threadIdx.x; o < m * 16; o += NW * 64) {
     const int i = o / 16, j = n0 + (o & 15);
     if (j >= p.n) continue;
     int v = 0;
 #pragma unroll
-    for (int u = 0; u < NW; ++u) v += part[u][o];
-    const float s = i == 0 ? sa[0] : i == 1 ? sa[1] : i == 2 ? sa[2] : sa[3];
-    i8_store<Y>(p, i, j, v, s, p.sb[j], p.bias ? p.bias[j] : 0.f);
+    for (int u = 0; u < NW; ++u) v += part[u][o >> 8][o & 255];
+    i8_store<Y>(p, i, j, v, scales[i], p.sb[j], p.bias ? p.bias[j] : 0.f);
   }
 }
 

@@ -85,8 +85,8 @@ int matmul(const char* op, const I8Args& p, int dtype, hipStream_t s) {
   return launched(op);
 }
 
-// one to four rows whose codes fit into a block's LDS: one launch, no workspace (see i8_fused_rows)
-bool fused_rows(int64_t m, int64_t k) { return m <= kFusedRows && m * row_bytes(k) <= kFusedBytes; }
+// up to 32 rows of together 64 items of 512 elements: one launch, no workspace (see i8_fused_rows)
+bool fused_rows(int64_t m, int64_t k) { return m <= kFusedRows && m * ((row_bytes(k) + 511) / 512) <= kFusedItems; }
 size_t linear_workspace(int64_t m, int64_t k) {
   return fused_rows(m, k) ? 0 : (size_t)m * ((size_t)row_bytes(k) + sizeof(float));
 }
@@ -232,8 +232,12 @@ int pclseg_op_linear_i8(const void* x, int dtype, int64_t x_stride, const int8_t
     with_type(dtype, [&](auto t) {
       with_type(y_dtype, [&](auto u) {
         typedef decltype(t) T;
-        i8_fused_rows<T, decltype(u), 8><<<dim3((unsigned)((n + 15) / 16)), dim3(512), (size_t)(m * ld), (hipStream_t)hip_stream>>>(
-            p, static_cast<const T*>(x), x_stride, (int)k);
+        typedef decltype(u) Y;
+        const dim3 g((unsigned)((n + 15) / 16));
+        const size_t lds = (size_t)(m * ld);
+        hipStream_t s = (hipStream_t)hip_stream;
+        if (m <= 16) i8_fused_rows<T, Y, 1><<<g, dim3(512), lds, s>>>(p, static_cast<const T*>(x), x_stride, (int)k);
+        else i8_fused_rows<T, Y, 2><<<g, dim3(512), lds, s>>>(p, static_cast<const T*>(x), x_stride, (int)k);
       });
     });
     return launched(op);

@@ -252,9 +252,9 @@ def label_logprobs(logits, labels=None, top_k=0, allowed=None):
   if allowed is not None:
     allowed, mstride = _mask(allowed, logits)
   size = _workspace("pclseg_op_label_logprobs_workspace", m, v, top_k)
-  logprob = torch.empty(shape, dtype=torch.float32, device=dev) if labels is not None else None
-  entropy = torch.empty(shape, dtype=torch.float32, device=dev)
-  lse = torch.empty(shape, dtype=torch.float32, device=dev)
+  logprob, entropy, lse = torch.empty((3,) + shape, dtype=torch.float32, device=dev).unbind(0)
+  if labels is None:
+    logprob = None
   ids = torch.empty(shape + (top_k,), dtype=torch.int32, device=dev) if top_k else None
   tops = torch.empty(shape + (top_k,), dtype=torch.float32, device=dev) if top_k else None
   if m:

@@ -148,8 +148,10 @@ def test_matmul_i8_sums_are_exact(cuda):
 
 
 @pytest.mark.parametrize("m,k,n", [(1, 333, 260), (7, 333, 260), (48, 333, 260), (100, 333, 260), (600, 333, 260),
-                                   # up to four rows take one launch, as long as their codes fit into a block's LDS
-                                   (1, 1, 1), (2, 64, 5), (3, 65, 16), (4, 4097, 33), (4, 12288, 20), (4, 12289, 20), (1, 49153, 9)])
+                                   # up to 32 rows of together 64 stretches of 512 columns take one launch
+                                   (1, 1, 1), (2, 64, 5), (3, 65, 16), (4, 4097, 33), (4, 8192, 20), (4, 8193, 20), (1, 32768, 40),
+                                   (1, 32769, 9), (5, 1, 3), (16, 2048, 7), (16, 2049, 7), (17, 1536, 40), (17, 1537, 40), (31, 1000, 300),
+                                   (32, 1024, 65), (32, 1025, 65), (33, 64, 20)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear_i8(cuda, m, k, n, dtype):
   x = rnd(m, m, k).to(dtype)

@@ -53,13 +53,13 @@ def test_matmul_i8_refuses(change, code, word):
   _refused("pclseg_op_matmul_i8", list({**MATMUL, **change}.values()), code, word)
 
 
-LINEAR = dict(x=P, dtype=0, x_stride=8, weight=P, weight_scale=P, m=5, n=3, k=8, bias=None, act=0, residual=None,
-              residual_stride=0, y=P, y_stride=3, y_dtype=1, workspace=P, workspace_bytes=5 * 68, stream=None)
+LINEAR = dict(x=P, dtype=0, x_stride=8, weight=P, weight_scale=P, m=33, n=3, k=8, bias=None, act=0, residual=None,
+              residual_stride=0, y=P, y_stride=3, y_dtype=1, workspace=P, workspace_bytes=33 * 68, stream=None)
 
 
 @pytest.mark.parametrize("change,code,word", [
   (dict(dtype=7), -1, "dtype"), (dict(y_dtype=7), -1, "dtype"), (dict(x_stride=7), -2, "stride"), (dict(x=None), -1, "NULL"),
-  (dict(workspace=None), -1, "workspace"), (dict(workspace_bytes=5 * 68 - 1), -1, "workspace"), (dict(workspace=P + 8), -1, "misaligned"),
+  (dict(workspace=None), -1, "workspace"), (dict(workspace_bytes=33 * 68 - 1), -1, "workspace"), (dict(workspace=P + 8), -1, "misaligned"),
   (dict(m=1 << 31), -2, "m must"), (dict(x=P + 1), -1, "misaligned"),
 ])
 def test_linear_i8_refuses(change, code, word):
@@ -68,9 +68,9 @@ def test_linear_i8_refuses(change, code, word):
 
 def test_workspace_sizes():
   lib, size = E.load_library(), ctypes.c_size_t()
-  assert lib.pclseg_op_linear_i8_workspace(5, 7, 65, ctypes.byref(size)) == 0 and size.value >= 5 * (128 + 4)
-  assert lib.pclseg_op_linear_i8_workspace(4, 7, 12288, ctypes.byref(size)) == 0 and size.value == 0      # one launch
-  assert lib.pclseg_op_linear_i8_workspace(4, 7, 12289, ctypes.byref(size)) == 0 and size.value >= 4 * 12416
+  assert lib.pclseg_op_linear_i8_workspace(33, 7, 65, ctypes.byref(size)) == 0 and size.value >= 33 * (128 + 4)
+  assert lib.pclseg_op_linear_i8_workspace(4, 7, 8192, ctypes.byref(size)) == 0 and size.value == 0      # one launch
+  assert lib.pclseg_op_linear_i8_workspace(4, 7, 8193, ctypes.byref(size)) == 0 and size.value >= 4 * 8320
   assert lib.pclseg_op_linear_i8_workspace(5, 7, 0, ctypes.byref(size)) == -2
   assert lib.pclseg_op_linear_i8_workspace(5, 7, 8, None) == -1
   for rows, classes in ((1, 20), (1, 2048), (1, 32768), (1 << 20, 50000)):
