@@ -1,7 +1,8 @@
 """pclsegmentation_amd — MI355X-native forward-pass engine for SqueezeSegV2 / Darknet-21/53
 LiDAR range-image segmentation, behind the reference's own Python surface
 (configs, load_model_config, ``model([lidar, mask]) -> (probabilities, predictions)``,
-the inference CLI).  Everything numerical runs in libpclseg.so (hand-written HIP, gfx950)."""
+the inference CLI).  Row operators on device tensors (8-bit linear layer, label log probabilities and their gradient) are in
+``pclsegmentation_amd.ops``.  Everything numerical runs in libpclseg.so (hand-written HIP, gfx950)."""
 import json as _json
 
 import numpy as _np

@@ -5,7 +5,8 @@ exact int64 counts) all stay on the device, only the final [NC,NC] matrix comes 
 
   python -m pclsegmentation_amd.eval -d <dataset dir> -i val -m squeezesegv2 -n squeezesegv2 -p model.npz
 
-Same flags as the reference (``-d/-i/-t/-p/-m/-n``).  The reference reads a TFRecord file that
+Same flags as the reference (``-d/-i/-t/-p/-m/-n``), plus ``--likelihood``: the mean negative log probability of the labels
+and the mean entropy of the predictions.  The reference reads a TFRecord file that
 its DataLoader writes from ``<data_path>/<image_set>/*.npy``; here the ``.npy`` scans
 ([H,W,6]: x,y,z,intensity,depth,label) are read directly — the TFRecord pipeline is training
 infrastructure and out of scope.  Like the reference (data_loader/data_loader.py:173-180) labels
@@ -87,6 +88,48 @@ class MeanIoU:
     return float(np.where(valid, tp / np.where(valid, denom, 1), 0.0).sum() / valid.sum())
 
 
+class LabelLikelihood:
+  """How well the logits' distribution fits the labels: mean negative log probability of the label and mean entropy
+  of the prediction, in nats, over the pixels that carry a label.  The class ``none_index`` (no label, not predicted) takes no
+  part: pixels labelled with it are not counted and it gets no probability.  Everything stays on the device until
+  ``result()``."""
+
+  def __init__(self, num_classes, none_index=None, device=0, name="LabelLikelihood"):
+    import torch
+    self.num_classes = int(num_classes)
+    self.none_index = none_index
+    self.name = name
+    self._dev = _engine.torch_device(device)
+    self._allowed = None
+    if none_index is not None:
+      self._allowed = torch.ones(self.num_classes, dtype=torch.bool, device=self._dev)
+      self._allowed[none_index] = False
+    self._sums = torch.zeros(3, dtype=torch.float64, device=self._dev)     # -log p, entropy, pixels
+
+  def reset_state(self):
+    self._sums.zero_()
+
+  def update_state(self, label, logits):
+    """label [...], logits [..., num_classes]: host arrays or device tensors."""
+    import torch
+    from . import ops as _ops
+    lab = torch.as_tensor(np.asarray(label) if not hasattr(label, "is_cuda") else label).to(self._dev, dtype=torch.int32)
+    x = torch.as_tensor(np.asarray(logits) if not hasattr(logits, "is_cuda") else logits).to(self._dev)
+    if x.shape[-1:] != (self.num_classes,) or lab.shape != x.shape[:-1]:
+      raise ValueError("labels %s do not match logits %s of %d classes" % (tuple(lab.shape), tuple(x.shape), self.num_classes))
+    counted = (lab >= 0) & (lab < self.num_classes)
+    if self.none_index is not None:
+      counted &= lab != self.none_index
+    out = _ops.label_logprobs(x, torch.where(counted, lab, torch.full_like(lab, -1)), allowed=self._allowed)
+    self._sums += torch.stack([-out.logprob.double().sum(), torch.where(counted, out.entropy, 0).double().sum(),
+                               counted.sum().double()])
+
+  def result(self):
+    """-> (mean -log p(label), mean entropy), 0 without a counted pixel."""
+    nll, entropy, n = self._sums.tolist()
+    return (nll / n, entropy / n) if n else (0.0, 0.0)
+
+
 def masked_labels(samples, mask, none_index):
   """The reference's ``label[~mask] = config.CLASSES.index("None")`` (eval.py / inference.py:65-66,
   data_loader/data_loader.py:176-180) on the device: samples [N,H,W,6] float32 (channel 5 = label),
@@ -108,14 +151,18 @@ def evaluation(arg):
     raise SystemExit("no scans under %s" % os.path.join(arg.data_path, arg.image_set))
   none_index = config.CLASSES.index("None")
   miou_tracker = MeanIoU(num_classes=config.NUM_CLASS, name="MeanIoU")
+  likelihood = LabelLikelihood(config.NUM_CLASS, none_index, device=model.device) if arg.likelihood else None
   print("Performing Evaluation")
   import torch
   dev = _engine.torch_device(model.device)
   for b0 in range(0, len(files), arg.batch):
     samples = torch.from_numpy(np.stack([np.load(f).astype(np.float32) for f in files[b0:b0 + arg.batch]])).to(dev)
-    predictions, mask = model.predict_raw(samples[..., :5], return_mask=True)       # device tensors
+    out = model.predict_raw(samples[..., :5], return_mask=True, return_logits=arg.likelihood)       # device tensors
+    predictions, mask = out[0], out[1]
     label = masked_labels(samples, mask, none_index)
     miou_tracker.update_state(label, predictions)
+    if likelihood:
+      likelihood.update_state(label, out[2])
   if miou_tracker.ignored:
     print("warning: %d pixels carry a label outside [0, %d) and were not counted"
           % (miou_tracker.ignored, config.NUM_CLASS))
@@ -127,6 +174,8 @@ def evaluation(arg):
     print("Precision: " + str(precision[i]))
     print("")
   print("MIoU: {} ".format(miou_tracker.result()))
+  if likelihood:
+    print("NLL: {}  Entropy: {} ".format(*likelihood.result()))
   return iou, recall, precision, miou_tracker.result()
 
 
@@ -142,6 +191,8 @@ def main(argv=None):
   parser.add_argument("-n", "--config", type=str, default="squeezesegv2",
                       help="Which configuration: `squeezesegv2`, `squeezesegv2kitti`, ...")
   parser.add_argument("--batch", type=int, default=32)
+  parser.add_argument("--likelihood", action="store_true",
+                      help="also print the mean negative log probability of the labels and the mean entropy (nats)")
   return evaluation(parser.parse_args(argv))
 
 

@@ -162,9 +162,10 @@ class PCLSegmentationNetwork:
     (lidar_input, lidar_mask), _, _ = data
     return self.call([lidar_input, lidar_mask], training=False)
 
-  def predict_raw(self, scans, return_mask=False):
+  def predict_raw(self, scans, return_mask=False, return_logits=False):
     """Raw scans [N,H,W,5] (x,y,z,intensity,depth) -> predictions, with the reference's
-    caller-side pre-processing (inference.py:50-62) done on the device."""
+    caller-side pre-processing (inference.py:50-62) done on the device; optionally the mask and the
+    logits [N,H,W,NUM_CLASS] behind them, in this order."""
     if _is_torch(scans) and _engine.on_device(scans):
       import torch
       scans = scans.float().contiguous()
@@ -173,15 +174,20 @@ class PCLSegmentationNetwork:
       eng.set_stream(_engine.stream_handle(scans.device))
       preds = torch.empty((n, h, w), dtype=torch.int32, device=scans.device)
       mask = torch.empty((n, h, w), dtype=torch.uint8, device=scans.device) if return_mask else None
-      eng.forward_raw(scans, n, preds, None, None, mask, mem=_engine.MEM_DEVICE)
-      return (preds, mask) if return_mask else preds
+      logits = (torch.empty((n, h, w, self.NUM_CLASS), dtype=torch.float32, device=scans.device)
+                if return_logits else None)
+      eng.forward_raw(scans, n, preds, None, logits, mask, mem=_engine.MEM_DEVICE)
+      out = (preds,) + ((mask,) if return_mask else ()) + ((logits,) if return_logits else ())
+      return out if len(out) > 1 else preds
     scans = np.ascontiguousarray(np.asarray(scans)[..., :5], dtype=np.float32)
     n, h, w, _ = scans.shape
     eng = self.engine(h, w)
     preds = np.empty((n, h, w), np.int32)
     mask = np.empty((n, h, w), np.uint8) if return_mask else None
-    eng.forward_raw(scans, n, preds, None, None, mask, mem=_engine.MEM_HOST)
-    return (_eager(preds), mask.astype(bool)) if return_mask else _eager(preds)
+    logits = np.empty((n, h, w, self.NUM_CLASS), np.float32) if return_logits else None
+    eng.forward_raw(scans, n, preds, None, logits, mask, mem=_engine.MEM_HOST)
+    out = (_eager(preds),) + ((mask.astype(bool),) if return_mask else ()) + ((_eager(logits),) if return_logits else ())
+    return out if len(out) > 1 else out[0]
 
   def get_config(self):
     return {"mc": self.mc}

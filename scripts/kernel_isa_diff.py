@@ -15,6 +15,7 @@ import tempfile
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 FILES = ["pclsegmentation_amd/csrc/pclseg_kernels.h", "pclsegmentation_amd/csrc/pclseg_api.hip",
          "pclsegmentation_amd/csrc/pclseg_graph.h", "include/pclseg.h"]
+LATER = ["pclsegmentation_amd/csrc/pclseg_status.h"]      # a header that older revisions do not have
 # the device side only, as assembly (the Makefile's flags; the host compile adds nothing to compare)
 HIPCC = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-Wno-unused-function", "--cuda-device-only", "-S"]
 
@@ -54,10 +55,12 @@ def manifest_of_revision(rev):
   """{mangled kernel name: hash of its instruction stream} of the default build of a git revision."""
   with tempfile.TemporaryDirectory() as tmp:
     old = os.path.join(tmp, "old_src")
-    for f in FILES:
+    for f in FILES + LATER:
       os.makedirs(os.path.dirname(os.path.join(old, f)), exist_ok=True)
-      with open(os.path.join(old, f), "wb") as fh:
-        fh.write(subprocess.check_output(["git", "show", "%s:%s" % (rev, f)], cwd=ROOT))
+      r = subprocess.run(["git", "show", "%s:%s" % (rev, f)], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.DEVNULL, check=f in FILES)
+      if r.returncode == 0:
+        with open(os.path.join(old, f), "wb") as fh:
+          fh.write(r.stdout)
     return stream_hashes(kernels(build(old, os.path.join(tmp, "a"), [])))
 
 
@@ -75,10 +78,12 @@ def main():
   rev, extra = sys.argv[1], sys.argv[2:]
   with tempfile.TemporaryDirectory() as tmp:
     old = os.path.join(tmp, "old_src")
-    for f in FILES:
+    for f in FILES + LATER:
       os.makedirs(os.path.dirname(os.path.join(old, f)), exist_ok=True)
-      with open(os.path.join(old, f), "wb") as fh:
-        fh.write(subprocess.check_output(["git", "show", "%s:%s" % (rev, f)], cwd=ROOT))
+      r = subprocess.run(["git", "show", "%s:%s" % (rev, f)], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.DEVNULL, check=f in FILES)
+      if r.returncode == 0:
+        with open(os.path.join(old, f), "wb") as fh:
+          fh.write(r.stdout)
     a = kernels(build(old, os.path.join(tmp, "a"), []))
     b = kernels(build(ROOT, os.path.join(tmp, "b"), extra))
   differ = sorted(k for k in a if k in b and a[k] != b[k])

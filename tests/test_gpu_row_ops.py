@@ -579,3 +579,60 @@ def test_only_the_rows_are_written(cuda):
                                               d.data_ptr(), None, None, None, 0, grad.data_ptr(), v + 5, stream))
     assert (grad[m:] == 5).all() and (grad[:, v:] == 5).all()
     assert torch.equal(grad[:m, :v], ops.label_logprobs_grad(logits, labels, fwd.lse, d_logprob=d))
+
+
+# ---------------------------------------------------------------------------------------------- in the evaluation
+
+def test_label_likelihood_tracker(cuda):
+  from pclsegmentation_amd import eval as ev
+  n, h, w, nc, none = 2, 5, 9, 11, 10
+  logits = (rnd(1, n, h, w, nc) * 3).float()
+  label = torch.randint(-1, nc + 1, (n, h, w), generator=torch.Generator().manual_seed(2)).to(torch.int32)
+  m = ev.LabelLikelihood(nc, none)
+  assert m.result() == (0.0, 0.0)
+  m.update_state(label[:1], logits[:1])                                     # accumulates; host tensors or device tensors
+  m.update_state(label[1:].to(cuda), logits[1:].to(cuda))
+  x, lab = logits.double().reshape(-1, nc)[:, :none], label.reshape(-1).long()
+  keep = (lab >= 0) & (lab < none)
+  logp = torch.log_softmax(x, -1)
+  nll = -logp[keep].gather(1, lab[keep][:, None]).mean()
+  entropy = -(logp.exp() * logp)[keep].sum(-1).mean()
+  got = m.result()
+  assert abs(got[0] - nll) <= 1e-5 and abs(got[1] - entropy) <= 1e-5      # about 100 roundings of values up to 10
+  m.reset_state()
+  assert m.result() == (0.0, 0.0)
+  with pytest.raises(ValueError):
+    m.update_state(label, logits[..., :5])
+
+
+def test_evaluation_prints_the_likelihood(cuda, tmp_path, capsys):
+  import numpy as np
+  import os
+  from pclsegmentation_amd import eval as ev
+  from pclsegmentation_amd import load_model_config
+  g = np.load(os.path.join(os.path.dirname(os.path.abspath(__file__)), "golden", "model_ssv2_real_32x240.npz"))
+  d = tmp_path / "data" / "val"
+  d.mkdir(parents=True)
+  samples = np.stack([np.concatenate([g["raw"][i], g["labels"][i][..., None].astype(np.float32)], -1) for i in range(2)])
+  for i in range(2):
+    np.save(str(d / ("s%d.npy" % i)), samples[i].astype(np.float64))
+  args = ["-d", str(tmp_path / "data"), "-i", "val", "-m", "squeezesegv2", "-n", "squeezesegv2"]
+  plain = ev.main(args)
+  assert "NLL" not in capsys.readouterr().out
+  with_nll = ev.main(args + ["--likelihood"])
+  out = capsys.readouterr().out
+  assert plain[3] == with_nll[3] and np.array_equal(plain[0], with_nll[0])      # the other metrics keep their values
+  got = [float(v) for v in (out.split("NLL:")[1].split()[0], out.split("Entropy:")[1].split()[0])]
+  mc, model = load_model_config("squeezesegv2", "squeezesegv2")
+  model.init_weights(4321)
+  preds, mask, logits = model.predict_raw(samples[..., :5], return_mask=True, return_logits=True)      # host arrays
+  none = mc.CLASSES.index("None")
+  lab = torch.from_numpy(np.where(mask, g["labels"], none).astype(np.int64)).reshape(-1)
+  x = torch.from_numpy(np.asarray(logits)).double().reshape(-1, mc.NUM_CLASS)
+  x[:, none] = -math.inf
+  logp = torch.log_softmax(x, -1)
+  keep = (lab != none) & (lab >= 0) & (lab < mc.NUM_CLASS)
+  p = torch.where(logp > -math.inf, logp.exp() * logp, torch.zeros_like(logp))
+  want = [-logp[keep].gather(1, lab[keep][:, None]).mean().item(), -p[keep].sum(-1).mean().item()]
+  assert all(abs(a - b) <= 1e-4 for a, b in zip(got, want))      # logits of two runs of the network agree to about 1e-5
+  assert torch.equal(torch.from_numpy(np.asarray(preds)), torch.from_numpy(np.asarray(model.predict_raw(samples[..., :5]))))
