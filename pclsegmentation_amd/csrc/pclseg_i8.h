@@ -239,7 +239,9 @@ __device__ __forceinline__ void i8_store(const I8Args& p, int64_t i, int j, int 
 
 // ---- few rows: the weights are read once, straight into the matrix operands
 // A block owns 16 channels and all of k; its NW waves take stretches of k (64 bytes of 16 weight rows an instruction, four
-// instructions in flight) and add their partial sums through LDS.  MT tiles of 16 rows share every weight fragment.
+// instructions in flight) and add their partial sums through LDS.  MT tiles of 16 rows share every weight fragment.  The
+// same kernel, with more rows in the grid's second axis, serves outputs of few tiles: k is split over the waves of a block
+// instead of one block walking all of it (80 x 146 x 3606: 14 us in six 64x64 tiles, 4 in 50 blocks).
 template <typename T, int MT, int NW>
 __global__ __launch_bounds__(NW * 64) void i8_few_rows(I8Args p) {
   __shared__ int part[NW][MT][256];
@@ -617,21 +619,36 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void i8_tiles(I8Args p, unsigned
     }
     return;
   }
+  // a tile at an edge: the same with a test a quad; a quad cut by the last channel goes element by element
+  const bool quad = col + 4 <= p.n, cut = col < p.n && !quad;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     to_slab(i);
+#pragma unroll 4
     for (int r = qr; r < 32; r += RP) {
       const int64_t row = m0 + wm + i * 32 + r;
-      if (row >= p.m) continue;
-      const float s = p.sa[row];
+      const bool live = row < p.m;
+      const float s = p.sa[live ? row : p.m - 1];
+      const u32x4 w = *reinterpret_cast<const u32x4*>(slab + r * SLD + qc);
+      float v[4], res[4] = {0.f, 0.f, 0.f, 0.f};
+      if (p.residual && quad && live) Quad<T>::load(static_cast<const T*>(p.residual) + row * p.ldr + col, res);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (col + e >= p.n) continue;
-        float v = activate(fmaf(slab[r * SLD + qc + e] * s, scale[e], bias[e]), p.act);
-        if (p.residual) v += Elem<T>::load(static_cast<const T*>(p.residual) + row * p.ldr + col + e);
-        static_cast<T*>(p.y)[row * p.ldy + col + e] = Elem<T>::from(v);
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(__uint_as_float(w[e]) * s, scale[e], bias[e]);
+      activate_all<4>(v, p.act);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += res[e];
+      if (quad && live) Quad<T>::store(static_cast<T*>(p.y) + row * p.ldy + col, v);
+      if (cut && live) {
+#pragma unroll
+        for (int e = 0; e < 3; ++e) {
+          if (col + e < p.n) {
+            if (p.residual) v[e] += Elem<T>::load(static_cast<const T*>(p.residual) + row * p.ldr + col + e);
+            static_cast<T*>(p.y)[row * p.ldy + col + e] = Elem<T>::from(v[e]);
+          }
+        }
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 

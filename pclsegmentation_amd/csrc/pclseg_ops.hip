@@ -28,6 +28,8 @@ bool dtype_ok(int d) { return d == PCLSEG_F32 || d == PCLSEG_BF16 || d == PCLSEG
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 size_t dtype_size(int d) { return d == PCLSEG_F32 ? 4 : 2; }
 constexpr int64_t kMaxBlocks = 0x7fffffff;
+// columns are counted in 32 bits, with room for a block's share behind the last; products of rows and columns stay below 2^63
+constexpr int64_t kMaxRows = (int64_t)1 << 40, kMaxColumns = 1 << 30;
 
 // calls f with a value of the element type
 template <typename F> void with_type(int dtype, F f) {
@@ -71,14 +73,23 @@ int matmul(const char* op, const I8Args& p, int dtype, hipStream_t s) {
   if (p.m > 64 && tiles(64, 64) > kMaxBlocks) return bad_shape(op, "more output tiles than a launch has blocks");
   with_type(dtype, [&](auto t) {
     typedef decltype(t) T;
-    const dim3 few((unsigned)((p.n + 15) / 16));
-    if (p.m <= 16) i8_few_rows<T, 1, 8><<<few, dim3(512), 0, s>>>(p);
-    else if (p.m <= 32) i8_few_rows<T, 2, 8><<<few, dim3(512), 0, s>>>(p);
-    else if (p.m <= 64) i8_few_rows<T, 4, 8><<<few, dim3(512), 0, s>>>(p);
-    // the largest tile that still gives most of the 256 CUs one: 8192x8192x4096 takes 297 us with 256x256 tiles, 299 with
-    // 128x128, 423 with 64x64; 8192x512x1024 18.8 / 10.5 / 11.5 us; 512x4096x4096 44 / 20.6 / 18.0 us
-    else if (p.kp == 64) launch_tiles<T, 128, 128, 64, 2, 2, 3>(p, s);
-    else if (tiles(256, 256) >= 192) launch_tiles<T, 256, 256, 128, 2, 4, 2>(p, s);
+    if (p.m <= 64 || tiles(64, 64) < 192) {
+      // row tiles a block shares its weights among: as many as there are, while 256 blocks remain
+      const int64_t cols = (p.n + 15) / 16;
+      const int mt = p.m > 32 && cols * ((p.m + 63) / 64) >= 256 ? 4 : p.m > 16 && cols * ((p.m + 31) / 32) >= 256 ? 2 : 1;
+      const dim3 g((unsigned)cols, (unsigned)((p.m + 16 * mt - 1) / (16 * mt)));
+      if (mt == 1) i8_few_rows<T, 1, 8><<<g, dim3(512), 0, s>>>(p);
+      else if (mt == 2) i8_few_rows<T, 2, 8><<<g, dim3(512), 0, s>>>(p);
+      else i8_few_rows<T, 4, 8><<<g, dim3(512), 0, s>>>(p);
+      return;
+    }
+    // The largest tile that fills the 256 CUs: 8192x8192x4096 takes 297 us with 256x256 tiles, 299 with 128x128, 423 with
+    // 64x64; 8192x512x1024 18.8 / 10.5 / 11.5 us; 512x4096x4096 44 / 20.6 / 18.0 us.  Between the first two the rounds decide,
+    // in units of a CU's time for a 128x128 tile: one 256x256 tile a CU costs 4, two 128x128 tiles 2 and 5 % more
+    // (15642x1260x2235 with its quantisation: 114 us in two rounds of 256x256, 1.2 of them needed, 101 in three of 128x128).
+    const int64_t big = (tiles(256, 256) + 255) / 256 * 4 * 20, mid = (tiles(128, 128) + 511) / 512 * 2 * 21;
+    if (p.kp == 64) launch_tiles<T, 128, 128, 64, 2, 2, 3>(p, s);
+    else if (tiles(256, 256) >= 192 && big <= mid) launch_tiles<T, 256, 256, 128, 2, 4, 2>(p, s);
     else if (tiles(128, 128) >= 192) launch_tiles<T, 128, 128, 128, 4, 2, 4>(p, s);
     else launch_tiles<T, 64, 64, 128, 2, 2, 4>(p, s);
   });
@@ -95,7 +106,7 @@ int check_product(const char* op, int64_t m, int64_t n, int64_t k, const int8_t*
                   const void* residual, int64_t residual_stride, const void* y, int64_t y_stride, int dtype) {
   if (!dtype_ok(dtype)) return bad(op, "unknown dtype");
   if (act < 0 || act > 3) return bad(op, "unknown activation");
-  if (m < 0 || n < 1 || n > 0x7fffffff - 256) return bad_shape(op, "m must not be negative, n must be in [1, 2^31 - 257]");
+  if (m < 0 || m > kMaxRows || n < 1 || n > kMaxColumns) return bad_shape(op, "m must be in [0, 2^40], n must be in [1, 2^30]");
   if (!row_bytes(k)) return bad_shape(op, "k must be in [1, 131071]");
   if (!b || !b_scale || (m && !y)) return bad(op, "NULL buffer");
   if (!aligned(b, 16)) return bad(op, "codes must be 16-byte aligned");
@@ -105,15 +116,15 @@ int check_product(const char* op, int64_t m, int64_t n, int64_t k, const int8_t*
 }
 
 // ---------------------------------------------------------------------------------------------- log probabilities
-constexpr int kThreadRow = 32, kGroupRow = 2048, kPiece = 2048, kRounds = 4, kManyRows = 2048, kFewRows = 512;
-constexpr int kOneLaunch = 16, kFewWaves = 4;       // pieces one block of 16 waves takes, pieces that 4 waves are enough for
+constexpr int kThreadRow = 32, kGroupRow = 2048, kPiece = 2048, kRounds = 4, kManyRows = 2048, kFewRows = 256;
+constexpr int kSortRows = 8192, kOneLaunch = 16, kFewWaves = 4;       // pieces one block of 16 waves takes, pieces that 4 waves are enough for
 
-// blocks a row is cut into: one up to 32768 classes (a piece for each of 16 waves); beyond that as many as keep few rows
-// from waiting on few CUs (one row of 131072: 20 us in one block, 6.9 + 4.3 in 16 and a second launch that joins them)
+// blocks a row is cut into: one up to 32768 classes (a piece for each of 16 waves) and from 32 rows on; else as many as keep
+// few rows from waiting on few CUs (one row of 131072: 20 us in one block, 6.9 + 4.3 in 16 and a second launch that joins them)
 int score_segs(int64_t rows, int64_t classes) {
   const int64_t pieces = (classes + kPiece - 1) / kPiece;
-  if (pieces <= kOneLaunch) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(pieces / 4, 64), 256 / rows));
+  if (pieces <= kOneLaunch || rows >= 32) return 1;
+  return (int)std::min<int64_t>(std::min<int64_t>(pieces / 4, 64), 256 / rows);
 }
 size_t score_workspace(int64_t rows, int64_t classes, int top_k) {
   const int segs = rows > 0 ? score_segs(rows, classes) : 1;
@@ -131,7 +142,9 @@ template <typename T, bool MASK> void launch_score(const ScoreArgs& a, hipStream
   const int v = a.classes;
   if (v <= kThreadRow) {
     launch_thread_rows<T, MASK, kThreadRow>(a, s);
-  } else if (v <= kGroupRow && !(v > 256 && a.top_k > kRounds)) {
+  } else if (v <= kGroupRow && (a.top_k <= kRounds || (v <= 256 && a.rows > kSortRows))) {
+    // (longer lists go to the waves below, which sort, unless many short rows make a wave for each the larger cost:
+    // 673x56 with 20 alternatives 23 us here, 8 there)
     auto grid = [&](int g) { return dim3((unsigned)((a.rows + 256 / g - 1) / (256 / g))); };
     if (v <= 8 * 32) logprob_group_rows<T, 8, MASK><<<grid(8), dim3(256), 0, s>>>(a);
     else if (v <= 16 * 32) logprob_group_rows<T, 16, MASK><<<grid(16), dim3(256), 0, s>>>(a);
@@ -162,8 +175,8 @@ template <typename T, bool MASK> void launch_score(const ScoreArgs& a, hipStream
 int check_rows(const char* op, const void* logits, int dtype, int64_t rows, int64_t classes, int64_t stride,
                const void* labels, int label_bytes, const uint8_t* allowed, int64_t allowed_stride, int top_k) {
   if (!dtype_ok(dtype)) return bad(op, "unknown dtype");
-  if (rows < 0 || classes < 1 || classes > 0x7fffffff - 4096)
-    return bad_shape(op, "rows must not be negative, classes must be in [1, 2^31 - 4097]");
+  if (rows < 0 || rows > kMaxRows || classes < 1 || classes > kMaxColumns)
+    return bad_shape(op, "rows must be in [0, 2^40], classes must be in [1, 2^30]");
   if (stride < classes) return bad_shape(op, "row stride smaller than classes");
   if (top_k < 0 || top_k > PCLSEG_TOP_MAX) return bad(op, "top_k must be in [0, 64]");
   if (rows && !logits) return bad(op, "logits is NULL");
@@ -308,7 +321,7 @@ int pclseg_op_label_logprobs_grad(const void* logits, int dtype, int64_t rows, i
   // a block takes 256 NI 16-byte pieces: that many of a long row, or whole short rows.  NI grows while the blocks are more
   // than the 2048 that run at once
   const int64_t vec = 16 / (int64_t)sz, nvec = (classes + vec - 1) / vec;
-  const int64_t all = rows > (int64_t(1) << 31) ? int64_t(1) << 40 : rows * nvec;
+  const int64_t all = std::min<int64_t>(rows, kMaxBlocks) * nvec;
   const int ni = all <= 2048 * 256 ? 1 : all <= 2 * 2048 * 256 ? 2 : 4;
   if (nvec > 256 * ni) {
     a.vecs = 256 * ni;

@@ -92,7 +92,13 @@ class Int8Rows:
   __slots__ = ("data", "scale", "k")
 
   def __init__(self, data, scale, k):
-    self.data, self.scale, self.k = data, scale, k
+    if (data.dtype != torch.int8 or data.dim() != 2 or data.shape[1] != _row_bytes(k) or not data.is_contiguous() or
+        scale.dtype != torch.float32 or tuple(scale.shape) != (data.shape[0],) or not scale.is_contiguous() or
+        scale.device != data.device):
+      _fail("Int8Rows holds contiguous int8 [rows, %d] (k %d) and float32 [rows] on one device, got %s %s and %s %s; "
+            "codes of another layout go through from_codes" % (_row_bytes(k), k, data.dtype, tuple(data.shape), scale.dtype,
+                                                              tuple(scale.shape)))
+    self.data, self.scale, self.k = data, scale, int(k)
 
   @classmethod
   def from_codes(cls, codes, scale):

@@ -280,7 +280,8 @@ def labels_for(rows, v, seed, dtype=torch.int32):
 
 SCORES = [(1, 1, 1), (5, 2, 3), (300, 3, 2), (257, 8, 8), (1000, 20, 3), (513, 31, 5), (70, 32, 32), (65, 33, 2), (40, 64, 64), (33, 100, 4),
           (31, 256, 20), (17, 257, 3), (9, 511, 32), (10, 513, 1), (6, 1031, 64), (5, 2048, 20), (7, 2049, 20), (3, 4097, 5), (4, 8193, 64),
-          (2, 30001, 20), (600, 2500, 3), (1, 131072, 20), (3, 131071, 32), (1, 300000, 64), (3, 131073, 7), (2, 1000003, 20), (1000, 5000, 0), (2100, 4099, 6), (2100, 2049, 0), (2, 9000, 0), (50, 77, 0)]
+          (2, 30001, 20), (600, 2500, 3), (1, 131072, 20), (3, 131071, 32), (1, 300000, 64), (3, 131073, 7), (2, 1000003, 20), (40, 40001, 20), (33, 131072, 3), (9000, 60, 9), (300, 56, 40), (600, 9001, 33), (1000, 5000, 0),
+          (2100, 4099, 6), (2100, 2049, 0), (2, 9000, 0), (50, 77, 0)]
 
 
 @pytest.mark.parametrize("rows,v,top_k", SCORES)
@@ -579,6 +580,32 @@ def test_only_the_rows_are_written(cuda):
                                               d.data_ptr(), None, None, None, 0, grad.data_ptr(), v + 5, stream))
     assert (grad[m:] == 5).all() and (grad[:, v:] == 5).all()
     assert torch.equal(grad[:m, :v], ops.label_logprobs_grad(logits, labels, fwd.lse, d_logprob=d))
+
+
+def test_offsets_beyond_32_bits(cuda):
+  """More than 2^31 elements in the logits, the gradient, and an output of the product: the last rows are the ones looked at."""
+  rows, v = 65540, 32769
+  x = torch.zeros((rows, v), dtype=BF16, device=cuda)
+  x[-3:] = rnd(1, 3, v).to(BF16).to(cuda)
+  labels = torch.full((rows,), 32768, dtype=torch.int32, device=cuda)
+  got = ops.label_logprobs(x, labels, top_k=3)
+  tail = ops.LabelLogprobs(*[t[-3:] for t in got])
+  ref = score64(x[-3:].cpu(), labels[-3:].cpu(), 3, None)
+  check_score(tail, ref, v, 3)
+  assert (got.lse[:-3] - math.log(v)).abs().max() <= 64 * U * 11 and (got.top_ids[:-3] == torch.arange(3, device=cuda, dtype=torch.int32)).all()
+  d = torch.ones(rows, device=cuda)
+  grad = ops.label_logprobs_grad(x, labels, got.lse, d_logprob=d)
+  want, bound = grad64(ref, labels[-3:].cpu(), got.lse[-3:].cpu().double(), None, d[-3:].cpu().double(), None, None, None, BF16)
+  close(grad[-3:], want, bound)
+  del x, grad, got
+  m, n, k = 132000, 16385, 40
+  a = torch.zeros((m, k), dtype=BF16, device=cuda)
+  a[-3:] = rnd(2, 3, k).to(BF16).to(cuda)
+  w = ops.quantize_rows(rnd(3, n, k).float().to(cuda))
+  y = ops.linear_i8(a, w)
+  q, s = quant64(a[-3:].cpu())
+  check_product(y[-3:], *product64(q, s, w.codes.cpu(), w.scale.cpu(), None, "none", None), BF16)
+  assert not y[:-3].any()
 
 
 # ---------------------------------------------------------------------------------------------- in the evaluation

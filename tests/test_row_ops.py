@@ -47,7 +47,8 @@ MATMUL = dict(a=P, a_scale=P, b=P, b_scale=P, m=2, n=3, k=8, bias=None, act=0, r
   (dict(n=1 << 31), -2, "n must"), (dict(k=0), -2, "k must"), (dict(k=131072), -2, "k must"), (dict(a=None), -1, "NULL"),
   (dict(b=None), -1, "NULL"), (dict(y=None), -1, "NULL"), (dict(a=P + 8), -1, "aligned"), (dict(b=P + 8), -1, "aligned"),
   (dict(y_stride=2), -2, "stride"), (dict(residual=P, residual_stride=2), -2, "stride"), (dict(y=P + 1), -1, "misaligned"),
-  (dict(m=1 << 40, n=1 << 20, y_stride=1 << 20), -2, "tiles"),
+  (dict(m=1 << 40, n=1 << 20, y_stride=1 << 20), -2, "tiles"), (dict(m=(1 << 40) + 1), -2, "m must"),
+  (dict(n=(1 << 30) + 1, y_stride=1 << 31), -2, "n must"),
 ])
 def test_matmul_i8_refuses(change, code, word):
   _refused("pclseg_op_matmul_i8", list({**MATMUL, **change}.values()), code, word)
@@ -87,6 +88,7 @@ SCORE = dict(logits=P, dtype=0, rows=2, classes=4, stride=4, labels=P, label_byt
 
 @pytest.mark.parametrize("change,code,word", [
   (dict(dtype=9), -1, "dtype"), (dict(rows=-1), -2, "rows"), (dict(classes=0), -2, "classes"), (dict(classes=1 << 31), -2, "classes"),
+  (dict(classes=(1 << 30) + 1, stride=1 << 31), -2, "classes"), (dict(rows=(1 << 40) + 1), -2, "rows"),
   (dict(stride=3), -2, "stride"), (dict(top_k=65), -1, "top_k"), (dict(top_k=-1), -1, "top_k"), (dict(logits=None), -1, "NULL"),
   (dict(label_bytes=2), -1, "int32"), (dict(labels=P + 2), -1, "misaligned"), (dict(labels=None), -1, "labels"),
   (dict(top_k=2), -1, "top_ids"), (dict(allowed=P, allowed_stride=3), -2, "mask"), (dict(logits=P + 2), -1, "misaligned"),
@@ -155,6 +157,10 @@ def test_python_layer_refuses(host_as_device):
     lambda: ops.quantize_rows(x.double()), lambda: ops.quantize_rows(torch.zeros(())), lambda: ops.quantize_rows(torch.zeros(2, 0)),
     lambda: ops.Int8Rows.from_codes(x, v), lambda: ops.Int8Rows.from_codes(x.to(torch.int8), torch.zeros(3)),
     lambda: ops.Int8Rows.from_kernel(torch.zeros(3, 3, 8, 4)),
+    lambda: ops.Int8Rows(torch.zeros((3, 8), dtype=torch.int8), torch.ones(3), 8), lambda: ops.Int8Rows(torch.zeros(3, 64), torch.ones(3), 8),
+    lambda: ops.Int8Rows(torch.zeros((3, 64), dtype=torch.int8), torch.ones(2), 8),
+    lambda: ops.Int8Rows(torch.zeros((3, 64), dtype=torch.int8), torch.ones(3), 65),
+    lambda: ops.Int8Rows(torch.zeros((3, 128), dtype=torch.int8)[:, :64], torch.ones(3), 8),
     lambda: ops.linear_i8(x, _rows8(k=9)), lambda: ops.linear_i8(x, x), lambda: ops.linear_i8(x, _rows8(), act="tanh"),
     lambda: ops.linear_i8(x, _rows8(), bias=torch.zeros(4)), lambda: ops.linear_i8(x, _rows8(), bias=torch.zeros(3).half()),
     lambda: ops.linear_i8(x, _rows8(), residual=torch.zeros(2, 4)), lambda: ops.linear_i8(x, _rows8(), residual=torch.zeros(2, 3).half()),
