@@ -430,12 +430,11 @@ template <> struct Quad<float> {
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(v[e]);
   }
-  static __device__ __forceinline__ void store(float* p, const float* f) { store16(p, pack16<float>(f)); }
+  static __device__ __forceinline__ void store(float* p, const float* f) { stream16(p, pack16<float>(f)); }
 };
-struct __attribute__((packed, aligned(2))) Pack8a2 { u32x2 v; };
 template <typename T> struct Quad16 {
   static __device__ __forceinline__ void load(const T* p, float* f) {
-    const u32x2 v = reinterpret_cast<const Pack8a2*>(p)->v;
+    const u32x2 v = *reinterpret_cast<const u32x2a2*>(p);
     const u32x4 w{v[0], v[1], 0u, 0u};
 #pragma unroll
     for (int e = 0; e < 4; ++e) f[e] = Elem<T>::get(w, e);
@@ -446,7 +445,7 @@ template <typename T> struct Quad16 {
     u32x2 v;
 #pragma unroll
     for (int e = 0; e < 2; ++e) v[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(F2{f[2 * e], f[2 * e + 1]}, T2));
-    reinterpret_cast<Pack8a2*>(p)->v = v;
+    __builtin_nontemporal_store((u32x2a2)v, reinterpret_cast<u32x2a2*>(p));
   }
 };
 template <> struct Quad<__bf16> : Quad16<__bf16> {};

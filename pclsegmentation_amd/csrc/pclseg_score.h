@@ -662,7 +662,7 @@ __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
     for (int e = 0; e < VEC; ++e) f[e] = x[e] == neg_inf() ? 0.f : f[e];
     T* dst = static_cast<T*>(a.grad) + (row0 + r) * a.grad_stride + c;
     if (inside) {
-      store16(dst, pack16<T>(f));
+      stream16(dst, pack16<T>(f));
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
