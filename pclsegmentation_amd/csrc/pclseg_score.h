@@ -157,9 +157,22 @@ __global__ __launch_bounds__(256, CAP <= 20 ? 6 : 4) void logprob_thread_rows(Sc
   Stat st{kLowest, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < CAP; ++j) st.m = fmaxf(st.m, x[j]);
+  // Rows this short are often decided: S = 1 + rest with a rest of 2^-10 would leave the logarithm 14 bits.  The terms below 1
+  // are summed by themselves (the fraction of a term of 1, the maximum, is 0); the two sums differ by the count of maxima.
+  float rest = 0.f;
 #pragma unroll
-  for (int j = 0; j < CAP; ++j) stat_add(st, x[j]);
-  const RowOut o = row_out(st);
+  for (int j = 0; j < CAP; ++j) {
+    const float z = x[j] - st.m, e = fast_exp(z);
+    st.s += e;
+    rest += __builtin_amdgcn_fractf(e);
+    st.t = fmaf(e, fmaxf(z, -200.f), st.t);
+  }
+  RowOut o = row_out(st);
+  if (!o.empty && !o.bad && rintf(st.s - rest) == 1.f) {
+    o.logs = log1pf(rest);
+    o.lse = st.m + o.logs;
+    o.entropy = o.logs - st.t / (1.f + rest);
+  }
   write_row<T>(a, row, o);
   if (a.top_k == 0) return;
   int32_t* ids = a.top_ids + row * a.top_k;
@@ -543,7 +556,9 @@ __global__ __launch_bounds__(256) void logprob_join(ScoreArgs a) {
 
 // ---- gradient
 // With p_j = e^(x_j - lse) (0 where not allowed), H the row's entropy, gl / ge / gt the gradients that arrive:
-//   d loss / d x_j = gl [j = label] + sum_i gt_i [j = id_i] - p_j (gl + sum_i gt_i) - ge p_j (x_j - lse + H)
+//   d loss / d x_j = G_j (1 - p_j) - p_j (W - G_j) - ge p_j (x_j - lse + H),
+//   G_j = gl [j = label] + sum_i gt_i [j = id_i],  W = gl + sum_i gt_i
+// 1 - p of a named class is taken from x - lse without the difference: a decided row's label keeps its significant bits.
 // One read of the logits and one write of the gradient.  A block owns whole rows, or a piece of one; the classes that its
 // rows' labels and alternatives name, and what arrives for them, are put into LDS first, and every 16-byte piece is compared
 // with its row's names while it is in registers: no element is written twice, equal names add up.
@@ -568,10 +583,21 @@ struct GradArgs {
 
 struct GradRow { float lse, w, ge, h; };   // w = gl + sum gt; empty rows have all of them 0
 
-__device__ __forceinline__ float grad_dense(const GradRow& r, float x) {
+// 1 - e^z: the series of e^z - 1 where the difference would cancel (7 terms: 0.35^7 / 8! < 2^-25), the difference elsewhere
+__device__ __forceinline__ float one_minus_exp(float z) {
+  float s = 1.f / 5040.f;
+  s = fmaf(s, z, 1.f / 720.f);
+  s = fmaf(s, z, 1.f / 120.f);
+  s = fmaf(s, z, 1.f / 24.f);
+  s = fmaf(s, z, 1.f / 6.f);
+  s = fmaf(s, z, 0.5f);
+  s = fmaf(s, z, 1.f);
+  return z > -0.35f ? -z * s : 1.f - fast_exp(z);
+}
+__device__ __forceinline__ float grad_dense(const GradRow& r, float w, float x) {
   const float z = x - r.lse, p = fast_exp(z);
   // an underflowed p takes the entropy term with it (0 * -inf otherwise)
-  return -p * fmaf(r.ge, fmaxf(z, -200.f) + r.h, r.w);
+  return -p * fmaf(r.ge, fmaxf(z, -200.f) + r.h, w);
 }
 
 constexpr int kGradNames = 1024;      // names a block holds
@@ -649,14 +675,24 @@ __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
     else load_tail<T, MASK>(static_cast<const T*>(a.x) + (row0 + r) * a.stride,
                             MASK ? a.allowed + (row0 + r) * a.allowed_stride : nullptr, c, c1, x);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = grad_dense(p, x[e]);
+    for (int e = 0; e < VEC; ++e) f[e] = 0.f;      // G_j first
+    bool named = false;
     for (int k = r * names; k < (r + 1) * names; ++k) {
       const int d = ids[k] - c;
       if ((unsigned)d < (unsigned)VEC) {
+        named = true;
         const float g = gs[k];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) f[e] += e == d ? g : 0.f;
       }
+    }
+    if (named) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        f[e] = fmaf(f[e], one_minus_exp(x[e] - p.lse), grad_dense(p, p.w - f[e], x[e]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] = grad_dense(p, p.w, x[e]);
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) f[e] = x[e] == neg_inf() ? 0.f : f[e];

@@ -456,6 +456,31 @@ def test_label_logprobs_grad_against_differences(cuda):
   assert (got.cpu().double() - want).abs().max() <= 1e-5        # 40 roundings of terms up to 5
 
 
+@pytest.mark.parametrize("v", [2, 3, 20, 32])
+@pytest.mark.parametrize("lead", [2.0, 6.0, 11.0, 30.0])
+def test_decided_rows_keep_their_significant_bits(cuda, v, lead):
+  """ln p of a class that has nearly everything is -(the rest): relative, not absolute, to 2^-24.  z = x - M is a few roundings
+  relative to the exponent, 3 u |z| in a term; the sums and the logarithm add 40 u.  The gradient of the label likewise."""
+  x = -rnd(v, 5, v).abs().float()
+  x[:, 1] = lead
+  labels = torch.ones(5, dtype=torch.int32)
+  got = ops.label_logprobs(x.to(cuda), labels.to(cuda), top_k=1)
+  z = x.double() - x.double()[:, 1:2]
+  z[:, 1] = -math.inf
+  rest = torch.exp(z).sum(1)
+  logp = -torch.log1p(rest)
+  rel = U * (3 * (lead + 5) + 40)
+  close(got.logprob, logp, rel * logp.abs())
+  close(got.top_logprobs[:, 0], logp, rel * logp.abs())
+  entropy = -logp + (torch.exp(z) * torch.where(z > -math.inf, -z, torch.zeros_like(z))).sum(1) / (1 + rest)
+  close(got.entropy, entropy, 2 * rel * entropy)
+  g = torch.full((5,), -0.75)
+  lse = got.lse.cpu().double()
+  grad = ops.label_logprobs_grad(x.to(cuda), labels.to(cuda), got.lse, d_logprob=g.to(cuda))[:, 1]
+  want = 0.75 * torch.expm1(x.double()[:, 1] - lse)
+  close(grad, want, 16 * U * want.abs())
+
+
 def test_label_logprobs_grad_names_that_coincide(cuda):
   """The label among the alternatives, and the same alternative named twice: their gradients add up."""
   x = rnd(1, 3, 50).float()
