@@ -350,9 +350,11 @@ def test_label_logprobs_odd_rows(cuda, v, dtype):
     check_score(ops.label_logprobs(x[r:r + 1].to(cuda), labels[r:r + 1].to(cuda), top_k=k), one, v, k)
 
 
-def test_label_logprobs_layouts(cuda):
-  base = rnd(1, 6, 4, 90).float().to(cuda)
-  for view in (base[..., 3:60], base[:, 2], base.transpose(0, 1), base[..., ::3], base[:1, :1].expand(5, 2, 90), base[0, 0]):
+@pytest.mark.parametrize("width", [90, 25, 3001])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_label_logprobs_layouts(cuda, width, dtype):
+  base = rnd(1, 6, 4, width).to(dtype).to(cuda)
+  for view in (base[..., 3:width - 4], base[:, 2], base.transpose(0, 1), base[..., ::3], base[:1, :1].expand(5, 2, width), base[0, 0]):
     v = view.shape[-1]
     flat = view.cpu().reshape(-1, v)
     labels = labels_for(len(flat), v, 1).view(view.shape[:-1])
@@ -361,7 +363,7 @@ def test_label_logprobs_layouts(cuda):
     ref = score64(flat, labels.reshape(-1), 2, None)
     check_score(ops.LabelLogprobs(*[t.reshape(-1, *t.shape[view.dim() - 1:]) for t in got]), ref, v, 2)
   assert ops.label_logprobs(base).logprob is None
-  none = ops.label_logprobs(base[:0], top_k=3)
+  none = ops.label_logprobs(base[:0], top_k=3)      # no rows
   assert none.lse.shape == (0, 4) and none.top_ids.shape == (0, 4, 3)
 
 
@@ -588,13 +590,20 @@ def test_only_the_rows_are_written(cuda):
   """The C entry points write the outputs' rows and nothing beside them."""
   from pclsegmentation_amd import engine as E
   lib, stream = E.load_library(), E.stream_handle(cuda)
-  for m, n, k in ((3, 21, 70), (70, 33, 130)):
+  for m, n, k in ((3, 21, 70), (70, 33, 130), (3000, 1030, 70), (700, 4000, 200)):
     w = ops.quantize_rows(rnd(1, n, k).float().to(cuda))
     x = ops.quantize_rows(rnd(2, m, k).float().to(cuda))
     y = torch.full((m + 2, n + 7), 5.0, device=cuda)
     E.check(lib.pclseg_op_matmul_i8(x.data.data_ptr(), x.scale.data_ptr(), w.data.data_ptr(), w.scale.data_ptr(), m, n, k, None, 0,
                                     None, 0, y.data_ptr(), n + 7, 0, stream))
     assert (y[m:] == 5).all() and (y[:, n:] == 5).all() and torch.equal(y[:m, :n], ops.matmul_i8(x, w))
+    # the residual may be the output
+    res = rnd(4, m, n).float().to(cuda)
+    want, z = ops.matmul_i8(x, w, act="relu", residual=res), torch.full((m + 2, n + 7), 5.0, device=cuda)
+    z[:m, :n] = res
+    E.check(lib.pclseg_op_matmul_i8(x.data.data_ptr(), x.scale.data_ptr(), w.data.data_ptr(), w.scale.data_ptr(), m, n, k, None, 1,
+                                    z.data_ptr(), n + 7, z.data_ptr(), n + 7, 0, stream))
+    assert torch.equal(z[:m, :n], want) and (z[m:] == 5).all() and (z[:, n:] == 5).all()
   for m, v in ((5, 21), (3, 9001)):
     logits = rnd(3, m, v).float().to(cuda)
     labels = labels_for(m, v, 1).to(cuda)

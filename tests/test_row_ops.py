@@ -180,3 +180,33 @@ def test_python_layer_refuses(host_as_device):
     with pytest.raises(ValueError):
       call()
       pytest.fail("call %d was accepted" % n)
+
+
+def test_calls_run_with_the_tensors_device_current(monkeypatch):
+  """With several devices the launch is made under the tensors' device, and the caller's is restored."""
+  class Dev:
+    index = 1
+  state = {"current": 0, "during": None}
+
+  class Guard:
+    def __init__(self, dev):
+      self.dev = dev
+
+    def __enter__(self):
+      self.was, state["current"] = state["current"], self.dev.index
+
+    def __exit__(self, *a):
+      state["current"] = self.was
+
+  def launch(x, stream):
+    state["during"] = (state["current"], x, stream)
+    return 0
+  monkeypatch.setattr(ops, "_several_devices", lambda: True)
+  monkeypatch.setattr(torch.cuda, "current_device", lambda: state["current"])
+  monkeypatch.setattr(torch.cuda, "device", Guard)
+  monkeypatch.setattr(E, "stream_handle", lambda dev: 77)
+  ops._call(Dev, launch, 5)
+  assert state == {"current": 0, "during": (1, 5, 77)}
+  state["current"] = 1
+  ops._call(Dev, launch, 6)
+  assert state == {"current": 1, "during": (1, 6, 77)}
