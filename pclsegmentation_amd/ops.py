@@ -43,6 +43,8 @@ def _on(t, dev, name):
 
 def _rows(t, cols):
   """[..., cols] as two axes with adjacent elements and rows that do not overlap (a copy where the strides say otherwise)."""
+  if t.is_contiguous():
+    return (t if t.dim() == 2 else t.view(-1, cols)), cols
   r = t if t.dim() == 2 else t.reshape(-1, cols)
   if cols > 1 and r.stride(1) != 1 or r.shape[0] > 1 and r.stride(0) < cols:
     r = r.contiguous()
@@ -203,7 +205,7 @@ def linear_i8(x, weight, bias=None, act="none", residual=None, out_dtype=None):
   r, stride = _rows(x, k)
   m = r.shape[0]
   bias, residual, rstride = _epilogue(dev, m, n, shape, weight, bias, act, residual, out_dtype)
-  y = torch.empty(shape, dtype=out_dtype, device=dev)
+  y = x.new_empty(shape, dtype=out_dtype)
   if m and n:
     size = _workspace("pclseg_op_linear_i8_workspace", m, n, k)
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
@@ -237,8 +239,7 @@ def _logits(logits):
   dt = _dtype(logits, "logits")
   if logits.dim() < 1 or logits.shape[-1] < 1:
     _fail("logits must be [..., classes], got shape %s" % (tuple(logits.shape),))
-  r, stride = _rows(logits, logits.shape[-1])
-  return dt, r, stride
+  return (dt,) + _rows(logits, logits.shape[-1])
 
 
 def label_logprobs(logits, labels=None, top_k=0, allowed=None):
@@ -258,11 +259,11 @@ def label_logprobs(logits, labels=None, top_k=0, allowed=None):
   if allowed is not None:
     allowed, mstride = _mask(allowed, logits)
   size = _workspace("pclseg_op_label_logprobs_workspace", m, v, top_k)
-  logprob, entropy, lse = torch.empty((3,) + shape, dtype=torch.float32, device=dev).unbind(0)
+  logprob, entropy, lse = logits.new_empty((3,) + shape, dtype=torch.float32).unbind(0)
   if labels is None:
     logprob = None
-  ids = torch.empty(shape + (top_k,), dtype=torch.int32, device=dev) if top_k else None
-  tops = torch.empty(shape + (top_k,), dtype=torch.float32, device=dev) if top_k else None
+  ids = logits.new_empty(shape + (top_k,), dtype=torch.int32) if top_k else None
+  tops = logits.new_empty(shape + (top_k,), dtype=torch.float32) if top_k else None
   if m:
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     _call(dev, _engine.load_library().pclseg_op_label_logprobs, r.data_ptr(), dt, m, v, stride, _ptr(labels),
@@ -302,7 +303,7 @@ def label_logprobs_grad(logits, labels, lse, d_logprob=None, entropy=None, d_ent
   mstride = 0
   if allowed is not None:
     allowed, mstride = _mask(allowed, logits)
-  grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+  grad = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty(logits.shape)
   if m:
     _call(dev, _engine.load_library().pclseg_op_label_logprobs_grad, r.data_ptr(), dt, m, v, stride,
           _ptr(labels) if d_logprob is not None else None, labels.element_size() if d_logprob is not None else 0,
