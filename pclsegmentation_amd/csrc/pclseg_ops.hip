@@ -83,12 +83,19 @@ int matmul(const char* op, const I8Args& p, int dtype, hipStream_t s) {
       else i8_few_rows<T, 4, 8><<<g, dim3(512), 0, s>>>(p);
       return;
     }
-    // The largest tile that fills the 256 CUs: 8192x8192x4096 takes 297 us with 256x256 tiles, 299 with 128x128, 423 with
-    // 64x64; 8192x512x1024 18.8 / 10.5 / 11.5 us; 512x4096x4096 44 / 20.6 / 18.0 us.  Between the first two the rounds decide,
+    // The largest tile that fills the 256 CUs: 8192x8192x4096 takes 301 us with 256x256 tiles, 302 with 128x128, 435 with
+    // 64x64; 8192x512x1024 17.3 / 9.6 / 10.6 us; 512x4096x4096 44 / 20.6 / 18.0 us.  Between the first two the rounds decide,
     // in units of a CU's time for a 128x128 tile: one 256x256 tile a CU costs 4, two 128x128 tiles 2 and 5 % more
     // (15642x1260x2235 with its quantisation: 114 us in two rounds of 256x256, 1.2 of them needed, 101 in three of 128x128).
+    // Up to 256 columns of many rows a tile is mostly stores: 128x128 with steps of 64 bytes, three of them on a CU, one
+    // storing while the others multiply, from 16 tiles a CU on (linear of 131072x512 float32: k = 128 78 us against 88 with
+    // 256x256, k = 256 109 against 117; 8192x2048 bf16, k = 256, four tiles a CU: 24.5 against 21.7; 131072x1024 float32,
+    // k = 512: 271 against 255).  Up to 64 channels nothing wider than they are (131072x64x128: 8.5 us against 13.4 with
+    // 128x128; the linear of 131072x64 bf16 from k = 50: 23 against 33).
     const int64_t big = (tiles(256, 256) + 255) / 256 * 4 * 20, mid = (tiles(128, 128) + 511) / 512 * 2 * 21;
-    if (p.kp == 64) launch_tiles<T, 128, 128, 64, 2, 2, 3>(p, s);
+    if (p.n <= 64 && p.kp == 64) launch_tiles<T, 128, 64, 64, 2, 2, 4>(p, s);
+    else if (p.n <= 64) launch_tiles<T, 64, 64, 128, 2, 2, 4>(p, s);
+    else if (p.kp == 64 || (p.kp <= 256 && tiles(128, 128) >= 4096)) launch_tiles<T, 128, 128, 64, 2, 2, 3>(p, s);
     else if (tiles(256, 256) >= 192 && big <= mid) launch_tiles<T, 256, 256, 128, 2, 4, 2>(p, s);
     else if (tiles(128, 128) >= 192) launch_tiles<T, 128, 128, 128, 4, 2, 4>(p, s);
     else launch_tiles<T, 64, 64, 128, 2, 2, 4>(p, s);

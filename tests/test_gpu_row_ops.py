@@ -112,7 +112,8 @@ def check_product(got, want, bound, dtype):
 PRODUCTS = [  # m, n, k
   (1, 1, 1), (1, 8, 16), (1, 4096, 512), (2, 17, 63), (5, 100, 65), (16, 33, 128), (17, 257, 1000), (32, 16, 4096), (33, 70, 300),
   (64, 511, 257), (65, 1, 5), (65, 129, 64), (127, 300, 40), (130, 64, 129), (200, 1000, 1000), (257, 513, 384), (3000, 4100, 200),
-  (4100, 3001, 64), (5000, 2600, 256), (1, 40, 131071), (70, 40, 20000)]
+  (4100, 3001, 64), (5000, 2600, 256), (70001, 1000, 200), (20000, 64, 50), (20001, 50, 200), (13000, 33, 64), (9000, 1100, 384), (9000, 3000, 640),
+  (1, 40, 131071), (70, 40, 20000)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
