@@ -27,9 +27,30 @@ int launched(const char* op) {
 bool dtype_ok(int d) { return d == PCLSEG_F32 || d == PCLSEG_BF16 || d == PCLSEG_F16; }
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 size_t dtype_size(int d) { return d == PCLSEG_F32 ? 4 : 2; }
-constexpr int64_t kMaxBlocks = 0x7fffffff;
+constexpr int64_t kMaxBlocks = 0x7fffffff, kMaxThreads = 0xffffffff;      // of a launch: blocks, and threads along an axis
 // columns are counted in 32 bits, with room for a block's share behind the last; products of rows and columns stay below 2^63
 constexpr int64_t kMaxRows = (int64_t)1 << 40, kMaxColumns = 1 << 30;
+
+// Launches on a stream one after the other; after one that fails or does not fit a launch, none.  dry: looks the sizes over only.
+struct Launch {
+  const char* op;
+  hipStream_t s;
+  bool dry = false;
+  int rc = PCLSEG_OK;
+  template <typename... P, typename... A> void run(void (*kernel)(P...), int64_t blocks, unsigned blocks_y, int threads, size_t lds, A... args) {
+    if (rc) return;
+    if (blocks > std::min<int64_t>(kMaxBlocks, kMaxThreads / threads)) {
+      rc = bad_shape(op, "more rows or output tiles than a launch has blocks for");
+      return;
+    }
+    if (dry) return;
+    kernel<<<dim3((unsigned)blocks, blocks_y), dim3(threads), lds, s>>>(args...);
+    rc = launched(op);
+  }
+  template <typename... P, typename... A> void operator()(void (*kernel)(P...), int64_t blocks, int threads, A... args) {
+    run(kernel, blocks, 1, threads, 0, args...);
+  }
+};
 
 // calls f with a value of the element type
 template <typename F> void with_type(int dtype, F f) {
@@ -44,43 +65,41 @@ int64_t row_bytes(int64_t k) {
   return k <= 64 ? 64 : (k + 127) / 128 * 128;
 }
 
-template <typename T, int G> void launch_quant(const QuantArgs& a, hipStream_t s) {
+template <typename T, int G> void launch_quant(const QuantArgs& a, Launch& go) {
   const int64_t blocks = (a.rows + 256 / G - 1) / (256 / G);
-  if (a.cols > 32 * G) quantize_rows_kernel<T, G, true><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(a);
-  else quantize_rows_kernel<T, G, false><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(a);
+  if (a.cols > 32 * G) go(quantize_rows_kernel<T, G, true>, blocks, 256, a);
+  else go(quantize_rows_kernel<T, G, false>, blocks, 256, a);
 }
 
-int quantize(const char* op, const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, int8_t* q, float* scale,
-             hipStream_t s) {
+int quantize(Launch go, const void* x, int dtype, int64_t rows, int64_t cols, int64_t stride, int8_t* q, float* scale) {
   QuantArgs a{x, rows, stride, (int)cols, q, row_bytes(cols), scale};
   with_type(dtype, [&](auto t) {
     typedef decltype(t) T;
-    if (cols <= 256) launch_quant<T, 8>(a, s);
-    else if (cols <= 2048) launch_quant<T, 64>(a, s);
-    else launch_quant<T, 256>(a, s);
+    if (cols <= 256) launch_quant<T, 8>(a, go);
+    else if (cols <= 2048) launch_quant<T, 64>(a, go);
+    else launch_quant<T, 256>(a, go);
   });
-  return launched(op);
+  return go.rc;
 }
 
 template <typename T, int BM, int BN, int BK, int WM, int WN, int OCC>
-void launch_tiles(const I8Args& p, hipStream_t s) {
+void launch_tiles(const I8Args& p, Launch& go) {
   const int64_t tm = (p.m + BM - 1) / BM, tn = (p.n + BN - 1) / BN;
-  i8_tiles<T, BM, BN, BK, WM, WN, OCC><<<dim3((unsigned)(tm * tn)), dim3(WM * WN * 64), 0, s>>>(p, (unsigned)tm, (unsigned)tn);
+  go(i8_tiles<T, BM, BN, BK, WM, WN, OCC>, tm * tn, WM * WN * 64, p, (unsigned)tm, (unsigned)tn);
 }
 
-int matmul(const char* op, const I8Args& p, int dtype, hipStream_t s) {
+int matmul(Launch go, const I8Args& p, int dtype) {
   auto tiles = [&](int bm, int bn) { return ((p.m + bm - 1) / bm) * ((p.n + (int64_t)bn - 1) / bn); };
-  if (p.m > 64 && tiles(64, 64) > kMaxBlocks) return bad_shape(op, "more output tiles than a launch has blocks");
   with_type(dtype, [&](auto t) {
     typedef decltype(t) T;
     if (p.m <= 64 || tiles(64, 64) < 192) {
       // row tiles a block shares its weights among: as many as there are, while 256 blocks remain
       const int64_t cols = (p.n + 15) / 16;
       const int mt = p.m > 32 && cols * ((p.m + 63) / 64) >= 256 ? 4 : p.m > 16 && cols * ((p.m + 31) / 32) >= 256 ? 2 : 1;
-      const dim3 g((unsigned)cols, (unsigned)((p.m + 16 * mt - 1) / (16 * mt)));
-      if (mt == 1) i8_few_rows<T, 1, 8><<<g, dim3(512), 0, s>>>(p);
-      else if (mt == 2) i8_few_rows<T, 2, 8><<<g, dim3(512), 0, s>>>(p);
-      else i8_few_rows<T, 4, 8><<<g, dim3(512), 0, s>>>(p);
+      const unsigned rows = (unsigned)((p.m + 16 * mt - 1) / (16 * mt));
+      if (mt == 1) go.run(i8_few_rows<T, 1, 8>, cols, rows, 512, 0, p);
+      else if (mt == 2) go.run(i8_few_rows<T, 2, 8>, cols, rows, 512, 0, p);
+      else go.run(i8_few_rows<T, 4, 8>, cols, rows, 512, 0, p);
       return;
     }
     // The largest tile that fills the 256 CUs: 8192x8192x4096 takes 301 us with 256x256 tiles, 302 with 128x128, 435 with
@@ -93,14 +112,14 @@ int matmul(const char* op, const I8Args& p, int dtype, hipStream_t s) {
     // k = 512: 271 against 255).  Up to 64 channels nothing wider than they are (131072x64x128: 8.5 us against 13.4 with
     // 128x128; the linear of 131072x64 bf16 from k = 50: 23 against 33).
     const int64_t big = (tiles(256, 256) + 255) / 256 * 4 * 20, mid = (tiles(128, 128) + 511) / 512 * 2 * 21;
-    if (p.n <= 64 && p.kp == 64) launch_tiles<T, 128, 64, 64, 2, 2, 4>(p, s);
-    else if (p.n <= 64) launch_tiles<T, 64, 64, 128, 2, 2, 4>(p, s);
-    else if (p.kp == 64 || (p.kp <= 256 && tiles(128, 128) >= 4096)) launch_tiles<T, 128, 128, 64, 2, 2, 3>(p, s);
-    else if (tiles(256, 256) >= 192 && big <= mid) launch_tiles<T, 256, 256, 128, 2, 4, 2>(p, s);
-    else if (tiles(128, 128) >= 192) launch_tiles<T, 128, 128, 128, 4, 2, 4>(p, s);
-    else launch_tiles<T, 64, 64, 128, 2, 2, 4>(p, s);
+    if (p.n <= 64 && p.kp == 64) launch_tiles<T, 128, 64, 64, 2, 2, 4>(p, go);
+    else if (p.n <= 64) launch_tiles<T, 64, 64, 128, 2, 2, 4>(p, go);
+    else if (p.kp == 64 || (p.kp <= 256 && tiles(128, 128) >= 4096)) launch_tiles<T, 128, 128, 64, 2, 2, 3>(p, go);
+    else if (tiles(256, 256) >= 192 && big <= mid) launch_tiles<T, 256, 256, 128, 2, 4, 2>(p, go);
+    else if (tiles(128, 128) >= 192) launch_tiles<T, 128, 128, 128, 4, 2, 4>(p, go);
+    else launch_tiles<T, 64, 64, 128, 2, 2, 4>(p, go);
   });
-  return launched(op);
+  return go.rc;
 }
 
 // up to 32 rows of together 64 items of 512 elements: one launch, no workspace (see i8_fused_rows)
@@ -138,43 +157,43 @@ size_t score_workspace(int64_t rows, int64_t classes, int top_k) {
   return segs == 1 ? 0 : (size_t)rows * segs * (sizeof(ScorePart) + (top_k ? 64 * sizeof(Key) : 0));
 }
 
-template <typename T, bool MASK, int CAP> void launch_thread_rows(const ScoreArgs& a, hipStream_t s) {
+template <typename T, bool MASK, int CAP> void launch_thread_rows(const ScoreArgs& a, Launch& go) {
   if constexpr (CAP > Elem<T>::VEC) {
-    if (a.classes <= CAP - Elem<T>::VEC) return launch_thread_rows<T, MASK, CAP - Elem<T>::VEC>(a, s);
+    if (a.classes <= CAP - Elem<T>::VEC) return launch_thread_rows<T, MASK, CAP - Elem<T>::VEC>(a, go);
   }
-  logprob_thread_rows<T, CAP, MASK><<<dim3((unsigned)((a.rows + 255) / 256)), dim3(256), 0, s>>>(a);
+  go(logprob_thread_rows<T, CAP, MASK>, (a.rows + 255) / 256, 256, a);
 }
 
-template <typename T, bool MASK> void launch_score(const ScoreArgs& a, hipStream_t s) {
+template <typename T, bool MASK> void launch_score(const ScoreArgs& a, Launch& go) {
   const int v = a.classes;
   if (v <= kThreadRow) {
-    launch_thread_rows<T, MASK, kThreadRow>(a, s);
+    launch_thread_rows<T, MASK, kThreadRow>(a, go);
   } else if (v <= kGroupRow && (a.top_k <= kRounds || (v <= 256 && a.rows > kSortRows))) {
     // (longer lists go to the waves below, which sort, unless many short rows make a wave for each the larger cost:
     // 673x56 with 20 alternatives 23 us here, 8 there)
-    auto grid = [&](int g) { return dim3((unsigned)((a.rows + 256 / g - 1) / (256 / g))); };
-    if (v <= 8 * 32) logprob_group_rows<T, 8, MASK><<<grid(8), dim3(256), 0, s>>>(a);
-    else if (v <= 16 * 32) logprob_group_rows<T, 16, MASK><<<grid(16), dim3(256), 0, s>>>(a);
-    else if (v <= 32 * 32) logprob_group_rows<T, 32, MASK><<<grid(32), dim3(256), 0, s>>>(a);
-    else logprob_group_rows<T, 64, MASK><<<grid(64), dim3(256), 0, s>>>(a);
+    auto blocks = [&](int g) { return (a.rows + 256 / g - 1) / (256 / g); };
+    if (v <= 8 * 32) go(logprob_group_rows<T, 8, MASK>, blocks(8), 256, a);
+    else if (v <= 16 * 32) go(logprob_group_rows<T, 16, MASK>, blocks(16), 256, a);
+    else if (v <= 32 * 32) go(logprob_group_rows<T, 32, MASK>, blocks(32), 256, a);
+    else go(logprob_group_rows<T, 64, MASK>, blocks(64), 256, a);
   } else {
-    const dim3 g((unsigned)(a.rows * a.segs));
+    const int64_t blocks = a.rows * a.segs;
     // one wave a row where that fills the chip: a list is kept and merged once a row instead of four times
     if (v > kPiece && a.rows < kManyRows) {
       if (v > kFewWaves * kPiece && a.rows <= kFewRows && a.segs == 1) {
-        if (a.top_k) logprob_wave_rows<T, 16, true, MASK><<<g, dim3(1024), 0, s>>>(a);
-        else logprob_wave_rows<T, 16, false, MASK><<<g, dim3(1024), 0, s>>>(a);
+        if (a.top_k) go(logprob_wave_rows<T, 16, true, MASK>, blocks, 1024, a);
+        else go(logprob_wave_rows<T, 16, false, MASK>, blocks, 1024, a);
       } else {
-        if (a.top_k) logprob_wave_rows<T, 4, true, MASK><<<g, dim3(256), 0, s>>>(a);
-        else logprob_wave_rows<T, 4, false, MASK><<<g, dim3(256), 0, s>>>(a);
+        if (a.top_k) go(logprob_wave_rows<T, 4, true, MASK>, blocks, 256, a);
+        else go(logprob_wave_rows<T, 4, false, MASK>, blocks, 256, a);
       }
     } else {
-      if (a.top_k) logprob_wave_rows<T, 1, true, MASK><<<g, dim3(64), 0, s>>>(a);
-      else logprob_wave_rows<T, 1, false, MASK><<<g, dim3(64), 0, s>>>(a);
+      if (a.top_k) go(logprob_wave_rows<T, 1, true, MASK>, blocks, 64, a);
+      else go(logprob_wave_rows<T, 1, false, MASK>, blocks, 64, a);
     }
     if (a.segs > 1) {
-      if (a.top_k) logprob_join<T, true><<<dim3((unsigned)a.rows), dim3(256), 0, s>>>(a);
-      else logprob_join<T, false><<<dim3((unsigned)a.rows), dim3(256), 0, s>>>(a);
+      if (a.top_k) go(logprob_join<T, true>, a.rows, 256, a);
+      else go(logprob_join<T, false>, a.rows, 256, a);
     }
   }
 }
@@ -209,7 +228,7 @@ int pclseg_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols
   if (rows == 0) return PCLSEG_OK;
   if (!x || !q || !scale) return bad(op, "NULL buffer");
   if (!aligned(x, dtype_size(dtype)) || !aligned(q, 8)) return bad(op, "misaligned x or codes");
-  return quantize(op, x, dtype, rows, cols, x_stride, q, scale, (hipStream_t)hip_stream);
+  return quantize({op, (hipStream_t)hip_stream}, x, dtype, rows, cols, x_stride, q, scale);
 } OP_CATCH
 
 int pclseg_op_matmul_i8(const int8_t* a, const float* a_scale, const int8_t* b, const float* b_scale, int64_t m,
@@ -223,7 +242,7 @@ int pclseg_op_matmul_i8(const int8_t* a, const float* a_scale, const int8_t* b, 
   if (!aligned(a, 16)) return bad(op, "codes must be 16-byte aligned");
   I8Args p{a, b, a_scale, b_scale, row_bytes(k), row_bytes(k), m, (int)n, (int)row_bytes(k), bias, act, residual,
            residual_stride, y, y_stride};
-  return matmul(op, p, dtype, (hipStream_t)hip_stream);
+  return matmul({op, (hipStream_t)hip_stream}, p, dtype);
 } OP_CATCH
 
 int pclseg_op_linear_i8_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes) try {
@@ -247,29 +266,30 @@ int pclseg_op_linear_i8(const void* x, int dtype, int64_t x_stride, const int8_t
   if (!x) return bad(op, "NULL buffer");
   if (!aligned(x, dtype_size(dtype))) return bad(op, "misaligned x");
   const int64_t ld = row_bytes(k);
+  Launch go{op, (hipStream_t)hip_stream};
   if (fused_rows(m, k)) {
     I8Args p{nullptr, weight, nullptr, weight_scale, ld, ld, m, (int)n, (int)ld, bias, act, residual, residual_stride, y, y_stride};
     with_type(dtype, [&](auto t) {
       with_type(y_dtype, [&](auto u) {
         typedef decltype(t) T;
         typedef decltype(u) Y;
-        const dim3 g((unsigned)((n + 15) / 16));
+        const int64_t blocks = (n + 15) / 16;
         const size_t lds = (size_t)(m * ld);
-        hipStream_t s = (hipStream_t)hip_stream;
-        if (m <= 16) i8_fused_rows<T, Y, 1><<<g, dim3(512), lds, s>>>(p, static_cast<const T*>(x), x_stride, (int)k);
-        else i8_fused_rows<T, Y, 2><<<g, dim3(512), lds, s>>>(p, static_cast<const T*>(x), x_stride, (int)k);
+        if (m <= 16) go.run(i8_fused_rows<T, Y, 1>, blocks, 1, 512, lds, p, static_cast<const T*>(x), x_stride, (int)k);
+        else go.run(i8_fused_rows<T, Y, 2>, blocks, 1, 512, lds, p, static_cast<const T*>(x), x_stride, (int)k);
       });
     });
-    return launched(op);
+    return go.rc;
   }
   if (!workspace || workspace_bytes < linear_workspace(m, k)) return bad(op, "workspace too small");
   if (!aligned(workspace, 16)) return bad(op, "misaligned workspace");
   int8_t* q = static_cast<int8_t*>(workspace);
   float* scale = reinterpret_cast<float*>(q + m * ld);
-  const int rq = quantize(op, x, dtype, m, k, x_stride, q, scale, (hipStream_t)hip_stream);
-  if (rq) return rq;
   I8Args p{q, weight, scale, weight_scale, ld, ld, m, (int)n, (int)ld, bias, act, residual, residual_stride, y, y_stride};
-  return matmul(op, p, y_dtype, (hipStream_t)hip_stream);
+  const int rm = matmul({op, go.s, true}, p, y_dtype);      // a product that does not fit a launch is refused before the first
+  if (rm) return rm;
+  const int rq = quantize(go, x, dtype, m, k, x_stride, q, scale);
+  return rq ? rq : matmul(go, p, y_dtype);
 } OP_CATCH
 
 int pclseg_op_label_logprobs_workspace(int64_t rows, int64_t classes, int top_k, size_t* bytes) try {
@@ -295,12 +315,12 @@ int pclseg_op_label_logprobs(const void* logits, int dtype, int64_t rows, int64_
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return bad(op, "workspace too small or misaligned");
   ScoreArgs a{logits, rows, stride, (int)classes, labels, label_bytes == 8, allowed, allowed_stride, top_k,
               logprob, entropy, lse, top_ids, top_logprobs, workspace, score_segs(rows, classes)};
-  if (rows > kMaxBlocks || rows * a.segs > kMaxBlocks) return bad_shape(op, "more rows than a launch has blocks");
+  Launch go{op, (hipStream_t)hip_stream};
   with_type(dtype, [&](auto t) {
-    if (allowed) launch_score<decltype(t), true>(a, (hipStream_t)hip_stream);
-    else launch_score<decltype(t), false>(a, (hipStream_t)hip_stream);
+    if (allowed) launch_score<decltype(t), true>(a, go);
+    else launch_score<decltype(t), false>(a, go);
   });
-  return launched(op);
+  return go.rc;
 } OP_CATCH
 
 int pclseg_op_label_logprobs_grad(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t stride,
@@ -339,22 +359,20 @@ int pclseg_op_label_logprobs_grad(const void* logits, int dtype, int64_t rows, i
   }
   a.magic = (uint32_t)(((1u << 20) + a.vecs - 1) / a.vecs);
   const int64_t blocks = a.cuts > 1 ? rows * a.cuts : (rows + a.rows_per_block - 1) / a.rows_per_block;
-  if (rows > kMaxBlocks * 256 || blocks > kMaxBlocks) return bad_shape(op, "more rows than a launch has blocks");
+  Launch go{op, (hipStream_t)hip_stream};
   with_type(dtype, [&](auto t) {
     typedef decltype(t) T;
-    const dim3 g((unsigned)blocks), b(256);
-    hipStream_t s = (hipStream_t)hip_stream;
     if (allowed) {
-      if (ni == 1) logprob_grad<T, true, 1><<<g, b, 0, s>>>(a);
-      else if (ni == 2) logprob_grad<T, true, 2><<<g, b, 0, s>>>(a);
-      else logprob_grad<T, true, 4><<<g, b, 0, s>>>(a);
+      if (ni == 1) go(logprob_grad<T, true, 1>, blocks, 256, a);
+      else if (ni == 2) go(logprob_grad<T, true, 2>, blocks, 256, a);
+      else go(logprob_grad<T, true, 4>, blocks, 256, a);
     } else {
-      if (ni == 1) logprob_grad<T, false, 1><<<g, b, 0, s>>>(a);
-      else if (ni == 2) logprob_grad<T, false, 2><<<g, b, 0, s>>>(a);
-      else logprob_grad<T, false, 4><<<g, b, 0, s>>>(a);
+      if (ni == 1) go(logprob_grad<T, false, 1>, blocks, 256, a);
+      else if (ni == 2) go(logprob_grad<T, false, 2>, blocks, 256, a);
+      else go(logprob_grad<T, false, 4>, blocks, 256, a);
     }
   });
-  return launched(op);
+  return go.rc;
 } OP_CATCH
 
 }  // extern "C"

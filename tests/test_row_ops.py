@@ -115,6 +115,31 @@ def test_label_logprobs_grad_refuses(change, code, word):
   _refused("pclseg_op_label_logprobs_grad", list({**GRAD, **change}.values()), code, word)
 
 
+FAR = P + (1 << 46)      # a gradient that does not overlap the logits
+
+
+# a launch has fewer than 2^32 threads along an axis: a size that does not fit, for each way of sharing rows out
+@pytest.mark.parametrize("fn,call", [
+  ("pclseg_op_quantize_rows", dict(QUANT, rows=(1 << 29) + 1)),                                     # 8 lanes a row
+  ("pclseg_op_quantize_rows", dict(QUANT, rows=(1 << 26) + 1, cols=257, x_stride=257)),             # 64
+  ("pclseg_op_quantize_rows", dict(QUANT, rows=1 << 24, cols=2049, x_stride=2049)),                 # 256
+  ("pclseg_op_matmul_i8", dict(MATMUL, m=1, n=1 << 27, y_stride=1 << 27)),                          # 512 threads, 16 channels
+  ("pclseg_op_matmul_i8", dict(MATMUL, m=1 << 30, k=65)),                                           # 256 threads, 64 rows
+  ("pclseg_op_matmul_i8", dict(MATMUL, m=1 << 31)),                                                 # 256 threads, 128 rows
+  ("pclseg_op_matmul_i8", dict(MATMUL, m=1 << 30, n=256, y_stride=256)),                            # 256 threads, 128x128
+  ("pclseg_op_linear_i8", dict(LINEAR, m=1, n=1 << 27, y_stride=1 << 27)),
+  ("pclseg_op_linear_i8", dict(LINEAR, m=(1 << 29) + 1, workspace_bytes=1 << 40)),                  # the quantisation
+  ("pclseg_op_linear_i8", dict(LINEAR, m=1 << 28, n=1024, y_stride=1024, workspace_bytes=1 << 40)),   # the product
+  ("pclseg_op_label_logprobs", dict(SCORE, rows=(1 << 32) + 1)),                                    # a thread a row
+  ("pclseg_op_label_logprobs", dict(SCORE, rows=(1 << 29) + 1, classes=33, stride=33)),             # 8 lanes
+  ("pclseg_op_label_logprobs", dict(SCORE, rows=1 << 26, classes=2049, stride=2049)),               # a wave
+  ("pclseg_op_label_logprobs_grad", dict(GRAD, rows=1 << 40, grad=FAR)),
+  ("pclseg_op_label_logprobs_grad", dict(GRAD, rows=1 << 24, classes=4096, stride=4096, grad=FAR, grad_stride=4096)),
+])
+def test_more_than_a_launch_holds_is_refused(fn, call):
+  _refused(fn, list(call.values()), -2, "launch")
+
+
 def test_no_rows_is_no_work():
   lib = E.load_library()
   assert lib.pclseg_op_quantize_rows(*{**QUANT, "rows": 0, "x": None}.values()) == 0
