@@ -347,7 +347,7 @@ int64_t pclseg_i8_row_bytes(int64_t k);
 
 /* Symmetric quantisation, one scale per row: scale = max|x| / 127 (float32), q = round(x / scale), ties to even.
  *   x      [rows, cols] dtype, row stride x_stride elements
- *   q      int8 [rows, pclseg_i8_row_bytes(cols)], 8-byte aligned, written whole: zeros behind cols
+ *   q      int8 [rows, pclseg_i8_row_bytes(cols)], 8-byte aligned, written whole: zeros behind cols; does not overlap x
  *   scale  float32 [rows]: 0 for a row of zeros, NaN (codes 0) for a row that holds an infinity or a NaN */
 int pclseg_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_stride, int8_t* q,
                             float* scale, void* hip_stream);
@@ -356,13 +356,15 @@ int pclseg_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols
  * with exact int32 sums.
  *   a      int8 [m, pclseg_i8_row_bytes(k)], b likewise [n, ...], 16-byte aligned; the bytes behind k are 0 in both
  *   act    0 none / 1 relu / 2 leaky(0.1) / 3 sigmoid
- *   y, residual [m, n] dtype, row strides in elements; residual and bias (float32 [n]) may be NULL.  y may be residual. */
+ *   y, residual [m, n] dtype, row strides in elements; residual and bias (float32 [n]) may be NULL.  y may be residual
+ *          (the same address and stride) and does not overlap it otherwise. */
 int pclseg_op_matmul_i8(const int8_t* a, const float* a_scale, const int8_t* b, const float* b_scale, int64_t m,
                         int64_t n, int64_t k, const float* bias, int act, const void* residual, int64_t residual_stride,
                         void* y, int64_t y_stride, int dtype, void* hip_stream);
 
 /* The layer on float rows: op_quantize_rows of x into the workspace, then op_matmul_i8 (a few rows: one launch, no workspace).
- *   x      [m, k] dtype; weight codes and scales as for b above
+ *   x      [m, k] dtype, does not overlap y (refused; rows side by side in one buffer do not overlap); weight codes and scales
+ *          as for b above
  *   workspace  pclseg_op_linear_i8_workspace bytes (may be 0), 16-byte aligned; two calls in flight need two */
 int pclseg_op_linear_i8_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes);
 int pclseg_op_linear_i8(const void* x, int dtype, int64_t x_stride, const int8_t* weight, const float* weight_scale,

@@ -27,6 +27,20 @@ int launched(const char* op) {
 bool dtype_ok(int d) { return d == PCLSEG_F32 || d == PCLSEG_BF16 || d == PCLSEG_F16; }
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 size_t dtype_size(int d) { return d == PCLSEG_F32 ? 4 : 2; }
+
+// Rows of `cols` elements of `size` bytes, `stride` elements apart.
+struct Rows { const void* p; int64_t stride, cols, size; };
+// Do two arrays of m >= 1 rows share a byte?  With equal strides in bytes the rows may lie side by side in one buffer; with
+// different ones address ranges that meet count as shared.
+bool overlap(const Rows& a, const Rows& b, int64_t m) {
+  typedef unsigned __int128 U;
+  const U a0 = (uintptr_t)a.p, b0 = (uintptr_t)b.p, as = (U)a.stride * (U)a.size, bs = (U)b.stride * (U)b.size;
+  const U aw = (U)(a.cols * a.size), bw = (U)(b.cols * b.size), above = (U)(m - 1);
+  if (a0 + above * as + aw <= b0 || b0 + above * bs + bw <= a0) return false;
+  if (m == 1 || as != bs) return true;
+  const U d = b0 >= a0 ? (b0 - a0) % as : (as - (a0 - b0) % as) % as;      // b's rows begin d bytes into a's
+  return d < aw || d + bw > as;
+}
 constexpr int64_t kMaxBlocks = 0x7fffffff, kMaxThreads = 0xffffffff;      // of a launch: blocks, and threads along an axis
 // columns are counted in 32 bits, with room for a block's share behind the last; products of rows and columns stay below 2^63
 constexpr int64_t kMaxRows = (int64_t)1 << 40, kMaxColumns = 1 << 30;
@@ -138,6 +152,11 @@ int check_product(const char* op, int64_t m, int64_t n, int64_t k, const int8_t*
   if (!aligned(b, 16)) return bad(op, "codes must be 16-byte aligned");
   if (y_stride < n || (residual && residual_stride < n)) return bad_shape(op, "row stride smaller than n");
   if (!aligned(y, dtype_size(dtype)) || !aligned(residual, dtype_size(dtype))) return bad(op, "misaligned y or residual");
+  // an element's residual is read by the lane that stores it: y itself is fine, any other overlap is a race
+  const int64_t sz = (int64_t)dtype_size(dtype);
+  if (m && residual && !(residual == y && residual_stride == y_stride) &&
+      overlap({residual, residual_stride, n, sz}, {y, y_stride, n, sz}, m))
+    return bad(op, "y overlaps the residual without being it");
   return PCLSEG_OK;
 }
 
@@ -228,6 +247,10 @@ int pclseg_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols
   if (rows == 0) return PCLSEG_OK;
   if (!x || !q || !scale) return bad(op, "NULL buffer");
   if (!aligned(x, dtype_size(dtype)) || !aligned(q, 8)) return bad(op, "misaligned x or codes");
+  const int rc = quantize({op, nullptr, true}, x, dtype, rows, cols, x_stride, q, scale);
+  if (rc) return rc;
+  const int64_t ld = row_bytes(cols);
+  if (overlap({x, x_stride, cols, (int64_t)dtype_size(dtype)}, {q, ld, ld, 1}, rows)) return bad(op, "codes overlap x");
   return quantize({op, (hipStream_t)hip_stream}, x, dtype, rows, cols, x_stride, q, scale);
 } OP_CATCH
 
@@ -267,8 +290,12 @@ int pclseg_op_linear_i8(const void* x, int dtype, int64_t x_stride, const int8_t
   if (!aligned(x, dtype_size(dtype))) return bad(op, "misaligned x");
   const int64_t ld = row_bytes(k);
   Launch go{op, (hipStream_t)hip_stream};
+  // few rows in one launch: every block reads all of x while others store y.  Refused for any number of rows alike, after the
+  // checks of sizes
+  const bool shared = overlap({x, x_stride, k, (int64_t)dtype_size(dtype)}, {y, y_stride, n, (int64_t)dtype_size(y_dtype)}, m);
   if (fused_rows(m, k)) {
     I8Args p{nullptr, weight, nullptr, weight_scale, ld, ld, m, (int)n, (int)ld, bias, act, residual, residual_stride, y, y_stride};
+    go.dry = shared;
     with_type(dtype, [&](auto t) {
       with_type(y_dtype, [&](auto u) {
         typedef decltype(t) T;
@@ -279,7 +306,7 @@ int pclseg_op_linear_i8(const void* x, int dtype, int64_t x_stride, const int8_t
         else go.run(i8_fused_rows<T, Y, 2>, blocks, 1, 512, lds, p, static_cast<const T*>(x), x_stride, (int)k);
       });
     });
-    return go.rc;
+    return go.rc ? go.rc : shared ? bad(op, "y overlaps x") : PCLSEG_OK;
   }
   if (!workspace || workspace_bytes < linear_workspace(m, k)) return bad(op, "workspace too small");
   if (!aligned(workspace, 16)) return bad(op, "misaligned workspace");
@@ -288,8 +315,10 @@ int pclseg_op_linear_i8(const void* x, int dtype, int64_t x_stride, const int8_t
   I8Args p{q, weight, scale, weight_scale, ld, ld, m, (int)n, (int)ld, bias, act, residual, residual_stride, y, y_stride};
   const int rm = matmul({op, go.s, true}, p, y_dtype);      // a product that does not fit a launch is refused before the first
   if (rm) return rm;
+  go.dry = shared;
   const int rq = quantize(go, x, dtype, m, k, x_stride, q, scale);
-  return rq ? rq : matmul(go, p, y_dtype);
+  if (rq) return rq;
+  return shared ? bad(op, "y overlaps x") : matmul(go, p, y_dtype);
 } OP_CATCH
 
 int pclseg_op_label_logprobs_workspace(int64_t rows, int64_t classes, int top_k, size_t* bytes) try {

@@ -698,3 +698,24 @@ def test_evaluation_prints_the_likelihood(cuda, tmp_path, capsys):
   want = [-logp[keep].gather(1, lab[keep][:, None]).mean().item(), -p[keep].sum(-1).mean().item()]
   assert all(abs(a - b) <= 1e-4 for a, b in zip(got, want))      # logits of two runs of the network agree to about 1e-5
   assert torch.equal(torch.from_numpy(np.asarray(preds)), torch.from_numpy(np.asarray(model.predict_raw(samples[..., :5]))))
+
+
+@pytest.mark.parametrize("m", [1, 32, 33, 300])
+def test_linear_i8_rows_side_by_side(cuda, m):
+  """Input, residual and output as columns of one buffer share no element; a residual may be the output."""
+  from pclsegmentation_amd import engine as E
+  lib, stream = E.load_library(), E.stream_handle(cuda)
+  k, n = 100, 40
+  w = ops.quantize_rows(rnd(1, n, k).float().to(cuda))
+  buf = rnd(2, m, k + 2 * n + 3).float().to(cuda)
+  x, res = buf[:, :k].contiguous(), buf[:, k:k + n].contiguous()
+  want = ops.linear_i8(x, w, residual=res)
+  work = torch.empty(m * 132, dtype=torch.uint8, device=cuda)
+  ld = buf.shape[1]
+  call = lambda r, y: E.check(lib.pclseg_op_linear_i8(buf.data_ptr(), 0, ld, w.data.data_ptr(), w.scale.data_ptr(), m, n, k, None, 0,
+                                                      r, ld, y, ld, 0, work.data_ptr(), work.numel(), stream))
+  tail = buf[:, k + 2 * n:].clone()
+  call(buf[:, k:].data_ptr(), buf[:, k + n:].data_ptr())
+  assert torch.equal(buf[:, k + n:k + 2 * n], want)
+  call(buf[:, k:].data_ptr(), buf[:, k:].data_ptr())
+  assert torch.equal(buf[:, k:k + n], want) and torch.equal(buf[:, :k], x) and torch.equal(buf[:, k + 2 * n:], tail)

@@ -235,3 +235,44 @@ def test_calls_run_with_the_tensors_device_current(monkeypatch):
   state["current"] = 1
   ops._call(Dev, launch, 6)
   assert state == {"current": 1, "during": (1, 6, 77)}
+
+
+# ---- outputs that share memory with inputs: one block stores while another still reads
+BIG = (ctypes.c_uint8 * (1 << 16))()
+Q = (ctypes.addressof(BIG) + 255) // 256 * 256
+
+
+@pytest.mark.parametrize("m", [1, 2, 32, 33, 70])
+@pytest.mark.parametrize("x,x_stride,y,y_stride,y_dtype", [
+  (Q, 8, Q, 8, 0),                        # in place
+  (Q, 8, Q + 16, 8, 0),                   # y begins inside x's first row
+  (Q + 16, 8, Q, 8, 0),
+  (Q, 20, Q + 28, 20, 0),                 # rows of one buffer, x in columns 0..7, y in 7..14
+  (Q + 28, 20, Q, 20, 0),
+  (Q, 20, Q + 56, 20, 0),                 # y in columns 14..21: its end is the next row's x (one row: behind it)
+  (Q, 20, Q, 40, 1),                      # 16-bit outputs over float inputs, the same bytes a row
+  (Q, 8, Q + 12, 9, 0),                   # different strides
+])
+def test_linear_i8_refuses_an_output_over_its_input(m, x, x_stride, y, y_stride, y_dtype):
+  if m == 1 and y == Q + 56:
+    pytest.skip("one row: y lies behind x")
+  change = dict(x=x, x_stride=x_stride, y=y, y_stride=y_stride, y_dtype=y_dtype, m=m, n=8, workspace=P, workspace_bytes=1 << 20)
+  _refused("pclseg_op_linear_i8", list({**LINEAR, **change}.values()), -1, "overlaps x")
+
+
+@pytest.mark.parametrize("fn,base", [("pclseg_op_matmul_i8", MATMUL), ("pclseg_op_linear_i8", dict(LINEAR, x=P + 2048, k=8))])
+@pytest.mark.parametrize("residual,stride", [(Q + 4, 3), (Q + 36, 3), (Q, 4), (Q + 28, 9), (Q + 4, 9)])
+def test_products_refuse_a_residual_partly_under_the_output(fn, base, residual, stride):
+  """y may be the residual; shifted or with another stride an element's residual may be gone before it is read."""
+  change = dict(m=4, n=3, y=Q, y_stride=9 if stride == 9 else 3, residual=residual, residual_stride=stride)
+  change["y_dtype" if "y_dtype" in base else "dtype"] = 0
+  if residual == Q + 36:
+    change.update(y=Q + 32)
+  if (residual, stride) == (Q + 28, 9):
+    change.update(n=8, y=Q)               # columns 7..14 of the residual under columns 0..7 of y
+  _refused(fn, list({**base, **change}.values()), -1, "overlaps the residual")
+
+
+def test_quantize_rows_refuses_codes_over_its_input():
+  for x, q in ((Q, Q), (Q + 32, Q), (Q, Q + 8), (Q, Q + 56)):
+    _refused("pclseg_op_quantize_rows", list({**QUANT, "x": x, "q": q}.values()), -1, "codes overlap")
