@@ -368,15 +368,13 @@ int pclseg_op_label_logprobs_grad(const void* logits, int dtype, int64_t rows, i
   if (rows == 0) return PCLSEG_OK;
   if (!lse || !grad) return bad(op, "NULL buffer");
   if (!aligned(grad, dtype_size(dtype))) return bad(op, "misaligned grad");
-  const uintptr_t sz = dtype_size(dtype), x0 = (uintptr_t)logits, g0 = (uintptr_t)grad;
-  const uintptr_t x1 = x0 + ((uintptr_t)(rows - 1) * stride + classes) * sz;
-  const uintptr_t g1 = g0 + ((uintptr_t)(rows - 1) * grad_stride + classes) * sz;
-  if (g0 < x1 && x0 < g1) return bad(op, "grad overlaps the logits");
+  const int64_t sz = (int64_t)dtype_size(dtype);
+  if (overlap({logits, stride, classes, sz}, {grad, grad_stride, classes, sz}, rows)) return bad(op, "grad overlaps the logits");
   GradArgs a{logits, rows, stride, (int)classes, labels, label_bytes == 8, allowed, allowed_stride, lse, entropy,
              d_logprob, d_entropy, top_ids, d_top, d_top ? top_k : 0, grad, grad_stride, 1, 1, 1, 0};
   // a block takes 256 NI 16-byte pieces: that many of a long row, or whole short rows.  NI grows while the blocks are more
   // than the 2048 that run at once
-  const int64_t vec = 16 / (int64_t)sz, nvec = (classes + vec - 1) / vec;
+  const int64_t vec = 16 / sz, nvec = (classes + vec - 1) / vec;
   const int64_t all = std::min<int64_t>(rows, kMaxBlocks) * nvec;
   const int ni = all <= 2048 * 256 ? 1 : all <= 2 * 2048 * 256 ? 2 : 4;
   if (nvec > 256 * ni) {

@@ -719,3 +719,18 @@ def test_linear_i8_rows_side_by_side(cuda, m):
   assert torch.equal(buf[:, k + n:k + 2 * n], want)
   call(buf[:, k:].data_ptr(), buf[:, k:].data_ptr())
   assert torch.equal(buf[:, k:k + n], want) and torch.equal(buf[:, :k], x) and torch.equal(buf[:, k + 2 * n:], tail)
+
+
+@pytest.mark.parametrize("rows,v", [(1, 20), (5, 21), (300, 20), (3, 9001)])
+def test_label_logprobs_grad_beside_the_logits(cuda, rows, v):
+  """The logits and their gradient as the two halves of one buffer's rows share no element."""
+  from pclsegmentation_amd import engine as E
+  buf = torch.full((rows, 2 * v + 3), 5.0, device=cuda)
+  buf[:, 1:1 + v] = rnd(1, rows, v).float().to(cuda)
+  logits, labels, d = buf[:, 1:1 + v].contiguous(), labels_for(rows, v, 1).to(cuda), torch.ones(rows, device=cuda)
+  fwd = ops.label_logprobs(logits, labels)
+  E.check(E.load_library().pclseg_op_label_logprobs_grad(
+    buf[:, 1:].data_ptr(), 0, rows, v, 2 * v + 3, labels.data_ptr(), 4, None, 0, fwd.lse.data_ptr(), None, d.data_ptr(), None, None,
+    None, 0, buf[:, 1 + v:].data_ptr(), 2 * v + 3, E.stream_handle(cuda)))
+  assert torch.equal(buf[:, 1 + v:1 + 2 * v], ops.label_logprobs_grad(logits, labels, fwd.lse, d_logprob=d))
+  assert torch.equal(buf[:, 1:1 + v], logits) and (buf[:, 0] == 5).all() and (buf[:, 1 + 2 * v:] == 5).all()

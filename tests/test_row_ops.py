@@ -276,3 +276,17 @@ def test_products_refuse_a_residual_partly_under_the_output(fn, base, residual, 
 def test_quantize_rows_refuses_codes_over_its_input():
   for x, q in ((Q, Q), (Q + 32, Q), (Q, Q + 8), (Q, Q + 56)):
     _refused("pclseg_op_quantize_rows", list({**QUANT, "x": x, "q": q}.values()), -1, "codes overlap")
+
+
+@pytest.mark.parametrize("grad", [Q + 12, Q + 20, Q + 8, Q - 12 + 32])
+def test_label_logprobs_grad_refuses_a_gradient_over_the_logits(grad):
+  """Rows of 4 floats, 8 apart: a gradient that begins anywhere but 16 bytes into the logits' rows shares some of them."""
+  _refused("pclseg_op_label_logprobs_grad", list({**GRAD, "logits": Q, "stride": 8, "grad": grad, "grad_stride": 8, "rows": 5}.values()),
+           -1, "overlaps the logits")
+
+
+def test_label_logprobs_grad_far_strides():
+  """Strides whose products with the rows pass 64 bits are compared as they are: this gradient lies 2^46 bytes behind the logits'
+  first row, inside their range."""
+  _refused("pclseg_op_label_logprobs_grad", list({**GRAD, "stride": 1 << 60, "rows": 1 << 39, "grad": FAR, "grad_stride": 4}.values()),
+           -1, "overlaps the logits")
