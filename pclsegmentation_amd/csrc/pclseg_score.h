@@ -4,8 +4,11 @@
 //   M = max x,  S = sum e^(x-M),  T = sum e^(x-M) (x-M)          (sums over A)
 //   lse = M + ln S,   logprob = (x[label] - M) - ln S,   entropy = ln S - T / S
 // (M, S, T) of two disjoint parts join with M = max(M1, M2), d = Mi - M <= 0:  S += Si e^d, T += e^d (Ti + d Si), so a row
-// is read once and can be cut anywhere.  All of it is float32: the terms of S and T have one sign and at most a few roundings
-// per element, 2^-24 each, and the differences x - M are taken before the exponential, so large logits lose nothing.
+// is read once and can be cut anywhere.  All of it is float32: the terms of S and T have one sign, and the differences x - M are
+// taken before the exponential, so large logits lose nothing.  A lane adds up to 32 elements one after the other; such sums of
+// a long row's pieces are added with the rounding of each addition carried into the next, so that a sum is a few tens of
+// roundings from the exact one, 2^-24 each, whatever the row's length (131072 terms one after the other, most of them
+// alike: 450 roundings off).
 // The exponential is v_exp_f32 on (x-M) log2 e: both roundings are relative to an exponent of at most a few tens.
 // Terms with x - M < -200 are 0 in float32; the clamp of the second factor at -200 keeps 0 * inf out of T.
 //
@@ -59,6 +62,13 @@ __device__ __forceinline__ void stat_add(Stat& a, float x) {   // a.m >= x unles
   const float z = x - a.m, e = fast_exp(z);
   a.s += e;
   a.t = fmaf(e, fmaxf(z, -200.f), a.t);
+}
+
+// sum += v with the rounding of the last addition: sum - lost is the sum
+__device__ __forceinline__ void add_carried(float& sum, float& lost, float v) {
+  const float y = v - lost, u = sum + y;
+  lost = (u - sum) - y;
+  sum = u;
 }
 
 // a row's results.  s == 0: nothing is allowed (or every allowed logit is -inf); s NaN: an allowed logit is NaN or +inf, the
@@ -388,6 +398,7 @@ __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
   const int p0 = (int)((int64_t)pieces * seg / a.segs), p1 = (int)((int64_t)pieces * (seg + 1) / a.segs);
 
   Stat st{kLowest, 0.f, 0.f};
+  float lost_s = 0.f, lost_t = 0.f;      // of st.s and st.t
   Key list = 0;
   // An element is offered to the list when it is at least thr.  A wave that has seen top_k elements of at least b takes the
   // next float above b: its later pieces hold higher indices, an equal value stays behind.  The other waves' b hold as they
@@ -469,13 +480,19 @@ __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
         }
       }
     }
-    st = stat_shift(st, fmaxf(st.m, lane_max));
+    const Stat lost = stat_shift(Stat{st.m, lost_s, lost_t}, fmaxf(st.m, lane_max));
+    st = stat_shift(st, lost.m);
+    lost_s = lost.s;
+    lost_t = lost.t;
+    Stat piece{st.m, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) stat_add(st, x[v][e]);
+      for (int e = 0; e < VEC; ++e) stat_add(piece, x[v][e]);
       __builtin_amdgcn_sched_barrier(0);      // 8 exponentials in flight at a time: more would only cost registers, and waves
     }
+    add_carried(st.s, lost_s, piece.s);
+    add_carried(st.t, lost_t, piece.t);
     if constexpr (TOP) {
       if (some) {
         // a lane's only offer is its maximum; several are read again (a register cannot be chosen by a lane)
@@ -500,6 +517,8 @@ __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
     }
   }
   if (TOP && n) flush(n);
+  st.s -= lost_s;
+  st.t -= lost_t;
   st = wave_join(st);
   if (lane == 0) stats[wave] = st;
   if constexpr (TOP) lists[wave][lane] = list;

@@ -734,3 +734,24 @@ def test_label_logprobs_grad_beside_the_logits(cuda, rows, v):
     None, 0, buf[:, 1 + v:].data_ptr(), 2 * v + 3, E.stream_handle(cuda)))
   assert torch.equal(buf[:, 1 + v:1 + 2 * v], ops.label_logprobs_grad(logits, labels, fwd.lse, d_logprob=d))
   assert torch.equal(buf[:, 1:1 + v], logits) and (buf[:, 0] == 5).all() and (buf[:, 1 + 2 * v:] == 5).all()
+
+
+@pytest.mark.parametrize("rows,v", [(2100, 131072), (40, 1 << 20), (1, 1 << 20), (300, 40000)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_long_rows_of_like_terms(cuda, rows, v, dtype):
+  """Terms that are all alike round the same way at every addition: the bound counts 32 of a lane's piece, 4 for the pieces
+  however many they are, 6 + 6 of the lanes and blocks, and none in proportion to the row's length.  The first 512 classes give
+  every lane an element above the others, whose terms are then no powers of two."""
+  j = torch.arange(v, dtype=torch.float64)
+  kinds = torch.stack([torch.where((j < 512) & (j % 4 == 0), 0.0, -5.0), torch.full((v,), 1.25, dtype=torch.float64),
+                       torch.where(j % 2 == 0, -3.0, -3.5) + 5.0 * (j < 512) * (j % 4 == 0),
+                       torch.where(j == 7, 4.0, -4.0)])
+  kinds = kinds[:min(rows, 4)]
+  ref = score64(kinds, None, 0, None)
+  x = kinds.to(dtype).to(cuda).repeat((rows + len(kinds) - 1) // len(kinds), 1)[:rows]
+  got = ops.label_logprobs(x)
+  which = torch.arange(rows) % len(kinds)
+  a, b, logs, m, lse, h = [ref[t].abs()[which] for t in ("a", "b", "logs", "m", "lse", "entropy")]
+  rel_s = U * (48 + 4 + 4 * a)
+  close(got.lse, ref["lse"][which], rel_s + 2 * U * logs + U * (m + lse))
+  close(got.entropy, ref["entropy"][which], rel_s + 2 * U * logs + rel_s * a + U * (4 * b + (8 + 48) * a + h))
