@@ -4,7 +4,8 @@
 //   M = max x,  S = sum e^(x-M),  T = sum e^(x-M) (x-M)          (sums over A)
 //   lse = M + ln S,   logprob = (x[label] - M) - ln S,   entropy = ln S - T / S
 // (M, S, T) of two disjoint parts join with M = max(M1, M2), d = Mi - M <= 0:  S += Si e^d, T += e^d (Ti + d Si), so a row
-// is read once and can be cut anywhere.  All of it is float32: the terms of S and T have one sign, and the differences x - M are
+// is read once and can be cut anywhere.  Rows are often decided: S = 1 + rest with a rest of 2^-10 would leave ln S 14 bits.
+// The maximum's term is kept apart from the others (one, s below), and ln S = ln(1 + rest) keeps the bits of the rest.  All of it is float32: the terms of S and T have one sign, and the differences x - M are
 // taken before the exponential, so large logits lose nothing.  A lane adds up to 32 elements one after the other; such sums of
 // a long row's pieces are added with the rounding of each addition carried into the next, so that a sum is a few tens of
 // roundings from the exact one, 2^-24 each, whatever the row's length (131072 terms one after the other, most of them
@@ -45,25 +46,17 @@ struct ScoreArgs {
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
-struct Stat { float m, s, t; };   // maximum, sum of e^(x-m), sum of e^(x-m)(x-m)
+// S = one + s: one is 1 where the term of a maximum is left out of s, else 0; t holds all of T
+struct Stat { float m, one, s, t; };
 
 __device__ __forceinline__ float fast_exp(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
 
-__device__ __forceinline__ Stat stat_shift(const Stat& a, float m) {   // the same sums relative to m >= a.m
-  const float d = fmaxf(a.m - m, -200.f), f = fast_exp(d);
-  return Stat{m, a.s * f, f * fmaf(d, a.s, a.t)};
+// What elements are worth that were summed relative to the maximum m: s the terms, below the terms less than 1 (a term of 1
+// has the fraction 0), t.  The two sums differ by the count of maxima; a single one is kept apart.
+__device__ __forceinline__ Stat stat_of(float m, float s, float below, float t) {
+  const bool one = rintf(s - below) == 1.f;
+  return Stat{m, one ? 1.f : 0.f, one ? below : s, t};
 }
-__device__ __forceinline__ Stat stat_join(const Stat& a, const Stat& b) {
-  const float m = fmaxf(a.m, b.m);
-  const Stat p = stat_shift(a, m), q = stat_shift(b, m);
-  return Stat{m, p.s + q.s, p.t + q.t};
-}
-__device__ __forceinline__ void stat_add(Stat& a, float x) {   // a.m >= x unless x is -inf, +inf or NaN
-  const float z = x - a.m, e = fast_exp(z);
-  a.s += e;
-  a.t = fmaf(e, fmaxf(z, -200.f), a.t);
-}
-
 // sum += v with the rounding of the last addition: sum - lost is the sum
 __device__ __forceinline__ void add_carried(float& sum, float& lost, float v) {
   const float y = v - lost, u = sum + y;
@@ -71,17 +64,19 @@ __device__ __forceinline__ void add_carried(float& sum, float& lost, float v) {
   sum = u;
 }
 
-// a row's results.  s == 0: nothing is allowed (or every allowed logit is -inf); s NaN: an allowed logit is NaN or +inf, the
+// a row's results.  S == 0: nothing is allowed (or every allowed logit is -inf); S NaN: an allowed logit is NaN or +inf, the
 // row has no distribution and every float result is NaN.
 struct RowOut { float m, logs, lse, entropy; bool empty, bad; };
 __device__ __forceinline__ RowOut row_out(const Stat& a) {
   RowOut o;
-  o.empty = a.s == 0.f;
-  o.bad = !(a.s < __builtin_inff());
+  const float sum = a.one + a.s;
+  o.empty = sum == 0.f;
+  o.bad = !(sum < __builtin_inff());
   o.m = a.m;
-  o.logs = logf(a.s);
+  // ln(one + s) of the rounded sum, and what the rounding left, to first order: the bits of a small s stay
+  o.logs = logf(sum) + (a.s - (sum - a.one)) * __builtin_amdgcn_rcpf(sum);
   o.lse = o.empty ? neg_inf() : (o.bad ? __builtin_nanf("") : a.m + o.logs);
-  o.entropy = o.empty ? 0.f : (o.bad ? __builtin_nanf("") : o.logs - a.t / a.s);
+  o.entropy = o.empty ? 0.f : (o.bad ? __builtin_nanf("") : o.logs - a.t / sum);
   return o;
 }
 __device__ __forceinline__ float row_logprob(const RowOut& o, float x) {
@@ -167,25 +162,17 @@ __global__ __launch_bounds__(256, CAP <= 20 ? 6 : 4) void logprob_thread_rows(Sc
   load_tail<T, MASK>(src, mask, CAP - VEC, a.classes, x + CAP - VEC);
 #pragma unroll
   for (int v = 0; v + 1 < NV; ++v) raw[v].expand(x + v * VEC);
-  Stat st{kLowest, 0.f, 0.f};
+  float top = kLowest, sum = 0.f, below = 0.f, t = 0.f;
 #pragma unroll
-  for (int j = 0; j < CAP; ++j) st.m = fmaxf(st.m, x[j]);
-  // Rows this short are often decided: S = 1 + rest with a rest of 2^-10 would leave the logarithm 14 bits.  The terms below 1
-  // are summed by themselves (the fraction of a term of 1, the maximum, is 0); the two sums differ by the count of maxima.
-  float rest = 0.f;
+  for (int j = 0; j < CAP; ++j) top = fmaxf(top, x[j]);
 #pragma unroll
   for (int j = 0; j < CAP; ++j) {
-    const float z = x[j] - st.m, e = fast_exp(z);
-    st.s += e;
-    rest += __builtin_amdgcn_fractf(e);
-    st.t = fmaf(e, fmaxf(z, -200.f), st.t);
+    const float z = x[j] - top, e = fast_exp(z);
+    sum += e;
+    below += __builtin_amdgcn_fractf(e);
+    t = fmaf(e, fmaxf(z, -200.f), t);
   }
-  RowOut o = row_out(st);
-  if (!o.empty && !o.bad && rintf(st.s - rest) == 1.f) {
-    o.logs = log1pf(rest);
-    o.lse = st.m + o.logs;
-    o.entropy = o.logs - st.t / (1.f + rest);
-  }
+  const RowOut o = row_out(stat_of(top, sum, below, t));
   write_row<T>(a, row, o);
   if (a.top_k == 0) return;
   int32_t* ids = a.top_ids + row * a.top_k;
@@ -274,29 +261,42 @@ __global__ __launch_bounds__(256) void logprob_group_rows(ScoreArgs a) {
     if ((v + 1) * G * VEC <= a.classes) raw[v].expand(x[v]);
     else if (v < nv) load_tail<T, MASK>(src, mask, (v * G + g) * VEC, a.classes, x[v]);
   }
-  Stat st{kLowest, 0.f, 0.f};
+  if (a.top_k) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (v < nv) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const bool b = x[v][e] > bv;
+          bv = b ? x[v][e] : bv;
+          bi = b ? (v * G + g) * VEC + e : bi;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (v < nv) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) bv = fmaxf(bv, x[v][e]);
+      }
+    }
+  }
+  const float top = group_max<G>(fmaxf(bv, kLowest));
+  float sum = 0.f, below = 0.f, t = 0.f;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     if (v < nv) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const bool b = x[v][e] > bv;
-        bv = b ? x[v][e] : bv;
-        bi = b ? (v * G + g) * VEC + e : bi;
+        const float z = x[v][e] - top, f = fast_exp(z);
+        sum += f;
+        below += __builtin_amdgcn_fractf(f);
+        t = fmaf(f, fmaxf(z, -200.f), t);
       }
     }
   }
-  st.m = group_max<G>(fmaxf(bv, kLowest));
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    if (v < nv) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) stat_add(st, x[v][e]);
-    }
-  }
-  st.s = group_sum<G>(st.s);
-  st.t = group_sum<G>(st.t);
-  const RowOut o = row_out(st);
+  const RowOut o = row_out(stat_of(top, group_sum<G>(sum), group_sum<G>(below), group_sum<G>(t)));
   if (g == 0 && live) write_row<T>(a, row, o);
   for (int k = 0; k < a.top_k; ++k) {
     // value first, then the lowest index: one key (-0 counts as 0)
@@ -368,16 +368,16 @@ __device__ __forceinline__ Key merge_lists(Key a, Key b_reversed, int lane) {
   return bitonic_clean(a > b_reversed ? a : b_reversed, lane);
 }
 
-__device__ __forceinline__ Stat wave_join(Stat st) {
-  const float m = group_max<64>(st.m);
-  st = stat_shift(st, m);
-  st.s = group_sum<64>(st.s);
-  st.t = group_sum<64>(st.t);
-  return st;
+// The statistics of G lanes together, in all of them.  The groups of a wave hold the same.  The first lane with the maximum keeps
+// its term apart, the others' terms are summed.
+template <int G> __device__ __forceinline__ Stat join(const Stat& st) {
+  const float m = group_max<G>(st.m), d = fmaxf(st.m - m, -200.f), f = fast_exp(d), all = st.one + st.s;
+  const bool keeps = __builtin_ctzll(__ballot(st.m == m)) == (int)(threadIdx.x & (G - 1));
+  return Stat{m, group_sum<G>(keeps ? st.one : 0.f), group_sum<G>(keeps ? st.s : all * f), group_sum<G>(f * fmaf(d, all, st.t))};
 }
 
 // a block's statistics and list in the workspace: [row * segs + seg]
-struct ScorePart { float m, s, t, pad; };
+struct ScorePart { float m, one, s, t; };
 
 template <typename T, int NW, bool TOP, bool MASK>
 __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
@@ -397,8 +397,8 @@ __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
   const int pieces = (int)(((int64_t)a.classes + pad + PIECE - 1) / PIECE);
   const int p0 = (int)((int64_t)pieces * seg / a.segs), p1 = (int)((int64_t)pieces * (seg + 1) / a.segs);
 
-  Stat st{kLowest, 0.f, 0.f};
-  float lost_s = 0.f, lost_t = 0.f;      // of st.s and st.t
+  // the wave's maximum (uniform), whether a term of it is apart, and each lane's sums relative to it
+  float top = kLowest, one = 0.f, sum = 0.f, sum_t = 0.f, lost = 0.f, lost_t = 0.f;
   Key list = 0;
   // An element is offered to the list when it is at least thr.  A wave that has seen top_k elements of at least b takes the
   // next float above b: its later pieces hold higher indices, an equal value stays behind.  The other waves' b hold as they
@@ -454,6 +454,22 @@ __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
       for (int e = 1; e < VEC; ++e) vec_max[v] = fmaxf(vec_max[v], x[v][e]);
       lane_max = fmaxf(lane_max, vec_max[v]);
     }
+    // A new maximum (about 4 of 25 pieces of a row in no order): what there was is taken relative to it, and its own term, in the
+    // first lane that holds it and there in the first 16 bytes, is kept out of that lane's sum (+inf stays in and makes it NaN)
+    int apart = -1;
+    bool keeps = false;
+    if (__ballot(lane_max > top)) {
+      const float m = group_max<64>(lane_max), d = fmaxf(top - m, -200.f), f = fast_exp(d), all = sum + (lane == 0 ? one : 0.f);
+      sum_t = f * fmaf(d, all, sum_t);
+      lost_t = f * fmaf(d, lost, lost_t);
+      sum = f * all;
+      lost *= f;
+      top = m;
+      one = 1.f;
+      keeps = m < __builtin_inff() && __builtin_ctzll(__ballot(lane_max == m)) == lane;
+#pragma unroll
+      for (int v = NV - 1; v >= 0; --v) apart = __ballot(keeps && vec_max[v] == m) ? v : apart;
+    }
     uint32_t offers = 0;      // bit v VEC + e: the element is offered to the list
     float least = thr, bound = kLowest;
     bool some = false;
@@ -480,19 +496,31 @@ __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
         }
       }
     }
-    const Stat lost = stat_shift(Stat{st.m, lost_s, lost_t}, fmaxf(st.m, lane_max));
-    st = stat_shift(st, lost.m);
-    lost_s = lost.s;
-    lost_t = lost.t;
-    Stat piece{st.m, 0.f, 0.f};
+    float s = 0.f, t = 0.f;
+    const float out = keeps ? top : __builtin_nanf("");
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (v == apart) {      // uniform; equal elements of the 16 bytes go together, all but one come back as terms of 1
+        s = keeps ? -1.f : 0.f;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          s += x[v][e] == out ? 1.f : 0.f;
+          x[v][e] = x[v][e] == out ? neg_inf() : x[v][e];
+        }
+      }
+    }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) stat_add(piece, x[v][e]);
+      for (int e = 0; e < VEC; ++e) {
+        const float z = x[v][e] - top, p = fast_exp(z);
+        s += p;
+        t = fmaf(p, fmaxf(z, -200.f), t);
+      }
       __builtin_amdgcn_sched_barrier(0);      // 8 exponentials in flight at a time: more would only cost registers, and waves
     }
-    add_carried(st.s, lost_s, piece.s);
-    add_carried(st.t, lost_t, piece.t);
+    add_carried(sum, lost, s);
+    add_carried(sum_t, lost_t, t);
     if constexpr (TOP) {
       if (some) {
         // a lane's only offer is its maximum; several are read again (a register cannot be chosen by a lane)
@@ -517,9 +545,7 @@ __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
     }
   }
   if (TOP && n) flush(n);
-  st.s -= lost_s;
-  st.t -= lost_t;
-  st = wave_join(st);
+  Stat st{top, one, group_sum<64>(sum - lost), group_sum<64>(sum_t - lost_t)};
   if (lane == 0) stats[wave] = st;
   if constexpr (TOP) lists[wave][lane] = list;
   __syncthreads();
@@ -533,13 +559,11 @@ __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
     }
   }
   if (wave) return;
-  st = stats[0];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) st = stat_join(st, stats[w]);
+  if constexpr (NW > 1) st = join<NW>(stats[lane & (NW - 1)]);
   if (a.segs > 1) {
     ScorePart* part = static_cast<ScorePart*>(a.part);
     const int64_t slot = row * a.segs + seg;
-    if (lane == 0) part[slot] = ScorePart{st.m, st.s, st.t, 0.f};
+    if (lane == 0) part[slot] = ScorePart{st.m, st.one, st.s, st.t};
     if constexpr (TOP) reinterpret_cast<Key*>(part + a.rows * a.segs)[slot * 64 + lane] = list;
     return;
   }
@@ -569,9 +593,9 @@ __global__ __launch_bounds__(256) void logprob_join(ScoreArgs a) {
     if (wave == 0) list = merge_lists(list, lists[1][63 - lane], lane);
   }
   if (wave) return;
-  Stat st{kLowest, 0.f, 0.f};
-  for (int s = lane; s < a.segs; s += 64) st = stat_join(st, Stat{part[s].m, part[s].s, part[s].t});
-  st = wave_join(st);
+  Stat st{kLowest, 0.f, 0.f, 0.f};
+  if (lane < a.segs) st = Stat{part[lane].m, part[lane].one, part[lane].s, part[lane].t};      // up to 64
+  st = join<64>(st);
   const RowOut o = row_out(st);
   if (lane == 0) write_row<T>(a, row, o);
   if (TOP && lane < a.top_k) {

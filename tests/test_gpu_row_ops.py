@@ -755,3 +755,44 @@ def test_long_rows_of_like_terms(cuda, rows, v, dtype):
   rel_s = U * (48 + 4 + 4 * a)
   close(got.lse, ref["lse"][which], rel_s + 2 * U * logs + U * (m + lse))
   close(got.entropy, ref["entropy"][which], rel_s + 2 * U * logs + rel_s * a + U * (4 * b + (8 + 48) * a + h))
+
+
+@pytest.mark.parametrize("rows,v", [(5, 32), (5, 33), (9, 200), (5, 513), (5, 1031), (5, 2048), (5, 2049), (1, 4099), (3, 30001), (40, 40001), (1, 131072),
+                                    (2100, 2500)])
+@pytest.mark.parametrize("lead", [2.0, 6.0, 11.0, 20.0, 30.0])
+@pytest.mark.parametrize("top_k", [0, 2, 20])
+def test_decided_rows_of_any_length(cuda, rows, v, lead, top_k):
+  """What stands beside a decided row's maximum keeps its bits for every length of a row and every place of the maximum.  z is 3
+  roundings relative to the exponent, the sums 64, the logarithm and what follows 40.  Rows with an excluded class behind
+  their last agree as well: the classes of a row do not choose its precision."""
+  x = -rnd(v, rows, v).abs().float()
+  at = (torch.arange(rows) * 7919 + 1) % v
+  at[0], at[-1] = v - 1, 0 if rows > 2 else v // 2
+  x[torch.arange(rows), at] = lead
+  labels = at.to(torch.int32)
+  z = x.double() - lead
+  z[torch.arange(rows), at] = -math.inf
+  rest = torch.exp(z).sum(1)
+  logp = -torch.log1p(rest)
+  rel = U * (3 * (lead + 5) + 40 + 64)
+  entropy = -logp + (torch.exp(z) * torch.where(z > -math.inf, -z, torch.zeros_like(z))).sum(1) / (1 + rest)
+  wide = torch.full((rows, v + 1), 1e30)
+  wide[:, :v] = x
+  for got in (ops.label_logprobs(x.to(cuda), labels.to(cuda), top_k=top_k),
+              ops.label_logprobs(wide.to(cuda), labels.to(cuda), top_k=top_k, allowed=(torch.arange(v + 1) < v).to(cuda))):
+    close(got.logprob, logp, rel * logp.abs())
+    close(got.entropy, entropy, 2 * rel * entropy)
+    if top_k:
+      assert torch.equal(got.top_ids[:, 0].cpu(), labels)
+      close(got.top_logprobs[:, 0], logp, rel * logp.abs())
+
+
+@pytest.mark.parametrize("v", [20, 300, 5000])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_several_maxima(cuda, v, dtype):
+  """Two and more equal maxima, next to each other, in different lanes, and at the two ends of a row."""
+  x = torch.full((6, v), -12.0, dtype=torch.float64)
+  for r, at in enumerate(([0, 1], [0, v - 1], [v // 2, v // 2 + 1, v - 1], [v - 2, v - 1], [3], list(range(0, v, 4)))):
+    x[r, at] = 5.0
+  labels = torch.tensor([1, 0, v - 1, 4, 3, 0], dtype=torch.int32)
+  check_score(ops.label_logprobs(x.to(dtype).to(cuda), labels.to(cuda), top_k=3), score64(x, labels, 3, None), v, 3)
