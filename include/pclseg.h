@@ -401,6 +401,15 @@ int pclseg_op_label_logprobs_grad(const void* logits, int dtype, int64_t rows, i
                                   const float* lse, const float* entropy, const float* d_logprob, const float* d_entropy,
                                   const int32_t* top_ids, const float* d_top, int top_k, void* grad, int64_t grad_stride,
                                   void* hip_stream);
+/* The same, with the log probabilities that op_label_logprobs wrote (logprob with labels, top_logprobs with top_ids and top_k;
+ * each may be NULL).  logit - lse is known to the rounding of lse, 2^-24 |lse|; a class that has nearly everything has a 1 - p
+ * of that size, and its gradient is right to 2^-24 only from its log probability.  The classes named by them need no gradient
+ * of their own: with d_entropy alone, labels and logprob (or one alternative) give the decided class its bits. */
+int pclseg_op_label_logprobs_grad_ex(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t stride,
+                                     const void* labels, int label_bytes, const uint8_t* allowed, int64_t allowed_stride,
+                                     const float* lse, const float* entropy, const float* logprob, const int32_t* top_ids,
+                                     const float* top_logprobs, const float* d_logprob, const float* d_entropy,
+                                     const float* d_top, int top_k, void* grad, int64_t grad_stride, void* hip_stream);
 
 #ifdef __cplusplus
 }

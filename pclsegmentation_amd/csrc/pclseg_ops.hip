@@ -232,6 +232,57 @@ int check_rows(const char* op, const void* logits, int dtype, int64_t rows, int6
   return PCLSEG_OK;
 }
 
+int score_grad(const char* op, const void* logits, int dtype, int64_t rows, int64_t classes, int64_t stride, const void* labels,
+               int label_bytes, const uint8_t* allowed, int64_t allowed_stride, const float* lse, const float* entropy,
+               const float* logprob, const int32_t* top_ids, const float* top_logprobs, const float* d_logprob,
+               const float* d_entropy, const float* d_top, int top_k, void* grad, int64_t grad_stride, void* hip_stream) {
+  const int rc = check_rows(op, logits, dtype, rows, classes, stride, labels, label_bytes, allowed, allowed_stride, top_k);
+  if (rc) return rc;
+  if (!d_logprob && !d_entropy && !d_top) return bad(op, "no gradient arrives");
+  if (d_logprob && !labels) return bad(op, "d_logprob needs labels");
+  if (d_entropy && !entropy) return bad(op, "d_entropy needs entropy");
+  if (d_top && (!top_ids || top_k < 1)) return bad(op, "d_top needs top_ids and top_k");
+  if (logprob && !labels) return bad(op, "logprob needs labels");
+  if (top_logprobs && (!top_ids || top_k < 1)) return bad(op, "top_logprobs needs top_ids and top_k");
+  if (grad_stride < classes) return bad_shape(op, "gradient stride smaller than classes");
+  if (rows == 0) return PCLSEG_OK;
+  if (!lse || !grad) return bad(op, "NULL buffer");
+  if (!aligned(grad, dtype_size(dtype))) return bad(op, "misaligned grad");
+  const int64_t sz = (int64_t)dtype_size(dtype);
+  if (overlap({logits, stride, classes, sz}, {grad, grad_stride, classes, sz}, rows)) return bad(op, "grad overlaps the logits");
+  GradArgs a{logits, rows, stride, (int)classes, d_logprob || logprob ? labels : nullptr, label_bytes == 8, allowed, allowed_stride,
+             lse, entropy, d_logprob, d_entropy, top_ids, d_top, d_top || top_logprobs ? top_k : 0, logprob, top_logprobs, grad,
+             grad_stride, 1, 1, 1, 0};
+  // a block takes 256 NI 16-byte pieces: that many of a long row, or whole short rows.  NI grows while the blocks are more
+  // than the 2048 that run at once
+  const int64_t vec = 16 / sz, nvec = (classes + vec - 1) / vec;
+  const int64_t all = std::min<int64_t>(rows, kMaxBlocks) * nvec;
+  const int ni = all <= 2048 * 256 ? 1 : all <= 2 * 2048 * 256 ? 2 : 4;
+  if (nvec > 256 * ni) {
+    a.vecs = 256 * ni;
+    a.cuts = (int)((nvec + 1 + a.vecs - 1) / a.vecs);      // one piece more: a row may begin inside its first
+  } else {
+    a.vecs = (int)nvec;
+    a.rows_per_block = (int)std::min<int64_t>(std::min<int64_t>(256, 256 * ni / nvec), kGradNames / (a.top_k + 1));
+  }
+  a.magic = (uint32_t)(((1u << 20) + a.vecs - 1) / a.vecs);
+  const int64_t blocks = a.cuts > 1 ? rows * a.cuts : (rows + a.rows_per_block - 1) / a.rows_per_block;
+  Launch go{op, (hipStream_t)hip_stream};
+  with_type(dtype, [&](auto t) {
+    typedef decltype(t) T;
+    if (allowed) {
+      if (ni == 1) go(logprob_grad<T, true, 1>, blocks, 256, a);
+      else if (ni == 2) go(logprob_grad<T, true, 2>, blocks, 256, a);
+      else go(logprob_grad<T, true, 4>, blocks, 256, a);
+    } else {
+      if (ni == 1) go(logprob_grad<T, false, 1>, blocks, 256, a);
+      else if (ni == 2) go(logprob_grad<T, false, 2>, blocks, 256, a);
+      else go(logprob_grad<T, false, 4>, blocks, 256, a);
+    }
+  });
+  return go.rc;
+}
+
 }  // namespace
 
 extern "C" {
@@ -357,49 +408,22 @@ int pclseg_op_label_logprobs_grad(const void* logits, int dtype, int64_t rows, i
                                   const float* lse, const float* entropy, const float* d_logprob, const float* d_entropy,
                                   const int32_t* top_ids, const float* d_top, int top_k, void* grad, int64_t grad_stride,
                                   void* hip_stream) try {
-  const char* op = "op_label_logprobs_grad";
-  const int rc = check_rows(op, logits, dtype, rows, classes, stride, labels, label_bytes, allowed, allowed_stride, top_k);
-  if (rc) return rc;
-  if (!d_logprob && !d_entropy && !d_top) return bad(op, "no gradient arrives");
-  if (d_logprob && !labels) return bad(op, "d_logprob needs labels");
-  if (d_entropy && !entropy) return bad(op, "d_entropy needs entropy");
-  if (d_top && (!top_ids || top_k < 1)) return bad(op, "d_top needs top_ids and top_k");
-  if (grad_stride < classes) return bad_shape(op, "gradient stride smaller than classes");
-  if (rows == 0) return PCLSEG_OK;
-  if (!lse || !grad) return bad(op, "NULL buffer");
-  if (!aligned(grad, dtype_size(dtype))) return bad(op, "misaligned grad");
-  const int64_t sz = (int64_t)dtype_size(dtype);
-  if (overlap({logits, stride, classes, sz}, {grad, grad_stride, classes, sz}, rows)) return bad(op, "grad overlaps the logits");
-  GradArgs a{logits, rows, stride, (int)classes, labels, label_bytes == 8, allowed, allowed_stride, lse, entropy,
-             d_logprob, d_entropy, top_ids, d_top, d_top ? top_k : 0, grad, grad_stride, 1, 1, 1, 0};
-  // a block takes 256 NI 16-byte pieces: that many of a long row, or whole short rows.  NI grows while the blocks are more
-  // than the 2048 that run at once
-  const int64_t vec = 16 / sz, nvec = (classes + vec - 1) / vec;
-  const int64_t all = std::min<int64_t>(rows, kMaxBlocks) * nvec;
-  const int ni = all <= 2048 * 256 ? 1 : all <= 2 * 2048 * 256 ? 2 : 4;
-  if (nvec > 256 * ni) {
-    a.vecs = 256 * ni;
-    a.cuts = (int)((nvec + 1 + a.vecs - 1) / a.vecs);      // one piece more: a row may begin inside its first
-  } else {
-    a.vecs = (int)nvec;
-    a.rows_per_block = (int)std::min<int64_t>(std::min<int64_t>(256, 256 * ni / nvec), kGradNames / (a.top_k + 1));
-  }
-  a.magic = (uint32_t)(((1u << 20) + a.vecs - 1) / a.vecs);
-  const int64_t blocks = a.cuts > 1 ? rows * a.cuts : (rows + a.rows_per_block - 1) / a.rows_per_block;
-  Launch go{op, (hipStream_t)hip_stream};
-  with_type(dtype, [&](auto t) {
-    typedef decltype(t) T;
-    if (allowed) {
-      if (ni == 1) go(logprob_grad<T, true, 1>, blocks, 256, a);
-      else if (ni == 2) go(logprob_grad<T, true, 2>, blocks, 256, a);
-      else go(logprob_grad<T, true, 4>, blocks, 256, a);
-    } else {
-      if (ni == 1) go(logprob_grad<T, false, 1>, blocks, 256, a);
-      else if (ni == 2) go(logprob_grad<T, false, 2>, blocks, 256, a);
-      else go(logprob_grad<T, false, 4>, blocks, 256, a);
-    }
-  });
-  return go.rc;
+  return score_grad("op_label_logprobs_grad", logits, dtype, rows, classes, stride, labels, label_bytes, allowed, allowed_stride, lse,
+                    entropy, nullptr, top_ids, nullptr, d_logprob, d_entropy, d_top, top_k, grad, grad_stride, hip_stream);
+} OP_CATCH
+
+}  // extern "C"
+
+// ---- the same with what the forward pass knew of the names
+extern "C" {
+
+int pclseg_op_label_logprobs_grad_ex(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t stride,
+                                     const void* labels, int label_bytes, const uint8_t* allowed, int64_t allowed_stride,
+                                     const float* lse, const float* entropy, const float* logprob, const int32_t* top_ids,
+                                     const float* top_logprobs, const float* d_logprob, const float* d_entropy,
+                                     const float* d_top, int top_k, void* grad, int64_t grad_stride, void* hip_stream) try {
+  return score_grad("op_label_logprobs_grad_ex", logits, dtype, rows, classes, stride, labels, label_bytes, allowed, allowed_stride,
+                    lse, entropy, logprob, top_ids, top_logprobs, d_logprob, d_entropy, d_top, top_k, grad, grad_stride, hip_stream);
 } OP_CATCH
 
 }  // extern "C"

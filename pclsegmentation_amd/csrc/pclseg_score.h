@@ -608,7 +608,9 @@ __global__ __launch_bounds__(256) void logprob_join(ScoreArgs a) {
 // With p_j = e^(x_j - lse) (0 where not allowed), H the row's entropy, gl / ge / gt the gradients that arrive:
 //   d loss / d x_j = G_j (1 - p_j) - p_j (W - G_j) - ge p_j (x_j - lse + H),
 //   G_j = gl [j = label] + sum_i gt_i [j = id_i],  W = gl + sum_i gt_i
-// 1 - p of a named class is taken from x - lse without the difference: a decided row's label keeps its significant bits.
+// 1 - p of a named class is taken from z = ln p without the difference.  z = x - lse is known to the rounding of lse, 2^-24 |lse|,
+// which is all of 1 - p for a class that has nearly everything; a name that brings the log probability of the forward pass
+// (relative to 2^-24) has that as its z and keeps its bits.
 // One read of the logits and one write of the gradient.  A block owns whole rows, or a piece of one; the classes that its
 // rows' labels and alternatives name, and what arrives for them, are put into LDS first, and every 16-byte piece is compared
 // with its row's names while it is in registers: no element is written twice, equal names add up.
@@ -620,10 +622,11 @@ struct GradArgs {
   int label64;
   const uint8_t* allowed;
   int64_t allowed_stride;
-  const float *lse, *entropy, *d_logprob, *d_entropy;   // entropy / d_entropy / d_logprob may be NULL
+  const float *lse, *entropy, *d_logprob, *d_entropy;   // all but lse may be NULL; labels NULL: the label is no name
   const int32_t* top_ids;
   const float* d_top;
-  int top_k;
+  int top_k;                                            // 0: the alternatives are no names
+  const float *logprob, *top_logprobs;                  // ln p of the names, or NULL
   void* grad;
   int64_t grad_stride;
   // a block: 16-byte pieces of rows_per_block rows (vecs each), or vecs pieces of one row that takes `cuts` blocks
@@ -644,8 +647,8 @@ __device__ __forceinline__ float one_minus_exp(float z) {
   s = fmaf(s, z, 1.f);
   return z > -0.35f ? -z * s : 1.f - fast_exp(z);
 }
-__device__ __forceinline__ float grad_dense(const GradRow& r, float w, float x) {
-  const float z = x - r.lse, p = fast_exp(z);
+__device__ __forceinline__ float grad_dense(const GradRow& r, float w, float z) {
+  const float p = fast_exp(z);
   // an underflowed p takes the entropy term with it (0 * -inf otherwise)
   return -p * fmaf(r.ge, fmaxf(z, -200.f) + r.h, w);
 }
@@ -659,13 +662,15 @@ __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
   __shared__ GradRow prm[256];
   __shared__ int ids[kGradNames];
   __shared__ float gs[kGradNames];
+  __shared__ float zs[kGradNames];      // ln p of a name, 1: not given
   const int64_t row0 = a.cuts > 1 ? (int64_t)(blockIdx.x / (unsigned)a.cuts) : (int64_t)blockIdx.x * a.rows_per_block;
   // the pieces of a long row begin at multiples of 16 bytes of the gradient, up to VEC - 1 elements before its first
   const int pad = a.cuts > 1 ? (int)((reinterpret_cast<uintptr_t>(static_cast<T*>(a.grad) + row0 * a.grad_stride) & 15) / sizeof(T)) : 0;
   const int c0 = a.cuts > 1 ? (int)(blockIdx.x % (unsigned)a.cuts) * a.vecs * VEC - pad : 0;
   const int c1 = a.cuts > 1 && a.classes - c0 > a.vecs * VEC ? c0 + a.vecs * VEC : a.classes;
   const int nr = a.cuts > 1 ? 1 : (int)(a.rows - row0 < a.rows_per_block ? a.rows - row0 : a.rows_per_block);
-  const int names = a.top_k + (a.d_logprob ? 1 : 0);
+  const int names = a.top_k + (a.labels ? 1 : 0);
+  const bool kept = a.logprob || a.top_logprobs;
   int rr[NI], cc[NI];
   Piece<T, MASK> raw[NI];
 #pragma unroll
@@ -681,17 +686,21 @@ __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
     const int r = i / names, n = i - r * names;
     const int64_t row = row0 + r;
     int64_t id;
-    float g;
+    float g = 0.f, z = 1.f;
     if (n < a.top_k) {
-      id = a.top_ids[row * a.top_k + n];
-      g = a.d_top[row * a.top_k + n];
+      const int64_t at = row * a.top_k + n;
+      id = a.top_ids[at];
+      if (a.d_top) g = a.d_top[at];
+      if (a.top_logprobs) z = a.top_logprobs[at];
     } else {
       id = a.label64 ? static_cast<const int64_t*>(a.labels)[row] : static_cast<const int32_t*>(a.labels)[row];
-      g = a.d_logprob[row];
+      if (a.d_logprob) g = a.d_logprob[row];
+      if (a.logprob) z = a.logprob[row];
     }
     const bool known = id >= 0 && id < a.classes;
     ids[i] = known ? (int)id : -1;
     gs[i] = known ? g : 0.f;
+    if (kept) zs[i] = z;
   }
   GradRow mine{0.f, 0.f, 0.f, 0.f};
   if ((int)threadIdx.x < nr) {
@@ -724,8 +733,12 @@ __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
     if (inside) raw[n].expand(x);
     else load_tail<T, MASK>(static_cast<const T*>(a.x) + (row0 + r) * a.stride,
                             MASK ? a.allowed + (row0 + r) * a.allowed_stride : nullptr, c, c1, x);
+    float z[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = 0.f;      // G_j first
+    for (int e = 0; e < VEC; ++e) {
+      f[e] = 0.f;      // G_j first
+      z[e] = x[e] - p.lse;
+    }
     bool named = false;
     for (int k = r * names; k < (r + 1) * names; ++k) {
       const int d = ids[k] - c;
@@ -734,15 +747,19 @@ __global__ __launch_bounds__(256) void logprob_grad(GradArgs a) {
         const float g = gs[k];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) f[e] += e == d ? g : 0.f;
+        if (kept) {
+          const float zk = zs[k];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) z[e] = e == d && zk <= 0.f ? zk : z[e];
+        }
       }
     }
     if (named) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        f[e] = fmaf(f[e], one_minus_exp(x[e] - p.lse), grad_dense(p, p.w - f[e], x[e]));
+      for (int e = 0; e < VEC; ++e) f[e] = fmaf(f[e], one_minus_exp(z[e]), grad_dense(p, p.w - f[e], z[e]));
     } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) f[e] = grad_dense(p, p.w, x[e]);
+      for (int e = 0; e < VEC; ++e) f[e] = grad_dense(p, p.w, z[e]);
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) f[e] = x[e] == neg_inf() ? 0.f : f[e];

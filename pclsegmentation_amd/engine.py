@@ -43,6 +43,7 @@ EXPORTS = [
   "pclseg_op_confusion_matrix", "pclseg_op_project", "pclseg_op_project_ex", "pclseg_op_split_f16_roundtrip",
   "pclseg_i8_row_bytes", "pclseg_op_quantize_rows", "pclseg_op_matmul_i8", "pclseg_op_linear_i8_workspace",
   "pclseg_op_linear_i8", "pclseg_op_label_logprobs_workspace", "pclseg_op_label_logprobs", "pclseg_op_label_logprobs_grad",
+  "pclseg_op_label_logprobs_grad_ex",
 ]
 
 
@@ -149,6 +150,8 @@ def load_library():
   lib.pclseg_op_label_logprobs.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp, i64, i32, vp, vp, vp, vp, vp, vp, sz, vp]
   lib.pclseg_op_label_logprobs_grad.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp, i64, vp, vp, vp, vp, vp, vp, i32, vp,
                                                 i64, vp]
+  lib.pclseg_op_label_logprobs_grad_ex.argtypes = [vp, i32, i64, i64, i64, vp, i32, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, i32,
+                                                   vp, i64, vp]
   for name in EXPORTS:
     fn = getattr(lib, name)
     if name not in ("pclseg_last_error", "pclseg_host_alloc", "pclseg_build_sha", "pclseg_i8_row_bytes"):

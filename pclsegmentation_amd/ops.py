@@ -273,40 +273,51 @@ def label_logprobs(logits, labels=None, top_k=0, allowed=None):
 
 
 def label_logprobs_grad(logits, labels, lse, d_logprob=None, entropy=None, d_entropy=None, top_ids=None, d_top=None,
-                        allowed=None):
+                        allowed=None, logprob=None, top_logprobs=None):
   """Gradient with respect to the logits (their shape and dtype) of a loss whose gradients with respect to label_logprobs'
   logprob, entropy and top_logprobs are d_logprob, d_entropy and d_top (float32; each may be None, one is given).  lse, entropy
   and top_ids are what label_logprobs returned for the same logits and mask; entropy is needed for d_entropy, top_ids for
-  d_top.  Excluded classes, rows without an allowed class and labels that are not counted get 0."""
+  d_top.  Excluded classes, rows without an allowed class and labels that are not counted get 0.
+
+  logprob (with labels) and top_logprobs (with top_ids) are what label_logprobs returned too.  Without them ln p is logit - lse,
+  right to the rounding of lse; with them the gradient of a label or alternative that has nearly all of a row's probability
+  is right to its own last bits (with d_entropy alone as well, where they name the decided class)."""
   dt, r, stride = _logits(logits)
   dev, (m, v) = logits.device, r.shape
   if d_logprob is None and d_entropy is None and d_top is None:
     _fail("one of d_logprob, d_entropy and d_top must be given")
   lse = _vector(lse, dev, m, "lse")
-  if d_logprob is not None:
+  if d_logprob is not None or logprob is not None:
     if labels is None:
-      _fail("d_logprob needs labels")
-    labels, d_logprob = _labels(labels, dev, m), _vector(d_logprob, dev, m, "d_logprob")
+      _fail("d_logprob and logprob need labels")
+    labels = _labels(labels, dev, m)
+    d_logprob = None if d_logprob is None else _vector(d_logprob, dev, m, "d_logprob")
+    logprob = None if logprob is None else _vector(logprob, dev, m, "logprob")
+  else:
+    labels = None
   if d_entropy is not None:
     if entropy is None:
       _fail("d_entropy needs entropy")
     entropy, d_entropy = _vector(entropy, dev, m, "entropy"), _vector(d_entropy, dev, m, "d_entropy")
   top_k = 0
-  if d_top is not None:
+  if d_top is not None or top_logprobs is not None:
     if top_ids is None:
-      _fail("d_top needs top_ids")
+      _fail("d_top and top_logprobs need top_ids")
     _on(top_ids, dev, "top_ids")
     top_k = top_ids.shape[-1] if top_ids.dim() else 0
     if top_ids.dtype != torch.int32 or top_ids.numel() != m * top_k:
       _fail("top_ids must be int32 [..., top_k], got %s of shape %s" % (top_ids.dtype, tuple(top_ids.shape)))
-    top_ids, d_top = top_ids.contiguous(), _vector(d_top, dev, m * top_k, "d_top")
+    top_ids = top_ids.contiguous()
+    d_top = None if d_top is None else _vector(d_top, dev, m * top_k, "d_top")
+    top_logprobs = None if top_logprobs is None else _vector(top_logprobs, dev, m * top_k, "top_logprobs")
   mstride = 0
   if allowed is not None:
     allowed, mstride = _mask(allowed, logits)
   grad = torch.empty_like(logits) if logits.is_contiguous() else logits.new_empty(logits.shape)
   if m:
-    _call(dev, _engine.load_library().pclseg_op_label_logprobs_grad, r.data_ptr(), dt, m, v, stride,
-          _ptr(labels) if d_logprob is not None else None, labels.element_size() if d_logprob is not None else 0,
-          _ptr(allowed), mstride, lse.data_ptr(), _ptr(entropy) if d_entropy is not None else None, _ptr(d_logprob),
-          _ptr(d_entropy), _ptr(top_ids) if top_k else None, _ptr(d_top) if top_k else None, top_k, grad.data_ptr(), v)
+    _call(dev, _engine.load_library().pclseg_op_label_logprobs_grad_ex, r.data_ptr(), dt, m, v, stride, _ptr(labels),
+          0 if labels is None else labels.element_size(), _ptr(allowed), mstride, lse.data_ptr(),
+          _ptr(entropy) if d_entropy is not None else None, _ptr(logprob), _ptr(top_ids) if top_k else None,
+          _ptr(top_logprobs) if top_k else None, _ptr(d_logprob), _ptr(d_entropy), _ptr(d_top) if top_k else None, top_k,
+          grad.data_ptr(), v)
   return grad

@@ -796,3 +796,107 @@ def test_several_maxima(cuda, v, dtype):
     x[r, at] = 5.0
   labels = torch.tensor([1, 0, v - 1, 4, 3, 0], dtype=torch.int32)
   check_score(ops.label_logprobs(x.to(dtype).to(cuda), labels.to(cuda), top_k=3), score64(x, labels, 3, None), v, 3)
+
+
+@pytest.mark.parametrize("rows,v", [(5, 2), (300, 20), (5, 33), (5, 1031), (3, 9001), (1, 131072)])
+@pytest.mark.parametrize("lead", [2.0, 6.0, 11.3, 20.3, 30.0])
+@pytest.mark.parametrize("masked", [False, True])
+def test_gradient_of_decided_rows(cuda, rows, v, lead, masked):
+  """Against the float64 gradient of the logits, not of the rounded lse: with the forward pass's log probabilities the gradient of
+  a class that has nearly everything is right to its own bits, whether it is the label, an alternative, or only has
+  an entropy to answer for.  rel bounds ln p as in test_decided_rows_of_any_length; the other classes' p = e^(x - lse) is right to the
+  rounding of lse and of three products with the exponent."""
+  x = -rnd(v + 1, rows, v).abs().float()
+  at = (torch.arange(rows) * 7919 + 1) % v
+  x[torch.arange(rows), at] = lead
+  r = torch.arange(rows)
+  allowed = torch.ones(rows, v, dtype=torch.bool)
+  if masked:
+    allowed[:, 0] = False
+    at[at == 0] = v - 1
+    x[r, at] = lead
+    x[:, 0] = math.nan
+  z = torch.where(allowed, x.double() - lead, -math.inf)
+  z[r, at] = -math.inf
+  rest = torch.exp(z).sum(1)
+  logp = torch.where(allowed, torch.where(z > -math.inf, z, 0.0) - torch.log1p(rest)[:, None], -math.inf)
+  p = torch.exp(logp)
+  lp0 = torch.where(allowed, logp, 0.0)
+  h = -(p * lp0).sum(1, keepdim=True)
+  q = -torch.expm1(lp0[r, at])
+  rel = U * (3 * (lead + 5) + 40 + 64)
+  dev = lambda t: None if t is None else t.to(cuda)
+  labels = at.to(torch.int32)
+  other = torch.where(at == v - 1, v - 2, v - 1).to(torch.int32)          # a label beside the decided class
+  got = ops.label_logprobs(dev(x), dev(labels), top_k=1, allowed=dev(allowed))
+  beside = ops.label_logprobs(dev(x), dev(other), top_k=1, allowed=dev(allowed))
+  g, ge = torch.full((rows,), -0.75), torch.full((rows,), 0.25)
+  kept = dict(lse=got.lse, allowed=dev(allowed))
+  # the rounding of p = e^(x - lse), relative, and what the label's p and z may be off
+  rp = U * (got.lse.cpu().double().abs().nan_to_num(0, 0, 0)[:, None] + 5 * lp0.abs() + 12)
+  named = torch.zeros_like(p)
+  named[r, at] = 1.0
+  own = q[:, None] * named
+
+  def check(grad, want, bound):
+    off = ~allowed
+    close(grad, torch.where(off, 0.0, want), torch.where(off, 0.0, bound) + 2.0 ** -140)
+
+  # the label, the alternative, and both (they add up)
+  want = g.double()[:, None] * torch.where(named > 0, own, -p)
+  bound = 0.75 * torch.where(named > 0, (rel + 24 * U) * own, p * rp)
+  a = ops.label_logprobs_grad(dev(x), dev(labels), d_logprob=dev(g), logprob=got.logprob, **kept)
+  check(a, want, bound)
+  b = ops.label_logprobs_grad(dev(x), None, d_top=dev(g[:, None]), top_ids=got.top_ids, top_logprobs=got.top_logprobs, **kept)
+  check(b, want, bound)
+  both = ops.label_logprobs_grad(dev(x), dev(labels), d_logprob=dev(g), logprob=got.logprob, d_top=dev(g[:, None]),
+                                 top_ids=got.top_ids, top_logprobs=got.top_logprobs, **kept)
+  check(both, 2 * want, 2 * bound)
+  # a row's gradient sums to 0: to the other classes' roundings
+  total = a.cpu().double().sum(1)
+  assert (total.abs() <= bound.sum(1) + 2.0 ** -140).all()
+  # the entropy alone, the decided class named by the label or by the alternative
+  eg = -0.25 * p * (lp0 + h)
+  eb = 0.25 * p * ((lp0.abs() + h) * torch.where(named > 0, 3 * rel + 12 * U, rp + 3 * rel))
+  for names in (dict(labels=dev(labels), logprob=got.logprob), dict(labels=None, top_ids=got.top_ids, top_logprobs=got.top_logprobs)):
+    check(ops.label_logprobs_grad(dev(x), names.pop("labels"), entropy=got.entropy, d_entropy=dev(ge), **names, **kept), eg, eb)
+  # a label beside the decided class: the decided class's own gradient is -p g, the label's g (1 - p)
+  if v > 2 + masked:
+    named = torch.zeros_like(p)
+    named[r, other.long()] = 1.0
+    want = -0.75 * torch.where(named > 0, 1 - p, -p)
+    check(ops.label_logprobs_grad(dev(x), dev(other), d_logprob=dev(g), logprob=beside.logprob, **kept), want,
+          0.75 * (p * rp + 24 * U * named))
+
+
+@pytest.mark.parametrize("rows,v,top_k", [(300, 20, 3), (9, 33, 40), (5, 4099, 20), (1, 131072, 64), (9000, 129, 1)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradient_with_log_probabilities(cuda, rows, v, top_k, dtype):
+  """The log probabilities of the forward pass change a gradient by roundings only; labels that are not counted, excluded labels and
+  rows with nothing, or with a NaN, as without them."""
+  x = (rnd(v, rows, v) * 2).to(dtype)
+  allowed = torch.rand((rows, v), generator=torch.Generator().manual_seed(v)) < 0.8
+  if rows > 4:
+    allowed[0] = False
+    allowed[3] = True
+    x[3, v // 2] = math.nan
+  labels = labels_for(rows, v, 9)
+  ref = score64(x, labels, top_k, allowed)
+  dev = lambda t: t.to(cuda)
+  fwd = ops.label_logprobs(dev(x), dev(labels), top_k=top_k, allowed=dev(allowed))
+  d_lp, d_h, d_top = rnd(1, rows).float(), rnd(2, rows).float(), rnd(3, rows, top_k).float()
+  got = ops.label_logprobs_grad(dev(x), dev(labels), fwd.lse, d_logprob=dev(d_lp), entropy=fwd.entropy, d_entropy=dev(d_h),
+                                top_ids=fwd.top_ids, d_top=dev(d_top), allowed=dev(allowed), logprob=fwd.logprob,
+                                top_logprobs=fwd.top_logprobs)
+  want, bound = grad64(ref, labels, fwd.lse.cpu().double(), fwd.entropy.cpu().double(), d_lp.double(), d_h.double(), fwd.top_ids.cpu(),
+                       d_top.double(), dtype)
+  # a name's ln p is x - lse to the roundings of both: 4 u (|lse| + |ln p| + 16) times what its p and 1 - p weigh
+  lse = fwd.lse.cpu().double().abs().nan_to_num(0, 0, 0)[:, None]
+  weight = d_lp.abs()[:, None] + d_top.abs().sum(1, keepdim=True) + d_h.abs()[:, None] * (ref["entropy"].nan_to_num()[:, None] + 2)
+  extra = 4 * U * (lse + 20) * weight.double()
+  if rows > 4:
+    assert torch.isnan(got[3][allowed[3]]).all() and not got[0].any()
+    keep = torch.arange(rows) != 3
+    close(got[keep.to(cuda)], want[keep], (bound + extra)[keep])
+  else:
+    close(got, want, bound + extra)

@@ -290,3 +290,38 @@ def test_label_logprobs_grad_far_strides():
   first row, inside their range."""
   _refused("pclseg_op_label_logprobs_grad", list({**GRAD, "stride": 1 << 60, "rows": 1 << 39, "grad": FAR, "grad_stride": 4}.values()),
            -1, "overlaps the logits")
+
+
+GRAD_EX = dict(logits=P, dtype=0, rows=2, classes=4, stride=4, labels=P, label_bytes=4, allowed=None, allowed_stride=0, lse=P,
+               entropy=P, logprob=P, top_ids=P, top_logprobs=P, d_logprob=P, d_entropy=P, d_top=P, top_k=2, grad=P + 1024, grad_stride=4,
+               stream=None)
+
+
+@pytest.mark.parametrize("change,code,word", [
+  (dict(dtype=9), -1, "dtype"), (dict(stride=3), -2, "stride"), (dict(grad_stride=3), -2, "gradient stride"),
+  (dict(d_logprob=None, d_entropy=None, d_top=None), -1, "no gradient"), (dict(labels=None), -1, "labels"),
+  (dict(labels=None, d_logprob=None), -1, "logprob needs labels"), (dict(entropy=None), -1, "entropy"), (dict(top_ids=None), -1, "top_ids"),
+  (dict(top_ids=None, d_top=None), -1, "top_logprobs needs"), (dict(top_k=0, d_top=None), -1, "top_logprobs needs"), (dict(lse=None), -1, "NULL"),
+  (dict(grad=P), -1, "overlaps"), (dict(grad=P + 1025), -1, "misaligned"), (dict(rows=1 << 40, grad=FAR), -2, "blocks"),
+])
+def test_label_logprobs_grad_ex_refuses(change, code, word):
+  _refused("pclseg_op_label_logprobs_grad_ex", list({**GRAD_EX, **change}.values()), code, word)
+
+
+def test_entry_points_of_the_second_block_are_behind_the_exception_barrier():
+  src = open(os.path.join(os.path.dirname(E.__file__), "csrc", "pclseg_ops.hip")).read()
+  defs = re.findall(r"^int (pclseg_\w+)\([^;{]*\)( try)? \{$", src, re.M)
+  assert len(defs) == 8 and all(t for _, t in defs) and src.count("} OP_CATCH\n") == 8
+
+
+def test_python_layer_refuses_log_probabilities_without_names(host_as_device):
+  x, i, v = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int32), torch.zeros(2)
+  two, ids = torch.zeros(2, 2), torch.zeros((2, 2), dtype=torch.int32)
+  for call in (lambda: ops.label_logprobs_grad(x, i, v, logprob=v),                       # no gradient arrives
+               lambda: ops.label_logprobs_grad(x, None, v, entropy=v, d_entropy=v, logprob=v),
+               lambda: ops.label_logprobs_grad(x, i, v, entropy=v, d_entropy=v, logprob=v[:1]),
+               lambda: ops.label_logprobs_grad(x, i, v, entropy=v, d_entropy=v, logprob=v.double()),
+               lambda: ops.label_logprobs_grad(x, i, v, entropy=v, d_entropy=v, top_logprobs=two),
+               lambda: ops.label_logprobs_grad(x, i, v, entropy=v, d_entropy=v, top_ids=ids, top_logprobs=two[:, :1])):
+    with pytest.raises(ValueError):
+      call()
