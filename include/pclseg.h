@@ -345,10 +345,11 @@ typedef enum pclseg_dtype { PCLSEG_F32 = 0, PCLSEG_BF16 = 1, PCLSEG_F16 = 2 } pc
 /* Bytes a row of k codes takes: k rounded up to 64, and to 128 above 64.  0 for k outside [1, PCLSEG_I8_K_MAX]. */
 int64_t pclseg_i8_row_bytes(int64_t k);
 
-/* Symmetric quantisation, one scale per row: scale = max|x| / 127 (float32), q = round(x / scale), ties to even.
+/* Symmetric quantisation, one scale per row: scale = max|x| / 127 (float32), q = round(x / scale), ties to even, within
+ * +-127 (beyond it only where a subnormal scale is rounded down).
  *   x      [rows, cols] dtype, row stride x_stride elements
  *   q      int8 [rows, pclseg_i8_row_bytes(cols)], 8-byte aligned, written whole: zeros behind cols; does not overlap x
- *   scale  float32 [rows]: 0 for a row of zeros, NaN (codes 0) for a row that holds an infinity or a NaN */
+ *   scale  float32 [rows]: 0 for a row of zeros (or below 64 * 2^-149; codes 0), NaN (codes 0) for a row that holds an infinity or a NaN */
 int pclseg_op_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_stride, int8_t* q,
                             float* scale, void* hip_stream);
 

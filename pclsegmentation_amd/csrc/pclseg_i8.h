@@ -1,7 +1,7 @@
 // pclseg_i8.h — the 8-bit linear layer: rows of activations quantised symmetrically with one scale per row, an int8 x int8
 // product on the matrix cores with exact int32 sums, one scale per output channel, and the epilogue of op_conv2d.
 //
-//   s[i] = max_k |x[i,k]| / 127,  q[i,k] = round(x[i,k] / s[i]) (ties to even)
+//   s[i] = max_k |x[i,k]| / 127,  q[i,k] = round(x[i,k] / s[i]) (ties to even, within +-127; 0 where s[i] is 0)
 //   y[i,j] = act( s[i] t[j] sum_k q[i,k] w[j,k] + bias[j] ) + residual[i,j]
 //
 // Codes lie in rows of `ld` bytes, a multiple of 64 (of 128 for k > 64) and zero behind k: every tile is read whole, without
@@ -63,6 +63,15 @@ __device__ __forceinline__ RowScale row_scale(float amax) {
   constexpr float c = 1.f / 127.f;
   const float a = amax * r.pre, q = a * c;
   r.s = fmaf(fmaf(-127.f, q, a), c, q);
+  if (r.pre != 1.f && r.s < 0x1p-62f) {
+    // the scale that is stored is s 2^-64, a subnormal number: the codes belong to what it is rounded to.  That takes two
+    // roundings, of which the exact remainder against 63.5 units says whether the second went the wrong way (a is a whole
+    // number of units, so there are no ties)
+    constexpr float unit = 0x1p-85f;
+    r.s = (r.s * 0x1p-64f) * 0x1p64f;
+    const float rest = fmaf(-127.f, r.s, a);
+    r.s += rest > 63.5f * unit ? unit : rest < -63.5f * unit ? -unit : 0.f;
+  }
   r.inv = r.s > 0.f ? __builtin_amdgcn_rcpf(r.s) : 0.f;      // one unit off: 2^-16 of a step in a code's quotient
   r.half = 0.5f * r.s;
   return r;
@@ -127,8 +136,9 @@ template <typename T> struct Eight {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = Elem<T>::get(v[e / Elem<T>::VEC], e % Elem<T>::VEC);
     if (r.pre != 1.f) {
+      const float most = 127.f * r.s;      // a rounded subnormal scale may be short of the row: 127 is the last code
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= r.pre;
+      for (int e = 0; e < 8; ++e) x[e] = fminf(fmaxf(x[e] * r.pre, -most), most);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) u[e] = quant(x[e], r, worst);

@@ -142,7 +142,7 @@ def _row_bytes(k):
 
 def quantize_rows(x):
   """Symmetric 8-bit codes of x [..., k]: scale = max|row| / 127, code = round(x / scale), ties to even.  A row of zeros has
-  the scale 0; a row with an infinity or a NaN has the scale NaN, and so are the products it takes part in."""
+  the scale 0 (and so does one whose scale is too small for a float32); a row with an infinity or a NaN has the scale NaN, and so are the products it takes part in."""
   _on(x, None, "x")
   dt = _dtype(x, "x")
   if x.dim() < 1:

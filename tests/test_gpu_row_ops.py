@@ -900,3 +900,26 @@ def test_gradient_with_log_probabilities(cuda, rows, v, top_k, dtype):
     close(got[keep.to(cuda)], want[keep], (bound + extra)[keep])
   else:
     close(got, want, bound + extra)
+
+
+@pytest.mark.parametrize("cols", [1, 40, 300, 3000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_quantize_rows_at_the_small_end(cuda, cols, dtype):
+  """Rows from 2^-149 to 2^-58: the scale is the float32 nearest to max / 127, a subnormal one too, and the codes belong to it."""
+  rows = 1500
+  g = torch.Generator().manual_seed(cols)
+  e = torch.rand(rows, 1, generator=g, dtype=torch.float64) * 91 - 149
+  x = (rnd(cols, rows, cols) * torch.exp2(e)).to(dtype)
+  steps = torch.arange(1, rows // 3 + 1, dtype=torch.float64)[:, None]        # maxima of 1, 2, 3, ... and 127.5, ... smallest steps
+  x[::3] = torch.round(steps * rnd(5, len(steps), cols).clamp(-1, 1)).to(dtype) * 2.0 ** -149 if dtype == F32 else x[::3]
+  if dtype == F32:
+    x[::3, 0] = (steps[:, 0] * 2.0 ** -149).to(dtype)
+  q, scale = quant64(x)
+  assert (scale == 0).sum() > (0 if dtype == BF16 else 20) and ((scale > 0) & (scale < 2.0 ** -126)).sum() > 100
+  got = ops.quantize_rows(x.to(cuda))
+  assert torch.equal(got.scale.cpu(), scale) and torch.equal(got.codes.cpu(), q)
+  w = ops.quantize_rows((rnd(2, 20, cols) * 2.0 ** 60).float().to(cuda))
+  for m in (8, 33):      # one launch and two, the same rows
+    y = ops.linear_i8(x[:m].to(cuda), w, out_dtype=F32)
+    assert torch.equal(y, ops.matmul_i8(ops.quantize_rows(x[:m].to(cuda)), w))
+    check_product(y, *product64(q[:m], scale[:m], w.codes.cpu(), w.scale.cpu(), None, "none", None), F32)
