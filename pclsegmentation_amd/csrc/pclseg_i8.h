@@ -241,9 +241,18 @@ __device__ __forceinline__ float activate(float v, int act) {
   return act == ACT_RELU ? relu(v) : act == ACT_LEAKY ? leaky(v) : act == ACT_SIGMOID ? sigmoid(v) : v;
 }
 
+// acc sa sb + bias.  Below 2^64 a row's scale takes the sum nowhere near the end of float32 (2^31 2^64); from there on the
+// channel's scale goes first, and what overflows then does so in the product of all three.  Whole multiples of a subnormal scale
+// are exact, so neither order loses bits below.
+constexpr float kFarScale = 0x1p64f;
+__device__ __forceinline__ float scaled(float acc, float sa, float sb, float bias) {
+  const bool far = sa >= kFarScale;
+  return fmaf(acc * (far ? sb : sa), far ? sa : sb, bias);
+}
+
 template <typename T>
 __device__ __forceinline__ void i8_store(const I8Args& p, int64_t i, int j, int acc, float sa, float sb, float bias) {
-  float v = activate((float)acc * sa * sb + bias, p.act);
+  float v = activate(scaled((float)acc, sa, sb, bias), p.act);
   if (p.residual) v += Elem<T>::load(static_cast<const T*>(p.residual) + i * p.ldr + j);
   static_cast<T*>(p.y)[i * p.ldy + j] = Elem<T>::from(v);
 }
@@ -611,11 +620,26 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void i8_tiles(I8Args p, unsigned
         }
 #pragma unroll
         for (int r = 0; r < HR; ++r) s[r] = (p.sa + row0 + r * RP)[qr];
+        float most = s[0];
+#pragma unroll
+        for (int r = 1; r < HR; ++r) most = fmaxf(most, s[r]);
+        const bool far = __ballot(most >= kFarScale) != 0;      // uniform: the selects cost nothing where no row needs them
 #pragma unroll
         for (int r = 0; r < HR; ++r) {
           const u32x4 w = *reinterpret_cast<const u32x4*>(slab + ((h + r) * RP + qr) * SLD + qc);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[r][e] = fmaf(__uint_as_float(w[e]) * s[r], scale[e], bias[e]);
+          for (int e = 0; e < 4; ++e) v[r][e] = __uint_as_float(w[e]);
+        }
+        if (__builtin_expect(far, 0)) {
+#pragma unroll
+          for (int r = 0; r < HR; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[r][e] = scaled(v[r][e], s[r], scale[e], bias[e]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < HR; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[r][e] = fmaf(v[r][e] * s[r], scale[e], bias[e]);
         }
         activate_all<HR * 4>(&v[0][0], p.act);
         if (p.residual) {
@@ -645,7 +669,7 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void i8_tiles(I8Args p, unsigned
       float v[4], res[4] = {0.f, 0.f, 0.f, 0.f};
       if (p.residual && quad && live) Quad<T>::load(static_cast<const T*>(p.residual) + row * p.ldr + col, res);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(__uint_as_float(w[e]) * s, scale[e], bias[e]);
+      for (int e = 0; e < 4; ++e) v[e] = scaled(__uint_as_float(w[e]), s, scale[e], bias[e]);
       activate_all<4>(v, p.act);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] += res[e];

@@ -923,3 +923,42 @@ def test_quantize_rows_at_the_small_end(cuda, cols, dtype):
     y = ops.linear_i8(x[:m].to(cuda), w, out_dtype=F32)
     assert torch.equal(y, ops.matmul_i8(ops.quantize_rows(x[:m].to(cuda)), w))
     check_product(y, *product64(q[:m], scale[:m], w.codes.cpu(), w.scale.cpu(), None, "none", None), F32)
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 21, 70), (40, 33, 130), (70, 400, 130), (3000, 1030, 70), (700, 4000, 200), (3000, 4100, 200), (20000, 64, 50)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_product_of_far_scales(cuda, m, n, k, dtype):
+  """Scales whose product is ordinary: the sum times either of them alone can pass float32's range, or fall below it."""
+  g = torch.Generator().manual_seed(m + n)
+  qa = torch.randint(-127, 128, (m, k), generator=g, dtype=torch.int8)
+  qb = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8)
+  qa[0], qb[0] = 127, 127
+  e = torch.tensor([-110.0, 0.0, 64.0, 120.0])[torch.randint(0, 4, (m,), generator=g)]
+  sb = (torch.rand(n, generator=g) + 0.5) * 2.0 ** -110
+  bias, residual = rnd(1, n).float(), rnd(2, m, n).to(dtype)
+  for sign in (1, -1):
+    e[0] = 120.0
+    sa = (torch.rand(m, generator=g) + 0.5) * torch.exp2(sign * e)
+    st = sb if sign == 1 else 1 / sb
+    a, b = ops.Int8Rows.from_codes(qa.to(cuda), sa.to(cuda)), ops.Int8Rows.from_codes(qb.to(cuda), st.to(cuda))
+    want, bound = product64(qa, sa, qb, st, bias, "leaky", residual)
+    assert want.abs().max() < 1e38 or sign == -1
+    got = ops.matmul_i8(a, b, bias=bias.to(cuda), act="leaky", residual=residual.to(cuda), out_dtype=dtype)
+    top = torch.finfo(dtype).max
+    # a float32 holds the product before the activation: -1.5 max is an infinity, though leaky would bring it back to -0.15 max
+    before = (qa.double() @ qb.double().t().contiguous()) * sa.double()[:, None] * st.double()[None, :]
+    fin = (want.abs() < top * 0.99) & (before.abs() < torch.finfo(F32).max * 0.99)
+    assert torch.isinf(got.cpu()[(want.abs() > top * 1.01) | (before.abs() > torch.finfo(F32).max * 1.01)]).all()
+    check_product(got[fin.to(cuda)], want[fin], bound[fin] + 2.0 ** -148, dtype)
+
+
+def test_linear_i8_of_rows_near_the_end_of_float32(cuda):
+  """Rows of 1e36 and more with weights that bring them back: one launch, two launches, tiles."""
+  k, n = 200, 300
+  w = ops.quantize_rows((rnd(2, n, k) * 1e-30).float().to(cuda))
+  for m in (2, 40, 3000):
+    x = (rnd(m, m, k).clamp(-3, 3) * 1e38).float()
+    x[1::2] *= 1e-35
+    got = ops.linear_i8(x.to(cuda), w)
+    q, s = quant64(x)
+    check_product(got, *product64(q, s, w.codes.cpu(), w.scale.cpu(), None, "none", None), F32)
