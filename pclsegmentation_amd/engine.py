@@ -244,12 +244,11 @@ def torch_device(index=0):
 
 
 def stream_handle(device):
-  """Raw hipStream_t of torch's current stream on ``device`` (what pclseg_set_stream takes)."""
+  """Raw hipStream_t of torch's current stream on ``device``, in any form torch takes (what pclseg_set_stream takes)."""
   import torch
-  index = getattr(device, "index", None)
-  if index is None:
-    return torch.cuda.current_stream(device).cuda_stream
-  return torch._C._cuda_getCurrentRawStream(index)      # the same handle without a Stream object: 0.1 us instead of 1.9
+  if type(device) is torch.device and device.index is not None and device.type == "cuda":
+    return torch._C._cuda_getCurrentRawStream(device.index)      # the same handle without a Stream object: 0.1 us instead of 1.9
+  return torch.cuda.current_stream(device).cuda_stream
 
 
 def on_device(x):

@@ -962,3 +962,10 @@ def test_linear_i8_of_rows_near_the_end_of_float32(cuda):
     got = ops.linear_i8(x.to(cuda), w)
     q, s = quant64(x)
     check_product(got, *product64(q, s, w.codes.cpu(), w.scale.cpu(), None, "none", None), F32)
+
+
+def test_stream_handle_of_the_current_stream(cuda):
+  from pclsegmentation_amd import engine as E
+  side = torch.cuda.Stream(cuda)
+  with torch.cuda.stream(side):
+    assert {E.stream_handle(d) for d in ("cuda:0", "cuda", 0, None, torch.device("cuda"), torch.device("cuda", 0))} == {side.cuda_stream}

@@ -371,3 +371,27 @@ def test_shipped_kernels_are_the_set_verified_on_an_mi355x():
   assert not new and not changed, "kernels that never ran on an MI355X in the shipped build: new %s changed %s" % (new[:3], changed[:3])
   # and the candidate switch really changes kernels (the manifest check is not vacuous)
   assert any(k not in want["kernels"] or cand[k] != want["kernels"][k] for k in cand)
+
+
+def test_stream_handle_takes_a_device_in_any_form(monkeypatch):
+  """A device with an index goes straight to its handle; names, numbers, None and a device without an index go to
+  torch.cuda.current_stream as they are (a str has an `index` too: a method), and what it refuses is refused."""
+  import torch
+
+  class Stream:
+    def __init__(self, handle):
+      self.cuda_stream = handle
+
+  def current_stream(device=None):
+    if isinstance(device, torch.device) and device.type != "cuda":
+      raise ValueError("Expected a cuda device")
+    return Stream(("stream", device))
+  monkeypatch.setattr(torch.cuda, "current_stream", current_stream)
+  monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: ("raw", int(index)), raising=False)
+  assert E.stream_handle(torch.device("cuda", 1)) == ("raw", 1)
+  assert E.stream_handle(torch.device("cuda:0")) == ("raw", 0)
+  for device in ("cuda:0", "cuda", 1, None, torch.device("cuda")):
+    assert E.stream_handle(device) == ("stream", device)
+  for device in (torch.device("cpu"), torch.device("cpu", 0)):
+    with pytest.raises(ValueError):
+      E.stream_handle(device)
