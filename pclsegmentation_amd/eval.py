@@ -151,13 +151,14 @@ def evaluation(arg):
     raise SystemExit("no scans under %s" % os.path.join(arg.data_path, arg.image_set))
   none_index = config.CLASSES.index("None")
   miou_tracker = MeanIoU(num_classes=config.NUM_CLASS, name="MeanIoU")
-  likelihood = LabelLikelihood(config.NUM_CLASS, none_index, device=model.device) if arg.likelihood else None
+  wanted = bool(getattr(arg, "likelihood", False))      # a caller's own namespace need not have it
+  likelihood = LabelLikelihood(config.NUM_CLASS, none_index, device=model.device) if wanted else None
   print("Performing Evaluation")
   import torch
   dev = _engine.torch_device(model.device)
   for b0 in range(0, len(files), arg.batch):
     samples = torch.from_numpy(np.stack([np.load(f).astype(np.float32) for f in files[b0:b0 + arg.batch]])).to(dev)
-    out = model.predict_raw(samples[..., :5], return_mask=True, return_logits=arg.likelihood)       # device tensors
+    out = model.predict_raw(samples[..., :5], return_mask=True, return_logits=wanted)       # device tensors
     predictions, mask = out[0], out[1]
     label = masked_labels(samples, mask, none_index)
     miou_tracker.update_state(label, predictions)

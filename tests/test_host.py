@@ -395,3 +395,44 @@ def test_stream_handle_takes_a_device_in_any_form(monkeypatch):
   for device in (torch.device("cpu"), torch.device("cpu", 0)):
     with pytest.raises(ValueError):
       E.stream_handle(device)
+
+
+def test_evaluation_takes_a_namespace_without_likelihood(monkeypatch, tmp_path, capsys):
+  """evaluation(arg) with the reference's own flags alone: the network and the counting replaced by host stand-ins."""
+  import types
+
+  import torch
+
+  from pclsegmentation_amd import eval as ev
+  classes = ["Car", "None"]
+
+  class Model:
+    device = 0
+
+    def init_weights(self, seed):
+      pass
+
+    def predict_raw(self, scans, return_mask=False, return_logits=False):
+      assert return_mask and not return_logits
+      shape = scans.shape[:3]
+      return torch.zeros(shape, dtype=torch.int32), torch.ones(shape, dtype=torch.uint8)
+
+  class Counts:
+    ignored, total_cm = 0, np.array([[4, 0], [0, 4]])
+
+    def __init__(self, num_classes, name):
+      pass
+
+    def update_state(self, label, predictions):
+      assert label.shape == predictions.shape
+
+    def result(self):
+      return 1.0
+  monkeypatch.setattr(ev, "load_model_config", lambda m, n: (types.SimpleNamespace(CLASSES=classes, NUM_CLASS=2), Model()))
+  monkeypatch.setattr(ev, "MeanIoU", Counts)
+  monkeypatch.setattr(E, "torch_device", lambda index=0: torch.device("cpu"))
+  (tmp_path / "val").mkdir()
+  np.save(str(tmp_path / "val" / "s.npy"), np.zeros((2, 4, 6)))
+  arg = types.SimpleNamespace(path_to_model=None, model="squeezesegv2", config="squeezesegv2", data_path=str(tmp_path), image_set="val", batch=1)
+  assert ev.evaluation(arg)[3] == 1.0
+  assert "NLL" not in capsys.readouterr().out
