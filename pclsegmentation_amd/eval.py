@@ -110,11 +110,16 @@ class LabelLikelihood:
     self._sums.zero_()
 
   def update_state(self, label, logits):
-    """label [...], logits [..., num_classes]: host arrays or device tensors."""
+    """label [...], logits [..., num_classes]: host arrays or device tensors of any number type (logits that are not float32,
+    bfloat16 or float16 are taken as float32)."""
     import torch
     from . import ops as _ops
-    lab = torch.as_tensor(np.asarray(label) if not hasattr(label, "is_cuda") else label).to(self._dev, dtype=torch.int32)
+    lab = torch.as_tensor(np.asarray(label) if not hasattr(label, "is_cuda") else label).to(self._dev)
+    if lab.dtype != torch.int32:
+      lab = lab.to(torch.int64)      # not to fewer bits: 2^32 is no label, and would become class 0
     x = torch.as_tensor(np.asarray(logits) if not hasattr(logits, "is_cuda") else logits).to(self._dev)
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+      x = x.float()
     if x.shape[-1:] != (self.num_classes,) or lab.shape != x.shape[:-1]:
       raise ValueError("labels %s do not match logits %s of %d classes" % (tuple(lab.shape), tuple(x.shape), self.num_classes))
     counted = (lab >= 0) & (lab < self.num_classes)

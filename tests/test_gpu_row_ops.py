@@ -969,3 +969,18 @@ def test_stream_handle_of_the_current_stream(cuda):
   side = torch.cuda.Stream(cuda)
   with torch.cuda.stream(side):
     assert {E.stream_handle(d) for d in ("cuda:0", "cuda", 0, None, torch.device("cuda"), torch.device("cuda", 0))} == {side.cuda_stream}
+
+
+def test_label_likelihood_of_any_number_type(cuda):
+  """NumPy's own float64 logits and int64 labels; labels that only differ from a class above bit 31 are none."""
+  from pclsegmentation_amd import eval as ev
+  logits = (rnd(1, 40, 7) * 3).float()
+  label = torch.randint(0, 7, (40,), generator=torch.Generator().manual_seed(3))
+  far = torch.cat([label, label[:5] + 2 ** 32, label[:5] - 2 ** 40])
+  want = ev.LabelLikelihood(7, 6)
+  want.update_state(label, logits)
+  for lab, x in ((label.numpy(), logits.double().numpy()), (label.double().numpy(), logits.double()), (label.to(torch.int16), logits),
+                 (far, torch.cat([logits, logits[:10]])), (far.to(cuda), torch.cat([logits, logits[:10]]).double().to(cuda))):
+    got = ev.LabelLikelihood(7, 6)
+    got.update_state(lab, x)
+    assert got.result() == want.result()
