@@ -243,12 +243,18 @@ def torch_device(index=0):
   return torch.device("cuda", int(index))
 
 
+_DEVICE_INDEX = {}      # torch.device of a GPU -> its index
+
+
 def stream_handle(device):
   """Raw hipStream_t of torch's current stream on ``device``, in any form torch takes (what pclseg_set_stream takes)."""
   import torch
-  if type(device) is torch.device and device.index is not None and device.type == "cuda":
-    return torch._C._cuda_getCurrentRawStream(device.index)      # the same handle without a Stream object: 0.1 us instead of 1.9
-  return torch.cuda.current_stream(device).cuda_stream
+  index = _DEVICE_INDEX.get(device)
+  if index is None:
+    if not isinstance(device, torch.device) or device.type != "cuda" or device.index is None:
+      return torch.cuda.current_stream(device).cuda_stream
+    index = _DEVICE_INDEX[device] = device.index
+  return torch._C._cuda_getCurrentRawStream(index)      # the same handle without a Stream object: 0.1 us instead of 1.9
 
 
 def on_device(x):
