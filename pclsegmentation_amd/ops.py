@@ -10,9 +10,12 @@ A 1x1 convolution of NHWC activations is linear_i8 on their last axis (``Int8Row
 logits of a model go into label_logprobs as they are, [..., classes].  Tensors are float32, bfloat16 or float16 on one MI355X;
 rows may have any stride as long as their elements are adjacent (others are copied).  Calls are asynchronous on torch's current
 stream of the tensors' device, allocate their outputs and workspace through torch and keep nothing, so they can be captured
-into a graph.  Like the rest of the package they compute outside of autograd.  All arithmetic is in libpclseg.so."""
+into a graph.  Like the rest of the package they compute outside of autograd: results carry no history, and a call that is
+given a tensor that requires a gradient while gradients are recorded warns of it.  All arithmetic is in libpclseg.so."""
 import ctypes
 import functools
+import sys
+import warnings
 from collections import namedtuple
 
 import torch
@@ -39,6 +42,13 @@ def _dtype(t, name):
 def _on(t, dev, name):
   if not isinstance(t, torch.Tensor) or (t.device != dev if dev is not None else not _engine.on_device(t)):
     _fail("%s must be a tensor on %s" % (name, dev or "the device"))
+  if t.requires_grad and torch.is_grad_enabled():
+    depth = 1
+    while sys._getframe(depth).f_globals is globals():      # to the caller's line
+      depth += 1
+    warnings.warn("pclseg: %s requires a gradient, but the row operators compute outside of autograd and none flows back to it (call "
+                  "them under torch.no_grad() or on detached tensors; label_logprobs_grad is the gradient of label_logprobs)" % name,
+                  stacklevel=depth + 1)
 
 
 def _rows(t, cols):

@@ -984,3 +984,11 @@ def test_label_likelihood_of_any_number_type(cuda):
     got = ev.LabelLikelihood(7, 6)
     got.update_state(lab, x)
     assert got.result() == want.result()
+
+
+def test_a_call_that_drops_a_gradient_runs_and_warns(cuda):
+  x = rnd(1, 5, 40).float().to(cuda).requires_grad_()
+  w = ops.quantize_rows(rnd(2, 7, 40).float().to(cuda))
+  with pytest.warns(UserWarning, match="outside of autograd"):
+    y = ops.linear_i8(x, w)
+  assert not y.requires_grad and torch.equal(y, ops.linear_i8(x.detach(), w))

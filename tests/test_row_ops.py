@@ -325,3 +325,25 @@ def test_python_layer_refuses_log_probabilities_without_names(host_as_device):
                lambda: ops.label_logprobs_grad(x, i, v, entropy=v, d_entropy=v, top_ids=ids, top_logprobs=two[:, :1])):
     with pytest.raises(ValueError):
       call()
+
+
+def test_inputs_that_require_a_gradient_are_warned_of(host_as_device, recwarn):
+  """Results carry no history: a call that would drop a gradient says so, and nothing is said where none is recorded.  (Each call
+  is refused for something else afterwards, so that none is launched.)"""
+  x, p, i = torch.zeros(2, 8), torch.zeros(2, 8, requires_grad=True), torch.zeros(3, dtype=torch.int32)
+  b = torch.zeros(4, requires_grad=True)
+  calls = [("x", lambda t: ops.quantize_rows(t.double())), ("x", lambda t: ops.linear_i8(t, _rows8(k=9))),
+           ("logits", lambda t: ops.label_logprobs(t, i)), ("logits", lambda t: ops.label_logprobs_grad(t, i, x[:, 0]))]
+  for name, call in calls:
+    with pytest.warns(UserWarning, match=name + " requires a gradient, but") as seen, pytest.raises(ValueError):
+      call(p)
+    assert seen[0].filename == __file__
+    with torch.no_grad(), pytest.raises(ValueError):
+      call(p)
+    for quiet in (x, p.detach()):
+      with pytest.raises(ValueError):
+        call(quiet)
+  for call in (lambda: ops.linear_i8(x, _rows8(), bias=b), lambda: ops.matmul_i8(_rows8(), _rows8(), bias=b)):
+    with pytest.warns(UserWarning, match="outside of autograd"), pytest.raises(ValueError):
+      call()
+  assert not recwarn.list
