@@ -7,7 +7,8 @@ SRCS  := $(CSRC)/pclseg_kernels.h $(CSRC)/pclseg_graph.h $(CSRC)/pclseg_api.hip 
 # sha256 over the sources (in the order bench.py's csrc_sha() reads them) FOLLOWED BY the build's -D switches, baked into
 # the library (pclseg_build_sha): bench.py compares it with the sources next to it and refuses to quote a PMC traffic
 # figure when the binary that ran was built from something else.  The shipped build has no switches, so its hash is the
-# hash of the sources alone; every stamps / tuning / variant build hashes differently and is never mistaken for it.
+# hash of the forward pass's sources alone; every stamps / tuning / variant build hashes differently and is never mistaken
+# for it.  The row operators have a hash of their own (pclseg_ops_build_sha, ops_sha below).
 sha = $(shell (cat $(SRCS); printf '%s' '$(strip $(1))') | sha256sum | cut -c1-16)
 # the row operators (include/pclseg.h, second half) are a translation unit of their own: the forward pass's device kernels
 # stay the instruction streams that tests/golden/verified_kernels_r03.json names.  Packed float32 instructions are off in it
@@ -16,6 +17,8 @@ OPS_SRCS := $(CSRC)/pclseg_ops.hip $(CSRC)/pclseg_rows.h $(CSRC)/pclseg_score.h 
 OPS_OBJ := build/pclseg_ops.o
 OPS_FLAGS := -Xclang -target-feature -Xclang -packed-fp32-ops
 HIPFLAGS := -O3 -std=c++17 --offload-arch=$(ARCH) -fPIC -Wall -Wno-unused-function
+# sha256 over the row operators' sources, then the flags they are compiled with
+ops_sha = $(shell (cat $(OPS_SRCS); printf '%s' '$(strip $(HIPFLAGS) $(OPS_FLAGS))') | sha256sum | cut -c1-16)
 # $(call hipbuild,<output>,<-D switches>)
 define hipbuild
 $(HIPCC) $(HIPFLAGS) $(2) -DPCLSEG_SRC_SHA=\"$(call sha,$(2))\" -c -o build/$(notdir $(1:.so=.o)) $(CSRC)/pclseg_api.hip
@@ -26,7 +29,7 @@ all: $(LIB)
 
 $(OPS_OBJ): $(OPS_SRCS)
 	@mkdir -p build
-	$(HIPCC) $(HIPFLAGS) $(OPS_FLAGS) -c -o $@ $(CSRC)/pclseg_ops.hip
+	$(HIPCC) $(HIPFLAGS) $(OPS_FLAGS) -DPCLSEG_OPS_SHA=\"$(ops_sha)\" -c -o $@ $(CSRC)/pclseg_ops.hip
 
 $(LIB): $(SRCS) $(CSRC)/pclseg_status.h $(OPS_OBJ)
 	$(call hipbuild,$@,$(EXTRA))
@@ -58,8 +61,12 @@ variant: $(SRCS) $(OPS_OBJ)
 carry: all
 	python3 scripts/carry_traffic.py profiles/r03_traffic.json ad2e081 profiles/r06_traffic.json $(wildcard profiles/r03_*_kernel_stats.csv)
 
+# the hash that a library built from the sources as they are would carry (tests/test_host.py)
+ops-sha:
+	@echo $(ops_sha)
+
 clean:
 	rm -f $(LIB) pclsegmentation_amd/libpclseg_*.so
 	rm -rf build sim/_build
 
-.PHONY: all clean stamps tuning variant candidates carry
+.PHONY: all clean ops-sha stamps tuning variant candidates carry

@@ -337,6 +337,10 @@ int pclseg_op_project_ex(const pclseg_proj_desc* desc, const float* points, int 
  * the current device, handle-less, asynchronous on `hip_stream` (NULL = default stream); nothing is allocated, kept or
  * synchronised, so every call can be captured into a graph.  Rows have unit element stride and any row stride; element
  * alignment is enough.  A count of rows of 0 is no work and succeeds. */
+
+/* First 16 digits of the sha256 over the row operators' sources and compiler flags (pclseg_build_sha covers the forward pass). */
+const char* pclseg_ops_build_sha(void);
+
 typedef enum pclseg_dtype { PCLSEG_F32 = 0, PCLSEG_BF16 = 1, PCLSEG_F16 = 2 } pclseg_dtype;
 
 #define PCLSEG_TOP_MAX 64      /* alternatives a row can be asked for */

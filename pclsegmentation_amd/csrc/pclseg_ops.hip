@@ -414,8 +414,15 @@ int pclseg_op_label_logprobs_grad(const void* logits, int dtype, int64_t rows, i
 
 }  // extern "C"
 
-// ---- the same with what the forward pass knew of the names
+#ifndef PCLSEG_OPS_SHA
+#define PCLSEG_OPS_SHA "unknown"
+#endif
+
 extern "C" {
+
+const char* pclseg_ops_build_sha(void) { return PCLSEG_OPS_SHA; }
+
+// the gradient with what the forward pass knew of the names
 
 int pclseg_op_label_logprobs_grad_ex(const void* logits, int dtype, int64_t rows, int64_t classes, int64_t stride,
                                      const void* labels, int label_bytes, const uint8_t* allowed, int64_t allowed_stride,

@@ -43,7 +43,7 @@ EXPORTS = [
   "pclseg_op_confusion_matrix", "pclseg_op_project", "pclseg_op_project_ex", "pclseg_op_split_f16_roundtrip",
   "pclseg_i8_row_bytes", "pclseg_op_quantize_rows", "pclseg_op_matmul_i8", "pclseg_op_linear_i8_workspace",
   "pclseg_op_linear_i8", "pclseg_op_label_logprobs_workspace", "pclseg_op_label_logprobs", "pclseg_op_label_logprobs_grad",
-  "pclseg_op_label_logprobs_grad_ex",
+  "pclseg_op_label_logprobs_grad_ex", "pclseg_ops_build_sha",
 ]
 
 
@@ -154,10 +154,12 @@ def load_library():
                                                    vp, i64, vp]
   for name in EXPORTS:
     fn = getattr(lib, name)
-    if name not in ("pclseg_last_error", "pclseg_host_alloc", "pclseg_build_sha", "pclseg_i8_row_bytes"):
+    if name not in ("pclseg_last_error", "pclseg_host_alloc", "pclseg_build_sha", "pclseg_ops_build_sha", "pclseg_i8_row_bytes"):
       fn.restype = ctypes.c_int
   lib.pclseg_host_alloc.restype = ctypes.c_void_p
   lib.pclseg_build_sha.restype = ctypes.c_char_p
+  lib.pclseg_ops_build_sha.argtypes = []
+  lib.pclseg_ops_build_sha.restype = ctypes.c_char_p
   lib.pclseg_i8_row_bytes.restype = ctypes.c_int64
   _lib = lib
   return lib
@@ -166,6 +168,11 @@ def load_library():
 def build_sha():
   """Source hash baked into the loaded binary (Makefile -DPCLSEG_SRC_SHA), "unknown" for a foreign build."""
   return load_library().pclseg_build_sha().decode()
+
+
+def ops_build_sha():
+  """The same of the row operators: their sources and compiler flags (Makefile ops_sha)."""
+  return load_library().pclseg_ops_build_sha().decode()
 
 
 def _raise(rc, handle=None):

@@ -436,3 +436,28 @@ def test_evaluation_takes_a_namespace_without_likelihood(monkeypatch, tmp_path, 
   arg = types.SimpleNamespace(path_to_model=None, model="squeezesegv2", config="squeezesegv2", data_path=str(tmp_path), image_set="val", batch=1)
   assert ev.evaluation(arg)[3] == 1.0
   assert "NLL" not in capsys.readouterr().out
+
+
+def test_binary_carries_the_hash_of_its_row_operators():
+  """A library with row kernels of other sources or flags is told from this tree's; the hash covers every file that their
+  translation unit includes, and its flags."""
+  import hashlib
+  import subprocess
+  make = open(os.path.join(ROOT, "Makefile")).read()
+  value = lambda name: re.search(r"^%s +[:?]?= (.*)$" % name, make, re.M).group(1).replace("$(CSRC)", "pclsegmentation_amd/csrc").replace("$(ARCH)", "gfx950")
+  files = value("OPS_SRCS").split()
+  csrc = os.path.join(ROOT, "pclsegmentation_amd", "csrc")
+  todo, included = ["pclseg_ops.hip"], set()
+  while todo:
+    for inc in re.findall(r'^#include "([^"]+)"', open(os.path.join(csrc, todo.pop())).read(), re.M):
+      path = os.path.normpath(os.path.join("pclsegmentation_amd/csrc", inc))
+      if path not in included:
+        included.add(path)
+        todo.append(os.path.relpath(os.path.join(ROOT, path), csrc))
+  assert set(files) == included | {"pclsegmentation_amd/csrc/pclseg_ops.hip"}
+  h = hashlib.sha256()
+  for f in files:
+    h.update(open(os.path.join(ROOT, f), "rb").read())
+  h.update((value("HIPFLAGS") + " " + value("OPS_FLAGS")).encode())
+  assert E.ops_build_sha() == h.hexdigest()[:16]
+  assert subprocess.check_output(["make", "-s", "-C", ROOT, "ops-sha"], text=True).strip() == E.ops_build_sha()
