@@ -992,3 +992,25 @@ def test_a_call_that_drops_a_gradient_runs_and_warns(cuda):
   with pytest.warns(UserWarning, match="outside of autograd"):
     y = ops.linear_i8(x, w)
   assert not y.requires_grad and torch.equal(y, ops.linear_i8(x.detach(), w))
+
+
+@pytest.mark.parametrize("m,n,k", [(9001, 3001, 640), (9000, 3000, 640), (4090, 4091, 200), (8192, 2048, 384)])
+@pytest.mark.parametrize("act", ["none", "relu", "leaky", "sigmoid"])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_tiles_with_their_epilogue(cuda, m, n, k, act, dtype):
+  """256x256 tiles, inside and at both edges, with bias, activation and residual together (reference on the device in float64,
+  whose products of integers are exact)."""
+  g = torch.Generator(device=cuda).manual_seed(m + n)
+  qa = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8, device=cuda)
+  qb = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8, device=cuda)
+  sa, sb = torch.rand(m, generator=g, device=cuda) * 1e-2 + 1e-4, torch.rand(n, generator=g, device=cuda) * 1e-2 / k ** 0.5 + 1e-6
+  bias = torch.randn(n, generator=g, device=cuda)
+  wide = torch.randn(m, n + 5, generator=g, device=cuda).to(dtype)
+  residual = wide[:, 2:2 + n]
+  got = ops.matmul_i8(ops.Int8Rows.from_codes(qa, sa), ops.Int8Rows.from_codes(qb, sb), bias=bias, act=act, residual=residual, out_dtype=dtype)
+  p = (qa.double() @ qb.double().t().contiguous()) * sa.double()[:, None] * sb.double()[None, :]
+  v = p + bias.double()
+  want = ACT64[act](v) + residual.double()
+  bound = 4 * U * p.abs() + 2 * U * v.abs() + (8 * U if act == "sigmoid" else 0.0) + U * want.abs()
+  bound = bound + half_step(dtype) * (want.abs() + bound) + tiny(dtype)
+  assert got.dtype == dtype and ((got.double() - want).abs() - bound).max() <= 0
