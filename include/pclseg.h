@@ -367,7 +367,8 @@ int pclseg_op_matmul_i8(const int8_t* a, const float* a_scale, const int8_t* b, 
                         int64_t n, int64_t k, const float* bias, int act, const void* residual, int64_t residual_stride,
                         void* y, int64_t y_stride, int dtype, void* hip_stream);
 
-/* The layer on float rows: op_quantize_rows of x into the workspace, then op_matmul_i8 (a few rows: one launch, no workspace).
+/* The layer on float rows: op_quantize_rows of x into the workspace, then op_matmul_i8 (few rows of a few
+ * thousand channels, or one or two long ones: one launch, no workspace).
  *   x      [m, k] dtype, does not overlap y (refused; rows side by side in one buffer do not overlap); weight codes and scales
  *          as for b above
  *   workspace  pclseg_op_linear_i8_workspace bytes (may be 0), 16-byte aligned; two calls in flight need two */

@@ -318,8 +318,9 @@ __global__ __launch_bounds__(NW * 64) void i8_few_rows(I8Args p) {
 }
 
 // ---- up to 32 short rows: quantisation and product in one launch
-// Every block quantises all rows again (from the L2) while its first weights are on their way, where a launch of its own
-// costs 3 us on the device and as much on the host.  The rows are cut into items of 512 elements, eight a lane; a wave takes
+// Every block quantises all rows again (from the L2), where a launch and a workspace of their own cost 3.5 us of a pass.
+// Its first weights are requested before the rows; loads come back in order, so the maximum waits for both and the weights are
+// there when the codes are.  The rows are cut into items of 512 elements, eight a lane; a wave takes
 // up to eight items and holds them in registers between the maximum and the codes.  Codes and scales stay in LDS.  MT tiles
 // of 16 rows share a weight fragment.
 constexpr int kFusedRows = 32, kFusedItems = 64;

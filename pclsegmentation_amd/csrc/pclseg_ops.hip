@@ -136,10 +136,20 @@ int matmul(Launch go, const I8Args& p, int dtype) {
   return go.rc;
 }
 
-// up to 32 rows of together 64 items of 512 elements: one launch, no workspace (see i8_fused_rows)
-bool fused_rows(int64_t m, int64_t k) { return m <= kFusedRows && m * ((row_bytes(k) + 511) / 512) <= kFusedItems; }
-size_t linear_workspace(int64_t m, int64_t k) {
-  return fused_rows(m, k) ? 0 : (size_t)m * ((size_t)row_bytes(k) + sizeof(float));
+// Up to 32 rows of together 64 items of 512 elements in one launch, no workspace (see i8_fused_rows): every block of 16 channels
+// quantises all rows, which saves a launch and a workspace (3.5 us of a pass, 13 us with two) and costs with the blocks.  A
+// pass of bf16 rows, one launch / two: up to 512 blocks, two a CU, and 2^14 items quantised in all
+//   1x1024 -> 8192   9.5 / 13.0   16x1024 -> 8192  10.9 / 13.2   32x1024 -> 4096  11.7 / 13.1     (one launch)
+//   1x1024 -> 32768 19.5 / 12.6    8x4096 -> 8192  15.5 / 12.8   32x1024 -> 8192  16.5 / 13.2   32x1024 -> 131072 180 / 53
+// and one or two rows of 4096 columns and more for any n: a block's 64 KB of weights take longer than its items
+//   1x4096 -> 131072  92 / 111     2x4096 -> 131072 102 / 113     4x4096 -> 32768  34.8 / 31.6 (two launches).
+bool fused_rows(int64_t m, int64_t n, int64_t k) {
+  const int64_t items = m * ((row_bytes(k) + 511) / 512), blocks = (n + 15) / 16;
+  if (m > kFusedRows || items > kFusedItems) return false;
+  return (m <= 2 && k >= 4096) || (blocks <= 512 && items * blocks <= 1 << 14);
+}
+size_t linear_workspace(int64_t m, int64_t n, int64_t k) {
+  return fused_rows(m, n, k) ? 0 : (size_t)m * ((size_t)row_bytes(k) + sizeof(float));
 }
 
 int check_product(const char* op, int64_t m, int64_t n, int64_t k, const int8_t* b, const float* b_scale, int act,
@@ -323,7 +333,7 @@ int pclseg_op_linear_i8_workspace(int64_t m, int64_t n, int64_t k, size_t* bytes
   const char* op = "op_linear_i8_workspace";
   if (!bytes) return bad(op, "bytes is NULL");
   if (m < 0 || m > kMaxBlocks || n < 1 || !row_bytes(k)) return bad_shape(op, "m must be in [0, 2^31), n positive, k in [1, 131071]");
-  *bytes = linear_workspace(m, k);
+  *bytes = linear_workspace(m, n, k);
   return PCLSEG_OK;
 } OP_CATCH
 
@@ -344,7 +354,7 @@ int pclseg_op_linear_i8(const void* x, int dtype, int64_t x_stride, const int8_t
   // few rows in one launch: every block reads all of x while others store y.  Refused for any number of rows alike, after the
   // checks of sizes
   const bool shared = overlap({x, x_stride, k, (int64_t)dtype_size(dtype)}, {y, y_stride, n, (int64_t)dtype_size(y_dtype)}, m);
-  if (fused_rows(m, k)) {
+  if (fused_rows(m, n, k)) {
     I8Args p{nullptr, weight, nullptr, weight_scale, ld, ld, m, (int)n, (int)ld, bias, act, residual, residual_stride, y, y_stride};
     go.dry = shared;
     with_type(dtype, [&](auto t) {
@@ -359,7 +369,7 @@ int pclseg_op_linear_i8(const void* x, int dtype, int64_t x_stride, const int8_t
     });
     return go.rc ? go.rc : shared ? bad(op, "y overlaps x") : PCLSEG_OK;
   }
-  if (!workspace || workspace_bytes < linear_workspace(m, k)) return bad(op, "workspace too small");
+  if (!workspace || workspace_bytes < linear_workspace(m, n, k)) return bad(op, "workspace too small");
   if (!aligned(workspace, 16)) return bad(op, "misaligned workspace");
   int8_t* q = static_cast<int8_t*>(workspace);
   float* scale = reinterpret_cast<float*>(q + m * ld);

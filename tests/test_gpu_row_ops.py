@@ -1014,3 +1014,17 @@ def test_large_tiles_with_their_epilogue(cuda, m, n, k, act, dtype):
   bound = 4 * U * p.abs() + 2 * U * v.abs() + (8 * U if act == "sigmoid" else 0.0) + U * want.abs()
   bound = bound + half_step(dtype) * (want.abs() + bound) + tiny(dtype)
   assert got.dtype == dtype and ((got.double() - want).abs() - bound).max() <= 0
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 1000, 8192), (1, 1000, 8193), (2, 4096, 20000), (3, 4096, 20000), (8, 4096, 4096), (8, 4096, 4097),
+                                   (17, 500, 8192), (17, 500, 8200), (32, 1024, 4097), (32, 64, 30001)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_linear_i8_few_rows_of_many_channels(cuda, m, k, n, dtype):
+  """Both sides of the rule for one launch or two."""
+  x, w = rnd(m, m, k).to(dtype), ops.quantize_rows((rnd(3, n, k) * 0.05).float().to(cuda))
+  bias, residual = rnd(4, n).float(), rnd(5, m, n).to(dtype)
+  got = ops.linear_i8(x.to(cuda), w, bias=bias.to(cuda), act="relu", residual=residual.to(cuda))
+  assert torch.equal(got, ops.matmul_i8(ops.quantize_rows(x.to(cuda)), w, bias=bias.to(cuda), act="relu", residual=residual.to(cuda),
+                                        out_dtype=dtype))
+  q, s = quant64(x)
+  check_product(got, *product64(q, s, w.codes.cpu(), w.scale.cpu(), bias, "relu", residual), dtype)

@@ -347,3 +347,17 @@ def test_inputs_that_require_a_gradient_are_warned_of(host_as_device, recwarn):
     with pytest.warns(UserWarning, match="outside of autograd"), pytest.raises(ValueError):
       call()
   assert not recwarn.list
+
+
+def test_workspace_of_few_rows_goes_by_the_channels_too():
+  """One launch (no workspace) quantises every row in every block of 16 channels: not beyond 512 blocks or 2^14 items of 512
+  elements in all, but for one or two rows of 4096 columns and more."""
+  lib, size = E.load_library(), ctypes.c_size_t()
+
+  def need(m, n, k):
+    assert lib.pclseg_op_linear_i8_workspace(m, n, k, ctypes.byref(size)) == 0
+    return size.value
+  for m, n, k in ((1, 8192, 1024), (16, 8192, 1024), (32, 4096, 1024), (8, 4096, 4096), (1, 1 << 20, 4096), (2, 131072, 16384)):
+    assert need(m, n, k) == 0
+  for m, n, k in ((1, 8193, 1024), (16, 8193, 1024), (32, 4097, 1024), (8, 4097, 4096), (1, 1 << 20, 4095), (3, 16384, 4096), (33, 16, 16)):
+    assert need(m, n, k) == m * (lib.pclseg_i8_row_bytes(k) + 4)
