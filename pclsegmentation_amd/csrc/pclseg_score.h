@@ -147,9 +147,10 @@ __device__ __forceinline__ void load_tail(const T* row, const uint8_t* mask, int
 
 // ---- V <= 32: a thread owns a row
 // CAP = classes rounded up to whole 16 bytes: only the last of the row's pieces can be cut.  A row of 20 floats is 80 bytes:
-// the 16-byte loads of a wave touch 40 lines, five times over, all of them in the L1 after the first.
+// the 16-byte loads of a wave touch 40 lines, five times over, all of them in the L1 after the first.  Four blocks a CU: with
+// six, 20 classes take the same (2097152 rows, float32: 39.7 us) and 24 or 32 spill (45 -> 59, 69 -> 143 us).
 template <typename T, int CAP, bool MASK>
-__global__ __launch_bounds__(256, CAP <= 20 ? 6 : 4) void logprob_thread_rows(ScoreArgs a) {
+__global__ __launch_bounds__(256, 4) void logprob_thread_rows(ScoreArgs a) {
   constexpr int VEC = Elem<T>::VEC, NV = CAP / VEC;
   const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (row >= a.rows) return;
