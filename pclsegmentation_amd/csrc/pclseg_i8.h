@@ -150,7 +150,8 @@ template <typename T> struct Eight {
   }
 };
 
-// Bound by memory: 8192 x 4096 bf16 in 17.8 us, 131072 x 512 float32 in 52 us (5.6 and 6.4 TB/s of what is read and written).
+// Bound by memory: 8192 x 4096 bf16 in 16.4 us, 131072 x 512 float32 in 56 us (one call after the other; 6.1 and 6.0 TB/s of
+// what is read and written).
 // G lanes own a row, each 8 elements of every stretch of 8 G; four stretches are kept in registers, so a row of up to 32 G
 // elements is read once.  Longer rows (REREAD) are read twice, the second time from the L2.  A row with an infinity or a
 // NaN gets the scale NaN and codes 0: its outputs are NaN, like those of a float32 product.
@@ -233,7 +234,8 @@ struct I8Args {
 
 __device__ __forceinline__ float relu(float v) { return v > 0.f ? v : (v != v ? v : 0.f); }
 __device__ __forceinline__ float leaky(float v) { return v > 0.f ? v : 0.1f * v; }
-// v_exp_f32 and v_rcp_f32, one unit in the last place each: within 4 * 2^-24 of the sigmoid, whose slope is 1/4
+// v_exp_f32 and v_rcp_f32, one unit in the last place each: within 4 * 2^-24 of the sigmoid, whose slope is 1/4.  Far below 0 the
+// error is |v| 2^-24 of the value, by the rounding of the exponent
 __device__ __forceinline__ float sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
 }
@@ -486,8 +488,9 @@ template <int N> __device__ __forceinline__ void activate_all(float* v, int act)
   }
 }
 
-// Measured (product alone): 8192x4096 -> 8192 bf16 250 us (2.2 PFLOP/s, the matrix pipes busy 59 % of the time at the 1.8 GHz
-// that the power limit leaves), 131072x512 -> 1024 float32 150 us (4 TB/s), 8192x1024 -> 512 float32 with residual 12.5 us.
+// Measured (the product alone, one call after the other): 8192x4096 -> 8192 bf16 235 us (2.3 PFLOP/s; 271 under a profiler, where the
+// matrix pipes were busy 59 % of the time at the 1.8 GHz that the power limit leaves), 131072x512 -> 1024 float32 138 us (4.4 TB/s),
+// 8192x1024 -> 512 float32 with residual 10.2 us.
 // The loop: a step's fragments are read from LDS one 32-byte slice of k ahead of the matrix instructions that use them, and
 // the barrier that hands a buffer over lies before the step's last slice, whose fragments are already in registers: the first
 // reads of the next tile run under those matrix instructions.

@@ -116,15 +116,17 @@ int matmul(Launch go, const I8Args& p, int dtype) {
       else go.run(i8_few_rows<T, 4, 8>, cols, rows, 512, 0, p);
       return;
     }
-    // The largest tile that fills the 256 CUs: 8192x8192x4096 takes 301 us with 256x256 tiles, 302 with 128x128, 435 with
-    // 64x64; 8192x512x1024 17.3 / 9.6 / 10.6 us; 512x4096x4096 44 / 20.6 / 18.0 us.  Between the first two the rounds decide,
-    // in units of a CU's time for a 128x128 tile: one 256x256 tile a CU costs 4, two 128x128 tiles 2 and 5 % more
-    // (15642x1260x2235 with its quantisation: 114 us in two rounds of 256x256, 1.2 of them needed, 101 in three of 128x128).
+    // The largest tile that fills the 256 CUs.  m x n x k, the product alone, one call after the other: 8192x8192x4096 bf16
+    // 290 us with 256x256 tiles, 303 with 128x128, 426 with 64x64; 8192x512x1024 float32 17.5 / 9.5 / 10.5 us; 512x4096x4096
+    // 44 / 20.6 / 18.0 us.  Between the first two the rounds decide, in units of a CU's time for a 128x128 tile: one 256x256 tile
+    // a CU costs 4, two 128x128 tiles 2 and 5 % more (15642x1260x2235 float32 with its quantisation, ten calls in a graph:
+    // 116 us in two rounds of 256x256, 1.2 of them needed, 97 in three of 128x128).
     // Up to 256 columns of many rows a tile is mostly stores: 128x128 with steps of 64 bytes, three of them on a CU, one
-    // storing while the others multiply, from 16 tiles a CU on (linear of 131072x512 float32: k = 128 78 us against 88 with
-    // 256x256, k = 256 109 against 117; 8192x2048 bf16, k = 256, four tiles a CU: 24.5 against 21.7; 131072x1024 float32,
-    // k = 512: 271 against 255).  Up to 64 channels nothing wider than they are (131072x64x128: 8.5 us against 13.4 with
-    // 128x128; the linear of 131072x64 bf16 from k = 50: 23 against 33).
+    // storing while the others multiply, from 16 tiles a CU on (with the quantisation, ten in a graph: 131072x512x128 float32
+    // 68 us against 78 with 256x256, 131072x512x256 89 against 97; the product 8192x2048x256 bf16, four tiles a CU: 24.5
+    // against 21.7; 131072x1024x512 float32: 206 against 205, and 286 against 276 with the caches flushed before each call).
+    // Up to 64 channels nothing wider than they are (the product 131072x64x128: 8.4 us against 14.1 with 128x128; with the
+    // quantisation and flushed caches 131072x64x50 bf16: 23 against 33).
     const int64_t big = (tiles(256, 256) + 255) / 256 * 4 * 20, mid = (tiles(128, 128) + 511) / 512 * 2 * 21;
     if (p.n <= 64 && p.kp == 64) launch_tiles<T, 128, 64, 64, 2, 2, 4>(p, go);
     else if (p.n <= 64) launch_tiles<T, 64, 64, 128, 2, 2, 4>(p, go);
@@ -175,7 +177,8 @@ constexpr int kThreadRow = 32, kGroupRow = 2048, kPiece = 2048, kRounds = 4, kMa
 constexpr int kSortRows = 8192, kOneLaunch = 16, kFewWaves = 4;       // pieces one block of 16 waves takes, pieces that 4 waves are enough for
 
 // blocks a row is cut into: one up to 32768 classes (a piece for each of 16 waves) and from 32 rows on; else as many as keep
-// few rows from waiting on few CUs (one row of 131072: 20 us in one block, 6.9 + 4.3 in 16 and a second launch that joins them)
+// few rows from waiting on few CUs (one row of 131072 with 20 alternatives: 22 us in one block, 12 in 16 and a second
+// launch that joins them)
 int score_segs(int64_t rows, int64_t classes) {
   const int64_t pieces = (classes + kPiece - 1) / kPiece;
   if (pieces <= kOneLaunch || rows >= 32) return 1;

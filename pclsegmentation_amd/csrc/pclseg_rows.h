@@ -51,8 +51,9 @@ template <typename T> __device__ __forceinline__ u32x4 load16(const T* p) {
   return *reinterpret_cast<const typename Elem<T>::Pack*>(p);
 }
 // Outputs that are written once and read by a later kernel pass the caches by: the lines they would push out are worth more
-// than those a reader would find (131072x512 -> 1024 float32 with its quantisation 258 -> 181 us, a layer, its log
-// probabilities and their gradient 539 -> 489 us; also where the output would fit: 8192x1024 -> 2048 bf16 54.9 -> 51.8 us).
+// than those a reader would find (ten passes of the same inputs in a graph: 131072x512 -> 1024 float32 with its
+// quantisation 271 -> 205 us, a layer, its log probabilities and their gradient 553 -> 505 us; also where the output would fit:
+// 8192x1024 -> 2048 bf16 34.7 -> 33.4 us.  The gradient of 4096x50001 bf16 by itself loses by it, 156 -> 160 us).
 template <typename T> __device__ __forceinline__ void stream16(T* p, const u32x4& v) {
   typedef typename Elem<T>::Pack Pack;
   __builtin_nontemporal_store((Pack)v, reinterpret_cast<Pack*>(p));

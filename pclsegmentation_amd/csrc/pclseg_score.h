@@ -10,7 +10,8 @@
 // a long row's pieces are added with the rounding of each addition carried into the next, so that a sum is a few tens of
 // roundings from the exact one, 2^-24 each, whatever the row's length (131072 terms one after the other, most of them
 // alike: 450 roundings off).
-// The exponential is v_exp_f32 on (x-M) log2 e: both roundings are relative to an exponent of at most a few tens.
+// The exponential is v_exp_f32 on (x-M) log2 e: the rounding of that product makes an error of |x-M| 2^-24 of the term, which
+// weighs e^(x-M) (4096 x 50001 bf16: 5.3e-8 from the exact values all in all).
 // Terms with x - M < -200 are 0 in float32; the clamp of the second factor at -200 keeps 0 * inf out of T.
 //
 // Three kernels, by the length of a row (what a row costs besides its elements is what differs):
@@ -18,8 +19,8 @@
 //   logprob_group_rows    V <= 2048  8, 16, 32 or 64 lanes own a row, held in registers; a short top list by rounds of argmax
 //   logprob_wave_rows     longer     a wave, the waves of a block, or several blocks stream a row in pieces of 2048 elements;
 //                                    a long top list as one sorted key per lane
-// What they reach: 4194304 x 20 float32 with 3 alternatives 118 us (503 MB, 4.3 TB/s), 4096 x 50001 bf16 with 8 alternatives
-// 99 us and without 78 us (410 MB, 5.2 TB/s), 333 x 1031 f16 with 32 alternatives 8.7 us.
+// What they reach, one call after the other: 4194304 x 20 float32 with 3 alternatives 112 us (503 MB, 4.5 TB/s), 4096 x 50001 bf16
+// with 8 alternatives 87 us and without 81 us (410 MB, 5.1 TB/s), 333 x 1031 f16 with 32 alternatives 8.2 us.
 #ifndef PCLSEG_SCORE_H_
 #define PCLSEG_SCORE_H_
 
@@ -393,7 +394,7 @@ __global__ __launch_bounds__(NW * 64) void logprob_wave_rows(ScoreArgs a) {
   const T* src = static_cast<const T*>(a.x) + row * a.stride;
   const uint8_t* mask = MASK ? a.allowed + row * a.allowed_stride : nullptr;
   // pieces begin at multiples of 16 bytes, `pad` elements before the row's first: rows of an odd length read at the rate of
-  // the others (4096 x 50001 bf16 without a top list 93 us unaligned, 78 aligned)
+  // the others (4096 x 50001 bf16 without a top list, when it was built: 93 us unaligned, 78 aligned)
   const int pad = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));
   const int pieces = (int)(((int64_t)a.classes + pad + PIECE - 1) / PIECE);
   const int p0 = (int)((int64_t)pieces * seg / a.segs), p1 = (int)((int64_t)pieces * (seg + 1) / a.segs);
