@@ -5,11 +5,11 @@
 //   lse = M + ln S,   logprob = (x[label] - M) - ln S,   entropy = ln S - T / S
 // (M, S, T) of two disjoint parts join with M = max(M1, M2), d = Mi - M <= 0:  S += Si e^d, T += e^d (Ti + d Si), so a row
 // is read once and can be cut anywhere.  Rows are often decided: S = 1 + rest with a rest of 2^-10 would leave ln S 14 bits.
-// The maximum's term is kept apart from the others (one, s below), and ln S = ln(1 + rest) keeps the bits of the rest.  All of it is float32: the terms of S and T have one sign, and the differences x - M are
-// taken before the exponential, so large logits lose nothing.  A lane adds up to 32 elements one after the other; such sums of
-// a long row's pieces are added with the rounding of each addition carried into the next, so that a sum is a few tens of
-// roundings from the exact one, 2^-24 each, whatever the row's length (131072 terms one after the other, most of them
-// alike: 450 roundings off).
+// The maximum's term is kept apart from the others (one, s below), and ln S = ln(1 + rest) keeps the bits of the rest.
+// All of it is float32: the terms of S and T have one sign, and the differences x - M are taken before the exponential, so large
+// logits lose nothing.  A lane adds up to 32 elements one after the other; such sums of a long row's pieces are added with the
+// rounding of each addition carried into the next, so that a sum is a few tens of roundings from the exact one, 2^-24 each,
+// whatever the row's length (131072 terms one after the other, most of them alike: 450 roundings off).
 // The exponential is v_exp_f32 on (x-M) log2 e: the rounding of that product makes an error of |x-M| 2^-24 of the term, which
 // weighs e^(x-M) (4096 x 50001 bf16: 5.3e-8 from the exact values all in all).
 // Terms with x - M < -200 are 0 in float32; the clamp of the second factor at -200 keeps 0 * inf out of T.
