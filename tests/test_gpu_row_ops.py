@@ -1028,3 +1028,60 @@ def test_linear_i8_few_rows_of_many_channels(cuda, m, k, n, dtype):
                                         out_dtype=dtype))
   q, s = quant64(x)
   check_product(got, *product64(q, s, w.codes.cpu(), w.scale.cpu(), bias, "relu", residual), dtype)
+
+
+@pytest.mark.parametrize("v", [33, 40, 257, 500, 1031, 2048])
+@pytest.mark.parametrize("top_k", [0, 1, 4])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_label_logprobs_odd_rows_and_masks_of_short_lists(cuda, v, top_k, dtype):
+  """Short lists of rows of middle length: equal logits, the lowest value throughout, all -inf, outliers, NaN, +inf, rows with
+  nothing, one or a few allowed, excluded classes that hold anything, rows behind a block's last."""
+  lo, hi = torch.finfo(dtype).min, torch.finfo(dtype).max
+  j = torch.arange(v)
+  rows = [torch.full((v,), 1.5), j * (8.0 / v), -j * (8.0 / v), torch.full((v,), lo), torch.full((v,), -math.inf), torch.zeros(v),
+          torch.where(j == v // 2, 1e4, 0.0), torch.where(j == 1, lo, 0.5), torch.full((v,), hi), torch.where(j == v - 1, math.nan, 1.0),
+          torch.where(j == 0, math.inf, 1.0), torch.where(j % 3 == 1, -math.inf, 2.0), torch.where(j == v - 1, 1.0, -math.inf)]
+  x = torch.stack([r.double() for r in rows] + list(rnd(v, 28, v) * 2)).to(dtype)
+  x[5, ::2] = -0.0
+  labels = (torch.arange(len(x)) * 7 % v).to(torch.int32)
+  got = ops.label_logprobs(x.to(cuda), labels.to(cuda), top_k=top_k)
+  ref = score64(x, labels, max(top_k, 1), None)
+  if not top_k:
+    ref["top_ids"] = ref["top_logprobs"] = None
+  check_score(got, ref, v, top_k)
+  g = torch.Generator().manual_seed(v)
+  allowed = torch.rand((len(x), v), generator=g) < 0.6
+  allowed[13] = False
+  allowed[14] = j == v - 1
+  allowed[15] = j < 2
+  allowed[16] = j == 0
+  fill = torch.tensor([math.nan, math.inf, -math.inf, lo, hi])
+  x = torch.where(allowed, x, fill[torch.randint(0, 5, x.shape, generator=g)].to(dtype))
+  for mask in (allowed, allowed[20]):
+    full = mask.expand(len(x), v)
+    y = torch.where(full, x, fill[torch.randint(0, 5, x.shape, generator=g)].to(dtype)) if mask.dim() == 1 else x
+    got = ops.label_logprobs(y.to(cuda), labels.to(cuda), top_k=top_k, allowed=mask.to(cuda))
+    check_score(got, score64(y, labels, max(top_k, 1), full), v, top_k)
+
+
+@pytest.mark.parametrize("m,v", [(1, 40000), (70, 1000), (300, 20)])
+def test_gradient_with_log_probabilities_captured_and_replayed(cuda, m, v):
+  """The pass and its gradient with the kept log probabilities in a graph on a stream of its own, with new logits for every replay."""
+  def both(x, labels, d):
+    f = ops.label_logprobs(x, labels, top_k=2)
+    return tuple(f) + (ops.label_logprobs_grad(x, labels, f.lse, d_logprob=d, entropy=f.entropy, d_entropy=d, top_ids=f.top_ids,
+                                               logprob=f.logprob, top_logprobs=f.top_logprobs),)
+  x, labels, d = rnd(1, m, v).float().to(cuda), labels_for(m, v, 2).to(cuda), rnd(3, m).float().to(cuda)
+  both(x, labels, d)
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph, stream=torch.cuda.Stream(cuda)):
+    out = both(x, labels, d)
+  for it in range(4):
+    x.copy_((rnd(10 + it, m, v) * 4).float())
+    x[:, it] += 25.0 * (it % 2)
+    want = both(x, labels, d)
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
